@@ -1,0 +1,98 @@
+/* Operators of a batch whose requests share a prompt prefix, bring low-rank adapters of their own and put controls on their
+ * logits (shared_prefix.cu, lora.cu, logit_controls.cu). Functions return 0, or a negative code when the arguments are outside
+ * what the kernels cover (nothing was launched then) or a launch failed (-100 - cudaError_t). */
+#ifndef XPOOL_REQUEST_API_H_
+#define XPOOL_REQUEST_API_H_
+
+#include <stdint.h>
+
+#include "xpool/api.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Decode attention of rows that share prefixes. A piece is a range of a prefix and the consecutive rows that read it together;
+ * every piece of a row leaves a partial result, to which the row's own tokens are added. */
+typedef struct XpPrefixPiece {
+  int leader;                 /* row whose block table names the prefix's pages */
+  int row0, rows;             /* rows of the piece */
+  int tok0, tok1;             /* tokens [tok0, tok1) of the sequence, tok0 a multiple of 64, tok1 of 16 */
+  int part;                   /* index of the partial result of these rows */
+  int pad0, pad1;
+} XpPrefixPiece;
+
+typedef struct XpDecodeSharedArgs {
+  XpDecodeAttnArgs a;         /* ws: partial sums [batch, q_heads, max_parts + own, head_dim], behind them (maximum, sum) pairs
+                                 [batch, q_heads, max_parts + own, 2]; own = num_splits when that is > 1, otherwise 0 */
+  const XpPrefixPiece* pieces;
+  const int* n_pieces;        /* device word */
+  const int* row_prefix;      /* [plan_rows] tokens that a row shares (a multiple of 16); a row of fewer tokens reads all on its own */
+  const int* row_parts;       /* [plan_rows] pieces of the row */
+  int max_pieces;             /* bound of *n_pieces */
+  int max_parts;              /* bound of row_parts */
+  int plan_rows;              /* rows behind these share nothing */
+  int reserved;
+} XpDecodeSharedArgs;
+int xp_decode_shared(const XpDecodeSharedArgs* a, void* stream);
+
+/* out[r] = y[r] + scale[s] B[s] (A[s] x[r]) with s the adapter slot of row r (none: out[r] = y[r]). A projection may have several
+ * parts, each with its own A and its own features: A's rows and the ranks lie part after part. */
+#define XP_LORA_PARTS 4
+typedef struct XpLoraItem {
+  int slot;                   /* adapter, or -1: rows without one */
+  int first, rows;            /* rows perm[first .. first + rows) */
+  int pad;
+} XpLoraItem;
+
+typedef struct XpLoraArgs {
+  const void* x;              /* bf16 [rows, ldx] */
+  const void* y;              /* bf16 [rows, ld_y] */
+  void* out;                  /* bf16 [rows, ld_out]; may be y */
+  const void* a;              /* bf16 [slots, parts, rank, k] */
+  const void* b;              /* bf16 [slots, n, rank] */
+  const float* scale;         /* [slots] */
+  const int* ranks;           /* [slots] rank in use, rounded up to 16; what lies behind it is zero */
+  const XpLoraItem* items;
+  const int* n_items;         /* device word */
+  const int* perm;            /* [rows] */
+  int rows, k, n, rank, parts, slots, max_items;
+  int ldx, ld_y, ld_out;
+  int part_end[XP_LORA_PARTS]; /* features [0, part_end[0]) are part 0, and so on; multiples of 8 */
+} XpLoraArgs;
+int xp_lora(const XpLoraArgs* a, void* stream);
+
+/* Controls on logits; every array may be null. Order: repetition, frequency, presence, bias, mask. */
+typedef struct XpLogitControls {
+  const int* history;         /* [history_slots, ld_history] tokens; ids outside the vocabulary count for nothing */
+  const int* history_rows;    /* [rows] slot of a row (null: row r is slot r) */
+  const int* lens;            /* [rows] tokens in the history */
+  const int* prompt_lens;     /* [rows] how many of them are the prompt's (null: none) */
+  const int* latest;          /* [rows] the last of the `lens` tokens, not stored yet: the call stores it (null: all are stored) */
+  const float* repetition;    /* [rows] a token that occurred: logit > 0 divided by it, others multiplied */
+  const float* frequency;     /* [rows] subtracted once for every occurrence behind the prompt */
+  const float* presence;      /* [rows] subtracted once if there is any */
+  const int* bias_ids;        /* [bias_total] rows one after the other: entries [bias_starts[r], bias_starts[r + 1]) */
+  const float* bias_values;
+  const int* bias_starts;     /* [rows + 1] */
+  const uint32_t* masks;      /* [mask_count, ld_mask] bit i % 32 of word i / 32: token i is allowed */
+  const int* mask_index;      /* [rows] mask of a row, outside [0, mask_count): none */
+  int history_slots, history_cap, ld_history, bias_total, mask_count, ld_mask;
+} XpLogitControls;
+
+typedef struct XpLogitArgs {
+  XpLogitControls c;
+  const void* logits;         /* [rows, ld] bf16 or fp32 */
+  void* out;                  /* adjusted logits [rows, ld_out], bf16 or fp32; null: tokens are selected instead */
+  const float* temps;         /* [rows] temperature (null or <= 0: the largest logit, ties to the lower id) */
+  const uint32_t* seeds;      /* [rows, 2] */
+  int* tokens;                /* [rows] */
+  float* values;              /* [rows] optional: the adjusted logit of the selected token */
+  int rows, vocab, ld, ld_out, f32, out_f32;
+} XpLogitArgs;
+int xp_logit_controls(const XpLogitArgs* a, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* XPOOL_REQUEST_API_H_ */

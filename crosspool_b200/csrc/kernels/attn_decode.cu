@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "xpool/api.h"
+#include "xpool/request_api.h"
 #include "xpool/sm100.cuh"
 #include "xpool/tensormap.hpp"
 #include "xpool/pdl.cuh"
@@ -282,6 +283,9 @@ decode_attn_kernel(XpDecodeAttnArgs a) {
 //
 // kSig: weights are sigmoids of the scores (no maximum, no sum), and the tiles may begin with the means of the blocks behind the
 // window, which come from a paged cache of their own in two boxes of eight rows.
+//
+// XpDecodeSharedArgs: the first tokens of a row belong to a prefix that shared_prefix.cu has multiplied for all rows that share
+// it. The kernel reads what lies behind them and adds the prefix's partial results when it finishes a head.
 constexpr int kTcStages = 3;
 
 __device__ __forceinline__ void tma_load_kv(uint32_t dst, const CUtensorMap* m, uint32_t bar, int d0, int head, int token) {
@@ -320,6 +324,45 @@ __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t packe
 
 __device__ __forceinline__ const XpDecodeAttnArgs& base_of(const XpDecodeRowsArgs& a) { return a.a; }
 __device__ __forceinline__ const XpDecodeAttnArgs& base_of(const XpDecodeAttnArgs& a) { return a; }
+__device__ __forceinline__ const XpDecodeAttnArgs& base_of(const XpDecodeSharedArgs& a) { return a.a; }
+
+template <typename A>
+constexpr bool kIsShared = std::is_same<A, XpDecodeSharedArgs>::value;
+
+// Partial results of a row of a shared prefix: sums of head hq and slot i, and their (maximum, sum of weights) pair.
+struct Partials {
+  float* sums;
+  float* pairs;
+  int slots;
+  template <int D>
+  static __device__ __forceinline__ Partials of(const XpDecodeSharedArgs& s, int b, int hq) {
+    const int slots = s.max_parts + (s.a.num_splits > 1 ? s.a.num_splits : 0);
+    const size_t all = static_cast<size_t>(s.a.batch) * s.a.q_heads * slots, at = (static_cast<size_t>(b) * s.a.q_heads + hq) * slots;
+    return {s.a.ws + at * D, s.a.ws + all * D + at * 2, slots};
+  }
+};
+// Tokens that row b shares: none where it has fewer than the prefix.
+__device__ __forceinline__ int shared_tokens(const XpDecodeSharedArgs& s, int b) {
+  const int p = b < s.plan_rows ? s.row_prefix[b] : 0;
+  return s.a.seq_lens[b] >= p ? p : 0;
+}
+// Tokens of a slice of a row's own: the plan's, or more where a row has more of them than its slices cover.
+__device__ __forceinline__ int own_chunk(int chunk_tokens, int nsplit, int own) {
+  return max(chunk_tokens, ((own + nsplit - 1) / nsplit + 15) & ~15);
+}
+// Adds slots [i0, i1) to (av, ll, mm): weighted sum of element d, sum of weights, maximum.
+template <int D>
+__device__ __forceinline__ void add_partials(const Partials& p, int i0, int i1, int d, float& av, float& ll, float& mm) {
+  float top = mm;
+  for (int i = i0; i < i1; ++i) top = fmaxf(top, p.pairs[2 * i]);
+  const float c = mm == -CUDART_INF_F ? 0.f : exp2f(mm - top);
+  av *= c, ll *= c, mm = top;
+  for (int i = i0; i < i1; ++i) {
+    const float m = p.pairs[2 * i], w = m == -CUDART_INF_F ? 0.f : exp2f(m - top);
+    ll += p.pairs[2 * i + 1] * w;
+    av += p.sums[static_cast<size_t>(i) * D + d] * w;
+  }
+}
 
 // What a row reads of its sequence: tokens [0, head) and [head + skip, len + skip), head and skip whole 16-token tiles. `len`
 // counts both; lo is the first token of the window. With pooled blocks the first `blocks` of [0, head) are those.
@@ -340,6 +383,9 @@ __device__ __forceinline__ Span row_span(const A& args, int b) {
       s.skip = (s.lo & ~15) - s.head;
       s.len -= s.skip;
     }
+  } else if constexpr (kIsShared<A>) {
+    s.skip = shared_tokens(args, b);
+    s.len = args.a.seq_lens[b] - s.skip;
   } else {
     s.len = args.seq_lens[b];
   }
@@ -357,7 +403,8 @@ __device__ __forceinline__ void store_out(const A& args, int b, int hq, int d, f
     }
     reinterpret_cast<__nv_bfloat16*>(args.a.out)[static_cast<size_t>(b) * args.ld_out + hq * args.v_valid + d] = __float2bfloat16_rn(v);
   } else {
-    reinterpret_cast<__nv_bfloat16*>(args.out)[(static_cast<size_t>(b) * args.q_heads + hq) * DV + d] = __float2bfloat16_rn(v);
+    const XpDecodeAttnArgs& a = base_of(args);
+    reinterpret_cast<__nv_bfloat16*>(a.out)[(static_cast<size_t>(b) * a.q_heads + hq) * DV + d] = __float2bfloat16_rn(v);
   }
 }
 
@@ -402,6 +449,7 @@ decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     chunk = (len + nsplit - 1) / nsplit;
     chunk = (chunk + 15) & ~15;
   }
+  if constexpr (kIsShared<A>) chunk = own_chunk(chunk, nsplit, len);
   const int t0 = split * chunk;
   const int t1 = min(len, t0 + chunk);
   if (a.chunk_tokens > 0 && nsplit > 1 && t0 >= len) return;  // the merge kernel skips this slice
@@ -681,6 +729,8 @@ decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     }
   }
   __syncthreads();
+  int parts = 0;
+  if constexpr (kIsShared<A>) parts = span.skip > 0 ? args.row_parts[b] : 0;
   for (int i = threadIdx.x; i < G * DV; i += kDecodeThreads) {
     const int gg = i / DV, d = i % DV;
     float mm = -CUDART_INF_F;
@@ -695,7 +745,17 @@ decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       av += rw[d] * c;
     }
     const int hq = hk * G + gg;
-    if (nsplit == 1) {
+    if constexpr (kIsShared<A>) {
+      const Partials p = Partials::of<DV>(args, b, hq);
+      if (nsplit == 1) {
+        add_partials<DV>(p, 0, parts, d, av, ll, mm);
+        store_out<DV>(args, b, hq, d, ll > 0.f ? av / ll : 0.f);
+      } else {
+        const int i = args.max_parts + split;
+        p.sums[static_cast<size_t>(i) * DV + d] = av;
+        if (d == 0) p.pairs[2 * i] = mm, p.pairs[2 * i + 1] = ll;
+      }
+    } else if (nsplit == 1) {
       store_out<DV>(args, b, hq, d, finish_out<kSig>(args, hq, av, ll, mm));
     } else {
       float* ws = a.ws + ((static_cast<size_t>(b) * a.q_heads + hq) * nsplit + split) * (DV + 2);
@@ -706,6 +766,23 @@ decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       }
     }
   }
+}
+
+// Prefix pieces and slices of a row's own tokens.
+template <int D>
+__global__ void shared_combine_kernel(XpDecodeSharedArgs args, int nsplit) {
+  pdl::wait();
+  pdl::release_short();
+  const XpDecodeAttnArgs& a = args.a;
+  const int hq = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
+  const int shared = shared_tokens(args, b), own = a.seq_lens[b] - shared;
+  const int chunk = own_chunk(a.chunk_tokens, nsplit, own);
+  nsplit = min(nsplit, (own + chunk - 1) / chunk);                                            // slices that ran
+  const Partials p = Partials::of<D>(args, b, hq);
+  float av = 0.f, ll = 0.f, mm = -CUDART_INF_F;
+  add_partials<D>(p, 0, shared > 0 ? args.row_parts[b] : 0, d, av, ll, mm);
+  add_partials<D>(p, args.max_parts, args.max_parts + nsplit, d, av, ll, mm);
+  reinterpret_cast<__nv_bfloat16*>(a.out)[(static_cast<size_t>(b) * a.q_heads + hq) * D + d] = __float2bfloat16_rn(ll > 0.f ? av / ll : 0.f);
 }
 
 template <int D, bool kSig = false, typename A>
@@ -771,7 +848,11 @@ static int launch_decode_tc(const A& args, int nsplit, cudaStream_t s) {
   }
   dim3 grid(nsplit, a.kv_heads, a.batch);
   pdl::launch(decode_attn_tc_kernel<DQ, DV, A, kSig>, grid, kDecodeThreads, kSmem, s, 1, mk, mv, mkp, mvp, args);
-  if (nsplit > 1) pdl::launch(decode_combine_kernel<DV, kSig, A>, dim3(a.q_heads, a.batch), DV, 0, s, 1, args, nsplit);
+  if constexpr (std::is_same<A, XpDecodeSharedArgs>::value) {
+    if (nsplit > 1) pdl::launch(shared_combine_kernel<DV>, dim3(a.q_heads, a.batch), DV, 0, s, 1, args, nsplit);
+  } else {
+    if (nsplit > 1) pdl::launch(decode_combine_kernel<DV, kSig, A>, dim3(a.q_heads, a.batch), DV, 0, s, 1, args, nsplit);
+  }
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -100 - static_cast<int>(e);
 }
@@ -840,4 +921,25 @@ extern "C" int xp_decode_rows(const XpDecodeRowsArgs* r, void* stream) {
   if (a->head_dim == 128 && r->v_dim == 128) return launch_decode_tc<128, 128>(*r, nsplit, s);
   if (a->head_dim == 192 && r->v_dim == 128) return launch_decode_tc<192, 128>(*r, nsplit, s);
   return -13;
+}
+
+extern "C" int xp_shared_prefix_pieces(const XpDecodeSharedArgs* a, void* stream);   // shared_prefix.cu
+
+extern "C" int xp_decode_shared(const XpDecodeSharedArgs* r, void* stream) {
+  using namespace xpool::attn;
+  const XpDecodeAttnArgs* a = &r->a;
+  if (a->batch <= 0) return 0;
+  if (a->kv_heads <= 0 || a->q_heads % a->kv_heads != 0) return -10;
+  const int nsplit = a->num_splits > 0 ? a->num_splits : 1;
+  if ((r->max_parts > 0 || nsplit > 1) && a->ws == nullptr) return -11;
+  if (a->q_heads / a->kv_heads > 16 || a->num_pages <= 0 || a->page_size < 16 || (a->page_size & (a->page_size - 1)) != 0 ||
+      a->chunk_tokens % 16 != 0 || (reinterpret_cast<uintptr_t>(a->q) & 15) != 0 || a->batch > 65535)
+    return -12;
+  if (a->head_dim != 64 && a->head_dim != 128) return -13;
+  if (r->max_pieces > 0) {
+    const int rc = xp_shared_prefix_pieces(r, stream);
+    if (rc != 0) return rc;
+  }
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return a->head_dim == 128 ? launch_decode_tc<128, 128>(*r, nsplit, s) : launch_decode_tc<64, 64>(*r, nsplit, s);
 }

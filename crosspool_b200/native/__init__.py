@@ -11,6 +11,7 @@ operators in :mod:`crosspool_b200.ops` have no eager substitute on the hot path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 from pathlib import Path
@@ -178,6 +179,16 @@ def check(rc: int, what: str, kernels_launched: int = 1) -> None:
     _launches += kernels_launched
 
 
+def on_device(device):
+    """Context in which ``device`` is the current one (kernels are launched on the current device)."""
+    import torch
+
+    return _HERE if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
+
+
 def launch_count() -> int:
     """Kernels of this library launched (or captured into a graph) so far by this process."""
     return _launches
@@ -253,6 +264,11 @@ class DecodeRowsArgs(C.Structure):
     ]
 
 
+class DecodeSharedArgs(C.Structure):
+    _fields_ = [("a", DecodeAttnArgs), ("pieces", C.c_void_p), ("n_pieces", C.c_void_p), ("row_prefix", C.c_void_p), ("row_parts", C.c_void_p),
+                ("max_pieces", C.c_int), ("max_parts", C.c_int), ("plan_rows", C.c_int), ("reserved", C.c_int)]
+
+
 class PrefillAttnArgs(C.Structure):
     _fields_ = [
         ("q", C.c_void_p),
@@ -299,10 +315,18 @@ class PrefillAttnArgs(C.Structure):
 def _struct(name: str, doc: str, **fields):
     """A ctypes.Structure whose fields are given as ``ctype="space separated names"`` groups in ABI order, keyed
     ``group_index_ctype``."""
-    types = {"ptr": C.c_void_p, "int": C.c_int, "float": C.c_float, "ptr8": C.c_void_p * 8, "ptr2": C.c_void_p * 2, "int2": C.c_int * 2}
+    types = {"ptr": C.c_void_p, "int": C.c_int, "float": C.c_float, "ptr8": C.c_void_p * 8, "ptr2": C.c_void_p * 2, "int2": C.c_int * 2, "int4": C.c_int * 4}
     decl = [(n, types[key.split("_", 1)[1]]) for key, names in fields.items() for n in names.split()]
     return type(name, (C.Structure,), {"_fields_": decl, "__doc__": doc})
 
+
+# request_api.h
+LoraArgs = _struct("LoraArgs", "XpLoraArgs", a_ptr="x y out a b scale ranks items n_items perm",
+                   b_int="rows k n rank parts slots max_items ldx ld_y ld_out", c_int4="part_end")
+LogitArgs = _struct("LogitArgs", "XpLogitArgs (its controls first)",
+                    a_ptr="history history_rows lens prompt_lens latest repetition frequency presence bias_ids bias_values bias_starts masks mask_index",
+                    b_int="history_slots history_cap ld_history bias_total mask_count ld_mask", c_ptr="logits out temps seeds tokens values",
+                    d_int="rows vocab ld ld_out f32 out_f32")
 
 # mixer_api.h
 ResidNormArgs = _struct("ResidNormArgs", "XpResidNormArgs", a_ptr="resid", b_ptr8="parts",
@@ -382,6 +406,9 @@ def _declare_attention(lib: C.CDLL) -> None:
     lib.xp_decode_attn.argtypes = [C.POINTER(DecodeAttnArgs), C.c_void_p]
     lib.xp_decode_rows.restype = C.c_int
     lib.xp_decode_rows.argtypes = [C.POINTER(DecodeRowsArgs), C.c_void_p]
+    for fn, args in (("xp_decode_shared", DecodeSharedArgs), ("xp_lora", LoraArgs), ("xp_logit_controls", LogitArgs)):
+        getattr(lib, fn).restype = C.c_int
+        getattr(lib, fn).argtypes = [C.POINTER(args), C.c_void_p]
     lib.xp_prefill_attn.argtypes = [C.POINTER(PrefillAttnArgs), C.c_void_p]
     lib.xp_decode_attn_splits.argtypes = [C.c_int, C.c_int, C.c_int]
     lib.xp_embedding.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]

@@ -9,7 +9,9 @@ from __future__ import annotations
 import ctypes as C
 import os
 import math
+from typing import Sequence
 
+import numpy as np
 import torch
 
 from .. import native
@@ -111,6 +113,184 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     a.status = status_words(q.device).data_ptr()
     native.check(native.kernels().xp_decode_attn(C.byref(a), _stream(q.device)), "xp_decode_attn",
                  2 if num_splits > 1 else 1)
+    return out
+
+
+# ---------------------------------------------------------------------------------------------- shared prefixes
+
+PREFIX_TOKENS = 16      # prefixes are shared in whole tiles of so many tokens; the rest of one is read by every row
+PIECE_TOKENS = 64       # pieces of a prefix begin at multiples of this
+
+
+def piece_rows(q_heads: int, kv_heads: int) -> int:
+    """Rows that one piece of a prefix may hold: two tiles of 128 query heads of a KV head."""
+    return 2 * (128 // (q_heads // kv_heads))
+
+
+def prefix_piece_tokens(groups: Sequence[tuple[int, int]], kv_heads: int, rows_per_piece: int, num_sms: int = 148) -> int:
+    """Tokens of a prefix that a CTA takes at once, for ``groups`` of (rows, prefix tokens): the split that fills the SMs with the
+    least time of the slowest one. A piece costs as long as about 128 more tokens take (its queries, the first copies, its result)."""
+    tiles = [(-(-n // rows_per_piece), p) for n, p in groups]
+    best, best_cost = PIECE_TOKENS, None
+    longest = max(p for _, p in tiles)
+    c = PIECE_TOKENS
+    while True:
+        units = kv_heads * sum(t * -(-p // c) for t, p in tiles)
+        parts = -(-longest // c)
+        cost = -(-units // num_sms) * (min(c, longest) + 128) + 8 * parts
+        if best_cost is None or cost < best_cost:
+            best, best_cost = c, cost
+        if c >= longest:
+            return best
+        c += max(PIECE_TOKENS, c // 4 // PIECE_TOKENS * PIECE_TOKENS)
+
+
+def shared_plan_words(rows: int, max_pieces: int) -> int:
+    """32-bit words of a plan for up to ``rows`` rows and ``max_pieces`` pieces."""
+    return 4 + 8 * max_pieces + 2 * rows
+
+
+def fill_shared_plan(sizes: Sequence[int], prefixes: Sequence[int], words: np.ndarray, rows: int, max_pieces: int, max_parts: int, *,
+                     q_heads: int, kv_heads: int) -> tuple[int, int]:
+    """Writes the plan of consecutive groups of rows (``sizes``) with ``prefixes`` tokens shared in each to ``words``; returns its
+    number of pieces and the most pieces of a row. Prefixes are cut so that neither exceeds its bound."""
+    per = piece_rows(q_heads, kv_heads)
+    pieces = words[4:4 + 8 * max_pieces].reshape(max_pieces, 8)
+    shared, parts = words[4 + 8 * max_pieces:][:rows], words[4 + 8 * max_pieces + rows:][:rows]
+    shared[:], parts[:] = 0, 0
+    groups, at = [], 0
+    for n, p in zip(sizes, prefixes):
+        p = p // PREFIX_TOKENS * PREFIX_TOKENS
+        if n > 0 and p > 0:
+            groups.append((at, n, p))
+        at += n
+    if not groups:
+        words[0] = 0
+        return 0, 0
+    longest = max(p for _, _, p in groups)
+    c = prefix_piece_tokens([(n, p) for _, n, p in groups], kv_heads, per)
+    while -(-longest // c) > max_parts or sum(-(-n // per) * -(-p // c) for _, n, p in groups) > max_pieces:
+        if c >= longest:
+            raise ValueError(f"{len(groups)} groups do not fit a plan of {max_pieces} pieces and {max_parts} parts")
+        c += PIECE_TOKENS
+    count = most = 0
+    for at, n, p in groups:
+        k = -(-p // c)
+        size = -(-p // (k * PIECE_TOKENS)) * PIECE_TOKENS          # even pieces
+        k = -(-p // size)
+        shared[at:at + n], parts[at:at + n] = p, k
+        for r in range(at, at + n, per):
+            m = min(per, at + n - r)
+            for i in range(k):
+                pieces[count] = (at, r, m, i * size, min(p, (i + 1) * size), i, 0, 0)
+                count += 1
+        most = max(most, k)
+    words[0] = count
+    return count, most
+
+
+class SharedPrefixPlan:
+    """Which rows of a decode batch share which prefix, in device memory (``words``), and the bounds that a call is launched with:
+    a captured graph may be replayed with other words that keep to them. ``own``: (slices, tokens per slice) of the rows' own tokens."""
+
+    def __init__(self, words: torch.Tensor, rows: int, max_pieces: int, max_parts: int, max_prefix: int, own: tuple[int, int], q_heads: int,
+                 kv_heads: int, head_dim: int):
+        self.words, self.rows, self.max_pieces, self.max_parts, self.max_prefix = words, rows, max_pieces, max_parts, max_prefix
+        self.own, self.q_heads, self.kv_heads, self.head_dim = own, q_heads, kv_heads, head_dim
+        base = words.data_ptr()
+        s = native.DecodeSharedArgs()
+        s.n_pieces, s.pieces = base, base + 16
+        s.row_prefix = base + 16 + 32 * max_pieces
+        s.row_parts = s.row_prefix + 4 * rows
+        s.max_pieces, s.max_parts, s.plan_rows = max_pieces, max_parts, rows
+        s.a.q_heads, s.a.kv_heads, s.a.head_dim = q_heads, kv_heads, head_dim
+        s.a.num_splits, s.a.chunk_tokens = own
+        self._fields = bytes(s)
+
+    def workspace_floats(self, batch: int) -> int:
+        """Elements of the fp32 workspace of a call over ``batch`` rows."""
+        slots = self.max_parts + (self.own[0] if self.own[0] > 1 else 0)
+        return batch * self.q_heads * slots * (self.head_dim + 2)
+
+
+def shared_prefix_plan(sizes: Sequence[int], prefixes: Sequence[int], *, rows: int, q_heads: int, kv_heads: int, head_dim: int, max_len: int,
+                       device: str | torch.device = "cuda") -> SharedPrefixPlan:
+    """The plan of a batch of ``rows`` rows whose first ``sizes[0]`` rows share their first ``prefixes[0]`` tokens (their block
+    tables name the same pages for them), the next ``sizes[1]`` rows ``prefixes[1]`` tokens and so on; rows behind the last group
+    share nothing. ``max_len``: bound of the sequence lengths while the plan is in use."""
+    if len(sizes) != len(prefixes) or any(n < 0 for n in sizes) or any(p < 0 for p in prefixes):
+        raise ValueError("a size and a prefix, neither negative, for every group")
+    if sum(sizes) > rows or (prefixes and max(prefixes) > max_len):
+        raise ValueError(f"groups of {sum(sizes)} rows and prefixes up to {max(prefixes, default=0)} for {rows} rows of {max_len} tokens")
+    _check_heads(q_heads, kv_heads, head_dim)
+    per = piece_rows(q_heads, kv_heads)
+    most = sum(-(-n // per) * -(-p // PIECE_TOKENS) for n, p in zip(sizes, prefixes))
+    host = np.zeros(shared_plan_words(rows, most), dtype=np.int32)
+    count, parts = fill_shared_plan(sizes, prefixes, host, rows, most, max(1, max(prefixes, default=0)), q_heads=q_heads, kv_heads=kv_heads)
+    words = np.concatenate([host[:4 + 8 * count], host[4 + 8 * most:]])
+    # slices for the longest tail of tokens behind a prefix (rows behind the groups may have max_len of them)
+    covered = [p // PREFIX_TOKENS * PREFIX_TOKENS for n, p in zip(sizes, prefixes) if n]
+    own = max_len - min(covered) if covered and sum(sizes) == rows else max_len
+    return SharedPrefixPlan(torch.from_numpy(words).to(device), rows, count, parts, max(prefixes, default=0),
+                            decode_plan(max(rows, 1), kv_heads, max(own, 1)), q_heads, kv_heads, head_dim)
+
+
+def _check_heads(q_heads: int, kv_heads: int, head_dim: int) -> None:
+    if kv_heads < 1 or q_heads % kv_heads or not 1 <= q_heads // kv_heads <= 16 or head_dim not in (64, 128):
+        raise ValueError(f"{q_heads} query and {kv_heads} KV heads of {head_dim}: up to 16 query heads per KV head of 64 or 128 are supported")
+
+
+def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                        plan: SharedPrefixPlan, *, out: torch.Tensor | None = None, ws: torch.Tensor | None = None,
+                        scale: float | None = None) -> torch.Tensor:
+    """:func:`paged_decode` for a batch whose rows share prefixes: every prefix of ``plan`` is read and multiplied once for all rows
+    of its group (``csrc/kernels/shared_prefix.cu``), then each row adds its own tokens. ``seq_lens`` count prefix and own tokens; a
+    row of fewer tokens than its group's prefix reads all of them on its own. Rows without tokens give zeros."""
+    batch, q_heads, d = q.shape
+    page, kv_heads = k_cache.shape[1], k_cache.shape[2]
+    if (q_heads, kv_heads, d) != (plan.q_heads, plan.kv_heads, plan.head_dim) or k_cache.shape != v_cache.shape or k_cache.shape[3] != d:
+        raise ValueError(f"q {tuple(q.shape)}, caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} for a plan of {plan.q_heads} query and "
+                         f"{plan.kv_heads} KV heads of {plan.head_dim}")
+    if page < 16 or page & (page - 1):
+        raise ValueError(f"pages of {page} tokens: powers of two from 16 on are supported")
+    dev = q.device
+    for t in (q, k_cache, v_cache):
+        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.data_ptr() % 16 or t.device != dev:
+            raise ValueError("queries and caches must be contiguous, 16-byte aligned bf16 on one device")
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_table.device != dev or seq_lens.device != dev:
+        raise ValueError("block_table and seq_lens must be int32 on the queries' device")
+    if block_table.dim() != 2 or block_table.shape[0] < batch or seq_lens.shape != (batch,) or not seq_lens.is_contiguous() \
+            or (block_table.shape[1] and block_table.stride(1) != 1):
+        raise ValueError(f"block_table {tuple(block_table.shape)} and seq_lens {tuple(seq_lens.shape)} for {batch} rows")
+    if plan.rows > batch or plan.words.device != dev or block_table.shape[1] * page < plan.max_prefix:
+        raise ValueError(f"a plan of {plan.rows} rows and prefixes of up to {plan.max_prefix} tokens for {batch} rows of {block_table.shape[1]} pages")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
+        raise ValueError("out must be like q")
+    need = plan.workspace_floats(batch)
+    if ws is None:
+        if need:
+            ws = torch.empty(need, dtype=torch.float32, device=dev)
+    elif ws.dtype != torch.float32 or ws.numel() < need or not ws.is_contiguous() or ws.device != dev:
+        raise ValueError(f"the workspace must hold {need} contiguous fp32 elements on the queries' device")
+    if not batch:
+        return out
+    if not k_cache.shape[0]:
+        raise ValueError("a cache of no pages")
+    s = native.DecodeSharedArgs.from_buffer_copy(plan._fields)
+    a = s.a
+    a.q, a.k_cache, a.v_cache, a.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
+    a.ws = ws.data_ptr() if ws is not None else None
+    a.block_table, a.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
+    a.batch, a.page_size, a.max_blocks, a.num_pages = batch, page, block_table.stride(0), k_cache.shape[0]
+    a.scale = scale if scale is not None else d ** -0.5
+    from .gemm import status_words
+
+    a.status = status_words(dev).data_ptr()
+    with native.on_device(dev):
+        native.check(native.kernels().xp_decode_shared(C.byref(s), _stream(dev)), "xp_decode_shared",
+                     1 + (plan.max_pieces > 0) + (plan.own[0] > 1))
     return out
 
 

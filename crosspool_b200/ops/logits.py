@@ -1,0 +1,155 @@
+"""Controls on logits, on the in-tree kernel (``csrc/kernels/logit_controls.cu``): penalties on the tokens that a row's prompt and
+answer already hold, biases on listed tokens, and bit masks of the tokens that a grammar allows.
+
+:func:`adjust_logits` stores the adjusted rows; :func:`select_tokens` reads the logits once and stores one token a row, greedily
+or by temperature (the draw of :func:`crosspool_b200.ops.attention.sample`).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+
+import torch
+
+from .. import native
+
+_INT, _FLOAT = torch.int32, torch.float32
+
+
+@dataclass(frozen=True)
+class LogitControls:
+    """What is done to the rows of a batch of logits; every tensor is optional and lives on the logits' device. Steps, in fp32 and
+    in this order: ``v / repetition`` where ``v > 0`` and ``v * repetition`` elsewhere, for tokens of the history; minus ``frequency``
+    times the occurrences behind the prompt; minus ``presence`` where there are any; plus the biases of the token; ``-inf`` where the
+    mask does not allow it.
+
+    The tensors are read when a call runs: their contents may change between calls (and between replays of a captured graph)."""
+
+    history: torch.Tensor | None = None        # int32 [slots, capacity] token ids; ids outside the vocabulary count for nothing
+    lens: torch.Tensor | None = None           # int32 [rows] tokens of the history in use
+    prompt_lens: torch.Tensor | None = None    # int32 [rows] how many of them are the prompt's (None: 0)
+    history_rows: torch.Tensor | None = None   # int32 [rows] slot of each row (None: row r is slot r; negative: no history)
+    latest: torch.Tensor | None = None         # int32 [rows] the last of the `lens` tokens, which the call stores into the history
+    repetition: torch.Tensor | None = None     # fp32 [rows]
+    frequency: torch.Tensor | None = None
+    presence: torch.Tensor | None = None
+    bias_ids: torch.Tensor | None = None       # int32 [entries], the rows' entries one after the other
+    bias_values: torch.Tensor | None = None    # fp32 [entries]; entries of one token add up
+    bias_starts: torch.Tensor | None = None    # int32 [rows + 1]
+    masks: torch.Tensor | None = None          # int32 [masks, words] bit i % 32 of word i / 32: token i is allowed
+    mask_index: torch.Tensor | None = None     # int32 [rows] mask of each row (outside the masks: none)
+
+    def __post_init__(self) -> None:
+        s = native.LogitArgs()
+        for name, dtype, dims in (("history", _INT, 2), ("history_rows", _INT, 1), ("lens", _INT, 1), ("prompt_lens", _INT, 1), ("latest", _INT, 1),
+                                  ("repetition", _FLOAT, 1), ("frequency", _FLOAT, 1), ("presence", _FLOAT, 1), ("bias_ids", _INT, 1),
+                                  ("bias_values", _FLOAT, 1), ("bias_starts", _INT, 1), ("masks", _INT, 2), ("mask_index", _INT, 1)):
+            t = getattr(self, name)
+            if t is None:
+                continue
+            if t.dtype != dtype or t.dim() != dims or (t.numel() and t.stride(-1) != 1):
+                raise ValueError(f"{name} must be {dtype} with {dims} dimensions and contiguous rows")
+            setattr(s, name, t.data_ptr() or None)
+        if (self.history is None) != (self.lens is None):
+            raise ValueError("history and lens come together")
+        for name in ("prompt_lens", "history_rows", "latest", "repetition", "frequency", "presence"):
+            if getattr(self, name) is not None and self.history is None:
+                raise ValueError(f"{name} needs a history")
+        given = [getattr(self, n) is not None for n in ("bias_ids", "bias_values", "bias_starts")]
+        if any(given) and not all(given):
+            raise ValueError("bias_ids, bias_values and bias_starts come together")
+        if (self.masks is None) != (self.mask_index is None):
+            raise ValueError("masks and mask_index come together")
+        rows, devices = set(), set()
+        for name in ("history_rows", "lens", "prompt_lens", "latest", "repetition", "frequency", "presence", "mask_index"):
+            if getattr(self, name) is not None:
+                rows.add(getattr(self, name).shape[0])
+        for name in self.__dataclass_fields__:
+            if getattr(self, name) is not None:
+                devices.add(getattr(self, name).device)
+        if self.bias_ids is not None:
+            if self.bias_ids.shape != self.bias_values.shape or not self.bias_starts.shape[0]:
+                raise ValueError("bias_ids and bias_values have an entry each, bias_starts one more than there are rows")
+            rows.add(self.bias_starts.shape[0] - 1)
+            s.bias_total = self.bias_ids.shape[0]
+        if len(rows) > 1 or len(devices) > 1:
+            raise ValueError(f"controls of {sorted(rows)} rows on {len(devices)} devices")
+        if self.history is not None:
+            s.history_slots, s.history_cap, s.ld_history = *self.history.shape, self.history.stride(0)
+            if self.history_rows is None and rows and self.history.shape[0] < max(rows):
+                raise ValueError(f"{self.history.shape[0]} histories for {max(rows)} rows")
+        if self.masks is not None:
+            s.mask_count, s.ld_mask = self.masks.shape[0], self.masks.stride(0)
+        object.__setattr__(self, "_fields", bytes(s))
+        object.__setattr__(self, "_rows", rows.pop() if rows else None)
+        object.__setattr__(self, "_device", devices.pop() if devices else None)
+
+    @property
+    def rows(self) -> int | None:
+        """Rows of logits that the controls belong to (None: no tensor says so)."""
+        return self._rows
+
+
+def _args(logits: torch.Tensor, c: LogitControls) -> "native.LogitArgs":
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
+        raise ValueError("logits must be bf16 or fp32 [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    if c._rows is not None and c._rows < rows:
+        raise ValueError(f"controls of {c._rows} rows for {rows} rows of logits")
+    if c._device is not None and c._device != logits.device:
+        raise ValueError(f"controls on {c._device} for logits on {logits.device}")
+    if c.masks is not None and c.masks.shape[0] and c.masks.shape[1] * 32 < vocab:
+        raise ValueError(f"masks of {c.masks.shape[1]} words for {vocab} tokens")
+    s = native.LogitArgs.from_buffer_copy(c._fields)
+    s.logits, s.rows, s.vocab, s.ld, s.f32 = logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, int(logits.dtype == _FLOAT)
+    return s
+
+
+def _launch(s, dev) -> None:
+    with native.on_device(dev):
+        native.check(native.kernels().xp_logit_controls(C.byref(s), torch.cuda.current_stream(dev).cuda_stream), "xp_logit_controls")
+
+
+def adjust_logits(logits: torch.Tensor, controls: LogitControls, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The logits after ``controls``, rounded once to ``out``'s type (bf16 or fp32; by default the logits' own). ``out`` may be
+    ``logits`` itself."""
+    s = _args(logits, controls)
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if out.shape != logits.shape or out.dtype not in (torch.bfloat16, _FLOAT) or out.stride(1) != 1 or out.device != logits.device:
+        raise ValueError("out must be bf16 or fp32 of the logits' shape, with contiguous rows, on their device")
+    if out.data_ptr() == logits.data_ptr() and out.numel() and (out.dtype != logits.dtype or out.stride(0) != logits.stride(0)):
+        raise ValueError("adjusting in place keeps type and pitch")
+    s.out, s.ld_out, s.out_f32 = out.data_ptr(), out.stride(0) if out.shape[0] > 1 else out.shape[1], int(out.dtype == _FLOAT)
+    if out.numel():
+        _launch(s, logits.device)
+    return out
+
+
+def select_tokens(logits: torch.Tensor, controls: LogitControls, temps: torch.Tensor | None = None, seeds: torch.Tensor | None = None, *,
+                  out: torch.Tensor | None = None, values: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per row from the logits after ``controls``: the largest one (ties go to the lower id), or where ``temps[r] > 0`` a
+    draw from ``softmax(adjusted / temperature)`` with ``seeds`` int32 ``[rows, 2]`` as in
+    :func:`crosspool_b200.ops.attention.sample`. ``values`` (fp32 ``[rows]``) receives the adjusted logit of the token. A row without
+    an allowed token gives token 0 and the value ``-inf``."""
+    s = _args(logits, controls)
+    rows, dev = logits.shape[0], logits.device
+    if logits.shape[1] == 0:
+        raise ValueError("logits of no tokens")
+    if out is None:
+        out = torch.empty(rows, dtype=_INT, device=dev)
+    for name, t, dtype, shape in (("out", out, _INT, (rows,)), ("values", values, _FLOAT, (rows,)), ("temps", temps, _FLOAT, (rows,)),
+                                  ("seeds", seeds, _INT, (rows, 2))):
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev):
+            raise ValueError(f"{name} must be contiguous {dtype} {shape} on the logits' device")
+    if (temps is None) != (seeds is None):
+        raise ValueError("temps and seeds come together")
+    s.tokens = out.data_ptr()
+    if values is not None:
+        s.values = values.data_ptr()
+    if temps is not None:
+        s.temps, s.seeds = temps.data_ptr(), seeds.data_ptr()
+    if rows:
+        _launch(s, dev)
+    return out

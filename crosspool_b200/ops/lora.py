@@ -1,0 +1,165 @@
+"""Low-rank adapters of many requests beside a shared projection, on the in-tree kernel (``csrc/kernels/lora.cu``).
+
+``lora_add(y, x, stack, plan)`` computes ``y[r] + scale[s] * (x[r] @ A[s].T) @ B[s].T`` for every row, ``s`` being the adapter
+of row ``r``; rows without one keep ``y``. The adapters of one projection live in an :class:`AdapterStack`; which row uses which
+is an :class:`AdapterPlan`, made once per batch and used by all layers and projections.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Sequence
+
+import numpy as np
+import torch
+
+from .. import native
+
+MAX_RANK = 128
+MAX_PARTS = 4
+ITEM_ROWS = 16        # rows of one adapter that a cluster of CTAs takes at once; a plan's items hold at most so many
+
+
+class AdapterStack:
+    """The adapters of one projection, slot by slot: ``a`` ``[slots, parts, rank, in]`` and ``b`` ``[slots, out, rank]`` in bf16,
+    a scale and a rank per slot. ``out_features``: a number, or one per part of a fused projection (q, k and v: each part has an
+    ``A`` of its own). Ranks are padded with zeros to ``rank``, the next multiple of 16 of ``max_rank``."""
+
+    def __init__(self, slots: int, in_features: int, out_features: int | Sequence[int], max_rank: int, device: str | torch.device = "cuda"):
+        self.parts = (int(out_features),) if isinstance(out_features, int) else tuple(int(n) for n in out_features)
+        if slots < 1 or not 1 <= max_rank <= MAX_RANK or not 1 <= len(self.parts) <= MAX_PARTS:
+            raise ValueError(f"{slots} slots, rank {max_rank}, {len(self.parts)} parts: at least one slot, ranks 1 to {MAX_RANK}, 1 to {MAX_PARTS} parts")
+        if in_features < 1 or in_features % 8 or any(n < 1 or n % 8 for n in self.parts):
+            raise ValueError(f"features {in_features} -> {self.parts}: multiples of 8 are supported")
+        self.slots, self.in_features, self.out_features = slots, in_features, sum(self.parts)
+        self.rank = (max_rank + 15) // 16 * 16
+        self.a = torch.zeros(slots, len(self.parts), self.rank, in_features, dtype=torch.bfloat16, device=device)
+        self.b = torch.zeros(slots, self.out_features, self.rank, dtype=torch.bfloat16, device=device)
+        self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
+        self.ranks = torch.zeros(slots, dtype=torch.int32, device=device)
+        self.device = self.a.device
+        end, ends = 0, []
+        for n in self.parts:
+            end += n
+            ends.append(end)
+        s = native.LoraArgs()
+        s.a, s.b, s.scale, s.ranks = self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), self.ranks.data_ptr()
+        s.k, s.n, s.rank, s.parts, s.slots = in_features, self.out_features, self.rank, len(self.parts), slots
+        s.part_end = (C.c_int * 4)(*(ends + [end] * (4 - len(ends))))
+        self._fields = bytes(s)
+
+    def load(self, slot: int, a: torch.Tensor | Sequence[torch.Tensor], b: torch.Tensor | Sequence[torch.Tensor], scale: float = 1.0) -> None:
+        """Puts an adapter into ``slot``: ``a`` ``[r, in]`` and ``b`` ``[out, r]``, or one pair per part (``None`` for a part
+        without one); ranks may differ between parts. Ordered with the work of the current stream."""
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot {slot} of {self.slots}")
+        pa, pb = ([a], [b]) if isinstance(a, torch.Tensor) else (list(a), list(b))
+        if len(pa) != len(self.parts) or len(pb) != len(self.parts):
+            raise ValueError(f"{len(pa)} and {len(pb)} matrices for {len(self.parts)} parts")
+        used = 0
+        for n, x, y in zip(self.parts, pa, pb):
+            if (x is None) != (y is None):
+                raise ValueError("a part has both matrices or none")
+            if x is None:
+                continue
+            r = x.shape[0]
+            if x.dim() != 2 or y.dim() != 2 or not 1 <= r <= self.rank or tuple(x.shape) != (r, self.in_features) or tuple(y.shape) != (n, r):
+                raise ValueError(f"matrices {tuple(x.shape)} and {tuple(y.shape)} for {self.in_features} -> {n} features, rank up to {self.rank}")
+            used = max(used, r)
+        self.a[slot].zero_()
+        self.b[slot].zero_()
+        at = 0
+        for i, (n, x, y) in enumerate(zip(self.parts, pa, pb)):
+            if x is not None:
+                self.a[slot, i, :x.shape[0]].copy_(x)
+                self.b[slot, at:at + n, :x.shape[0]].copy_(y)
+            at += n
+        self.scale[slot:slot + 1].fill_(float(scale))
+        self.ranks[slot:slot + 1].fill_((used + 15) // 16 * 16)
+
+    def clear(self, slot: int) -> None:
+        """Empties ``slot``: rows that name it keep ``y``."""
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"slot {slot} of {self.slots}")
+        self.ranks[slot:slot + 1].zero_()
+
+
+def plan_words(rows: int) -> int:
+    """32-bit words of a plan of up to ``rows`` rows."""
+    return 4 + 5 * rows
+
+
+def fill_plan(index: Sequence[int], words: np.ndarray, rows: int, bare: bool = True) -> int:
+    """Writes the plan of ``index`` (adapter slot per row, negative: none) to ``words`` (``plan_words(rows)`` of them); returns its
+    number of items. ``bare``: rows without an adapter get items too (they are copied when the result goes elsewhere)."""
+    idx = np.maximum(np.asarray(index, dtype=np.int64).reshape(-1), -1)
+    order = np.argsort(idx, kind="stable")
+    srt = idx[order]
+    starts = np.flatnonzero(np.r_[True, srt[1:] != srt[:-1]]) if len(srt) else np.zeros(0, dtype=np.int64)
+    counts = np.diff(np.r_[starts, len(srt)])
+    pieces = -(-counts // ITEM_ROWS)
+    run = np.repeat(np.arange(len(starts)), pieces)
+    nth = np.arange(len(run)) - np.repeat(np.cumsum(pieces) - pieces, pieces)
+    first = starts[run] + nth * ITEM_ROWS
+    n = np.minimum(ITEM_ROWS, counts[run] - nth * ITEM_ROWS)
+    slot = srt[starts][run] if len(starts) else run
+    if not bare:
+        keep = slot >= 0
+        first, n, slot = first[keep], n[keep], slot[keep]
+    items = words[4:4 + 4 * rows].reshape(rows, 4)
+    items[:len(slot), 0], items[:len(slot), 1], items[:len(slot), 2] = slot, first, n
+    words[4 + 4 * rows:4 + 4 * rows + len(order)] = order
+    words[0] = len(slot)
+    return len(slot)
+
+
+class AdapterPlan:
+    """Which adapter every row of a batch uses, in device memory (``words``), for up to ``rows`` rows. ``max_items`` bounds the
+    items that the words may hold while the plan is in use (a captured graph replays with new words)."""
+
+    def __init__(self, words: torch.Tensor, rows: int, max_items: int, slots: int):
+        self.words, self.rows, self.max_items, self.slots = words, rows, max_items, slots
+        base = words.data_ptr()
+        self._items, self._n_items, self._perm = base + 16, base, base + 16 + 16 * rows
+
+
+def adapter_plan(index: Sequence[int], stack: "AdapterStack | int", device: str | torch.device | None = None) -> AdapterPlan:
+    """The plan of a batch whose row ``r`` uses adapter slot ``index[r]`` (negative: none), for stacks of as many slots as ``stack``
+    has (or is)."""
+    slots = stack.slots if isinstance(stack, AdapterStack) else int(stack)
+    if device is None:
+        device = stack.device if isinstance(stack, AdapterStack) else "cuda"
+    rows = len(index)
+    if rows and max(index) >= slots:
+        raise ValueError(f"adapter slot {max(index)} of {slots}")
+    host = np.zeros(plan_words(rows), dtype=np.int32)
+    n = fill_plan(index, host, rows)
+    return AdapterPlan(torch.from_numpy(host).to(device), rows, n, slots)
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: AdapterPlan, *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``y[rows, out] + scale * (x[rows, in] @ A.T) @ B.T`` with every row's own adapter, rounded once; sums in fp32. ``out`` may
+    be ``y`` itself. bf16; rows may have a pitch (a multiple of 8 elements), so that a slice of a wider buffer can be read or written."""
+    rows = x.shape[0]
+    if out is None:
+        out = torch.empty(rows, stack.out_features, dtype=torch.bfloat16, device=x.device)
+    if x.dim() != 2 or x.shape[1] != stack.in_features or y.shape != (rows, stack.out_features) or out.shape != y.shape:
+        raise ValueError(f"x {tuple(x.shape)}, y {tuple(y.shape)}, out {tuple(out.shape)} beside a {stack.in_features} -> {stack.out_features} stack")
+    if rows != plan.rows or plan.slots > stack.slots:
+        raise ValueError(f"a plan of {plan.rows} rows and {plan.slots} slots for {rows} rows and {stack.slots} slots")
+    dev = stack.device
+    for t in (x, y, out):
+        if t.dtype != torch.bfloat16 or t.device != dev:
+            raise ValueError(f"{t.dtype} on {t.device}: bf16 on the stack's device ({dev}) is supported")
+        if t.stride(1) != 1 or (rows > 1 and t.stride(0) % 8) or t.data_ptr() % 16:
+            raise ValueError("rows must be contiguous, 16-byte aligned, with pitches of whole 16 bytes")
+    if plan.words.device != dev:
+        raise ValueError("the plan lives on another device")
+    s = native.LoraArgs.from_buffer_copy(stack._fields)
+    s.x, s.y, s.out = x.data_ptr(), y.data_ptr(), out.data_ptr()
+    s.items, s.n_items, s.perm = plan._items, plan._n_items, plan._perm
+    s.rows, s.max_items = rows, plan.max_items
+    s.ldx, s.ld_y, s.ld_out = x.stride(0), y.stride(0), out.stride(0)
+    with native.on_device(dev):
+        native.check(native.kernels().xp_lora(C.byref(s), torch.cuda.current_stream(dev).cuda_stream), "xp_lora")
+    return out
