@@ -120,6 +120,7 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 
 PREFIX_TOKENS = 16      # prefixes are shared in whole tiles of so many tokens; the rest of one is read by every row
 PIECE_TOKENS = 64       # pieces of a prefix begin at multiples of this
+MAX_PARTS = 32          # pieces of one prefix (partial results that a row's kernel merges)
 
 
 def piece_rows(q_heads: int, kv_heads: int) -> int:
@@ -138,7 +139,7 @@ def prefix_piece_tokens(groups: Sequence[tuple[int, int]], kv_heads: int, rows_p
         units = kv_heads * sum(t * -(-p // c) for t, p in tiles)
         parts = -(-longest // c)
         cost = -(-units // num_sms) * (min(c, longest) + 128) + 8 * parts
-        if best_cost is None or cost < best_cost:
+        if parts <= MAX_PARTS and (best_cost is None or cost < best_cost):
             best, best_cost = c, cost
         if c >= longest:
             return best
@@ -226,7 +227,7 @@ def shared_prefix_plan(sizes: Sequence[int], prefixes: Sequence[int], *, rows: i
     per = piece_rows(q_heads, kv_heads)
     most = sum(-(-n // per) * -(-p // PIECE_TOKENS) for n, p in zip(sizes, prefixes))
     host = np.zeros(shared_plan_words(rows, most), dtype=np.int32)
-    count, parts = fill_shared_plan(sizes, prefixes, host, rows, most, max(1, max(prefixes, default=0)), q_heads=q_heads, kv_heads=kv_heads)
+    count, parts = fill_shared_plan(sizes, prefixes, host, rows, most, MAX_PARTS, q_heads=q_heads, kv_heads=kv_heads)
     words = np.concatenate([host[:4 + 8 * count], host[4 + 8 * most:]])
     # slices for the longest tail of tokens behind a prefix (rows behind the groups may have max_len of them)
     covered = [p // PREFIX_TOKENS * PREFIX_TOKENS for n, p in zip(sizes, prefixes) if n]
@@ -268,6 +269,8 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be like q")
+    if out.data_ptr() % 16 or (ws is not None and ws.data_ptr() % 16):
+        raise ValueError("out and the workspace must be 16-byte aligned")
     need = plan.workspace_floats(batch)
     if ws is None:
         if need:
