@@ -23,17 +23,23 @@ typedef struct XpPrefixPiece {
 } XpPrefixPiece;
 
 typedef struct XpDecodeSharedArgs {
-  XpDecodeAttnArgs a;         /* ws: partial sums [batch, q_heads, max_parts + own, head_dim], behind them (maximum, sum) pairs
-                                 [batch, q_heads, max_parts + own, 2]; own = num_splits when that is > 1, otherwise 0 */
+  XpDecodeAttnArgs a;         /* ws: partial sums [batch, q_heads, max_parts + own_slots, head_dim], then their (maximum, sum) pairs
+                                 [batch, q_heads, max_parts + own_slots, 2], then batch + 4 words. num_splits and chunk_tokens
+                                 (and ws as they want it) are read where max_pieces is 0 */
   const XpPrefixPiece* pieces;
-  const int* n_pieces;        /* device word */
+  const int* n_pieces;        /* device words: number of pieces, tokens of the longest one */
   const int* row_prefix;      /* [plan_rows] tokens that a row shares (a multiple of 16); a row of fewer tokens reads all on its own */
   const int* row_parts;       /* [plan_rows] pieces of the row */
   int max_pieces;             /* bound of *n_pieces */
-  int max_parts;              /* bound of row_parts */
+  int max_parts;              /* bound of row_parts, up to XP_PREFIX_PARTS */
   int plan_rows;              /* rows behind these share nothing */
+  int own_slots;              /* partial results of a row's own tokens, 2 to XP_PREFIX_OWN */
+  int max_len;                /* bound of the sequences' lengths: rows are read no further */
   int reserved;
 } XpDecodeSharedArgs;
+#define XP_PREFIX_PARTS 32
+#define XP_PREFIX_OWN 64
+#define XP_PREFIX_ROWS 4096   /* largest batch */
 int xp_decode_shared(const XpDecodeSharedArgs* a, void* stream);
 
 /* out[r] = y[r] + scale[s] B[s] (A[s] x[r]) with s the adapter slot of row r (none: out[r] = y[r]). A projection may have several

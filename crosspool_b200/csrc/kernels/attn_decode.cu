@@ -12,7 +12,6 @@
 #include <type_traits>
 
 #include "xpool/api.h"
-#include "xpool/request_api.h"
 #include "xpool/sm100.cuh"
 #include "xpool/tensormap.hpp"
 #include "xpool/pdl.cuh"
@@ -283,9 +282,6 @@ decode_attn_kernel(XpDecodeAttnArgs a) {
 //
 // kSig: weights are sigmoids of the scores (no maximum, no sum), and the tiles may begin with the means of the blocks behind the
 // window, which come from a paged cache of their own in two boxes of eight rows.
-//
-// XpDecodeSharedArgs: the first tokens of a row belong to a prefix that shared_prefix.cu has multiplied for all rows that share
-// it. The kernel reads what lies behind them and adds the prefix's partial results when it finishes a head.
 constexpr int kTcStages = 3;
 
 __device__ __forceinline__ void tma_load_kv(uint32_t dst, const CUtensorMap* m, uint32_t bar, int d0, int head, int token) {
@@ -324,45 +320,6 @@ __device__ __forceinline__ uint32_t pack_rest(float lo, float hi, uint32_t packe
 
 __device__ __forceinline__ const XpDecodeAttnArgs& base_of(const XpDecodeRowsArgs& a) { return a.a; }
 __device__ __forceinline__ const XpDecodeAttnArgs& base_of(const XpDecodeAttnArgs& a) { return a; }
-__device__ __forceinline__ const XpDecodeAttnArgs& base_of(const XpDecodeSharedArgs& a) { return a.a; }
-
-template <typename A>
-constexpr bool kIsShared = std::is_same<A, XpDecodeSharedArgs>::value;
-
-// Partial results of a row of a shared prefix: sums of head hq and slot i, and their (maximum, sum of weights) pair.
-struct Partials {
-  float* sums;
-  float* pairs;
-  int slots;
-  template <int D>
-  static __device__ __forceinline__ Partials of(const XpDecodeSharedArgs& s, int b, int hq) {
-    const int slots = s.max_parts + (s.a.num_splits > 1 ? s.a.num_splits : 0);
-    const size_t all = static_cast<size_t>(s.a.batch) * s.a.q_heads * slots, at = (static_cast<size_t>(b) * s.a.q_heads + hq) * slots;
-    return {s.a.ws + at * D, s.a.ws + all * D + at * 2, slots};
-  }
-};
-// Tokens that row b shares: none where it has fewer than the prefix.
-__device__ __forceinline__ int shared_tokens(const XpDecodeSharedArgs& s, int b) {
-  const int p = b < s.plan_rows ? s.row_prefix[b] : 0;
-  return s.a.seq_lens[b] >= p ? p : 0;
-}
-// Tokens of a slice of a row's own: the plan's, or more where a row has more of them than its slices cover.
-__device__ __forceinline__ int own_chunk(int chunk_tokens, int nsplit, int own) {
-  return max(chunk_tokens, ((own + nsplit - 1) / nsplit + 15) & ~15);
-}
-// Adds slots [i0, i1) to (av, ll, mm): weighted sum of element d, sum of weights, maximum.
-template <int D>
-__device__ __forceinline__ void add_partials(const Partials& p, int i0, int i1, int d, float& av, float& ll, float& mm) {
-  float top = mm;
-  for (int i = i0; i < i1; ++i) top = fmaxf(top, p.pairs[2 * i]);
-  const float c = mm == -CUDART_INF_F ? 0.f : exp2f(mm - top);
-  av *= c, ll *= c, mm = top;
-  for (int i = i0; i < i1; ++i) {
-    const float m = p.pairs[2 * i], w = m == -CUDART_INF_F ? 0.f : exp2f(m - top);
-    ll += p.pairs[2 * i + 1] * w;
-    av += p.sums[static_cast<size_t>(i) * D + d] * w;
-  }
-}
 
 // What a row reads of its sequence: tokens [0, head) and [head + skip, len + skip), head and skip whole 16-token tiles. `len`
 // counts both; lo is the first token of the window. With pooled blocks the first `blocks` of [0, head) are those.
@@ -383,9 +340,6 @@ __device__ __forceinline__ Span row_span(const A& args, int b) {
       s.skip = (s.lo & ~15) - s.head;
       s.len -= s.skip;
     }
-  } else if constexpr (kIsShared<A>) {
-    s.skip = shared_tokens(args, b);
-    s.len = args.a.seq_lens[b] - s.skip;
   } else {
     s.len = args.seq_lens[b];
   }
@@ -403,8 +357,7 @@ __device__ __forceinline__ void store_out(const A& args, int b, int hq, int d, f
     }
     reinterpret_cast<__nv_bfloat16*>(args.a.out)[static_cast<size_t>(b) * args.ld_out + hq * args.v_valid + d] = __float2bfloat16_rn(v);
   } else {
-    const XpDecodeAttnArgs& a = base_of(args);
-    reinterpret_cast<__nv_bfloat16*>(a.out)[(static_cast<size_t>(b) * a.q_heads + hq) * DV + d] = __float2bfloat16_rn(v);
+    reinterpret_cast<__nv_bfloat16*>(args.out)[(static_cast<size_t>(b) * args.q_heads + hq) * DV + d] = __float2bfloat16_rn(v);
   }
 }
 
@@ -422,79 +375,12 @@ __device__ __forceinline__ float finish_out(const A& args, int hq, float av, flo
   return ll > 0.f ? av / ll : 0.f;
 }
 
-constexpr int kWarpParts = 4;     // partial results of a CTA's own tokens: one per warp, red[warp][16][DV + 2]
-
-// Merges the warps' partial results of row b's heads and, when its own tokens are not cut into slices, those of the `parts` pieces
-// of its prefix; stores the heads, or the slice's partial result. The weight of every partial result is computed once per head (a
-// warp per head) and the sums are read 16 bytes a lane: with the weights in the inner loop the CTAs of 256 rows of nine pieces
-// took 103 us instead of 45.
-constexpr int kMergeParts = 32;
-template <int DV>
-__device__ __forceinline__ void finish_shared(const XpDecodeSharedArgs& args, const float* red, int b, int hk, int G, int nsplit, int split, int parts) {
-  __shared__ float wt[16][kWarpParts + kMergeParts + 1];        // weights of warps and pieces, then 1 / sum of weights
-  const XpDecodeAttnArgs& a = args.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (nsplit > 1) parts = 0;
-  for (int g = warp; g < G; g += kDecodeThreads / 32) {
-    const Partials p = Partials::of<DV>(args, b, hk * G + g);
-    const float* own = red + (lane * 16 + g) * (DV + 2) + DV;
-    float2 mo = make_float2(-CUDART_INF_F, 0.f), mp = mo;
-    if (lane < kWarpParts) mo = make_float2(own[0], own[1]);
-    if (lane < parts) mp = reinterpret_cast<const float2*>(p.pairs)[lane];
-    float top = fmaxf(mo.x, mp.x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float co = mo.x == -CUDART_INF_F ? 0.f : exp2f(mo.x - top), cp = mp.x == -CUDART_INF_F ? 0.f : exp2f(mp.x - top);
-    float sum = mo.y * co + mp.y * cp;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane < kWarpParts) wt[g][lane] = co;
-    if (lane < parts) wt[g][kWarpParts + lane] = cp;
-    if (lane == 0) {
-      wt[g][kWarpParts + kMergeParts] = sum > 0.f ? 1.f / sum : 0.f;
-      if (nsplit > 1) reinterpret_cast<float2*>(p.pairs)[args.max_parts + split] = make_float2(top, sum);
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x * 4; i < G * DV; i += kDecodeThreads * 4) {
-    const int g = i / DV, d = i % DV, hq = hk * G + g;
-    const Partials p = Partials::of<DV>(args, b, hq);
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWarpParts; ++w) {
-      const float* rw = red + (w * 16 + g) * (DV + 2) + d;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(rw[e], wt[g][w], v[e]);
-    }
-#pragma unroll 8
-    for (int s = 0; s < parts; ++s) {
-      const float4 o = *reinterpret_cast<const float4*>(p.sums + static_cast<size_t>(s) * DV + d);
-      const float c = wt[g][kWarpParts + s];
-      v[0] = fmaf(o.x, c, v[0]), v[1] = fmaf(o.y, c, v[1]), v[2] = fmaf(o.z, c, v[2]), v[3] = fmaf(o.w, c, v[3]);
-    }
-    if (nsplit > 1) {
-      *reinterpret_cast<float4*>(p.sums + static_cast<size_t>(args.max_parts + split) * DV + d) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      const float c = wt[g][kWarpParts + kMergeParts];
-      uint2 r;
-      r.x = pack_bf16(v[0] * c, v[1] * c), r.y = pack_bf16(v[2] * c, v[3] * c);
-      *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (static_cast<size_t>(b) * a.q_heads + hq) * DV + d) = r;
-    }
-  }
-}
-
 template <int DQ, int DV, typename A, bool kSig = false>
 __global__ void __launch_bounds__(kDecodeThreads, 2)
 decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                       const __grid_constant__ CUtensorMap tmap_kp, const __grid_constant__ CUtensorMap tmap_vp, A args) {
-  // Behind the kernel of the prefix pieces, which has itself waited for everything before it, the row's own tokens may be read
-  // at once; its partial results are waited for below.
-  bool behind_pieces = false;
-  if constexpr (kIsShared<A>) behind_pieces = args.max_pieces > 0;
-  if (!behind_pieces) {
-    pdl::wait();
-    pdl::release();
-  }
+  pdl::wait();
+  pdl::release();
   constexpr bool kRows = std::is_same<A, XpDecodeRowsArgs>::value;
   static_assert(kRows || !kSig, "sigmoid weights are a form of single rows");
   const XpDecodeAttnArgs& a = base_of(args);
@@ -516,7 +402,6 @@ decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     chunk = (len + nsplit - 1) / nsplit;
     chunk = (chunk + 15) & ~15;
   }
-  if constexpr (kIsShared<A>) chunk = own_chunk(chunk, nsplit, len);
   const int t0 = split * chunk;
   const int t1 = min(len, t0 + chunk);
   if (a.chunk_tokens > 0 && nsplit > 1 && t0 >= len) return;  // the merge kernel skips this slice
@@ -796,14 +681,6 @@ decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     }
   }
   __syncthreads();
-  if constexpr (kIsShared<A>) {
-    if (behind_pieces) {
-      pdl::wait();
-      pdl::release();
-    }
-    finish_shared<DV>(args, red, b, hk, G, nsplit, split, span.skip > 0 ? args.row_parts[b] : 0);
-    return;
-  }
   for (int i = threadIdx.x; i < G * DV; i += kDecodeThreads) {
     const int gg = i / DV, d = i % DV;
     float mm = -CUDART_INF_F;
@@ -829,23 +706,6 @@ decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
       }
     }
   }
-}
-
-// Prefix pieces and slices of a row's own tokens.
-template <int D>
-__global__ void shared_combine_kernel(XpDecodeSharedArgs args, int nsplit) {
-  pdl::wait();
-  pdl::release_short();
-  const XpDecodeAttnArgs& a = args.a;
-  const int hq = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const int shared = shared_tokens(args, b), own = a.seq_lens[b] - shared;
-  const int chunk = own_chunk(a.chunk_tokens, nsplit, own);
-  nsplit = min(nsplit, (own + chunk - 1) / chunk);                                            // slices that ran
-  const Partials p = Partials::of<D>(args, b, hq);
-  float av = 0.f, ll = 0.f, mm = -CUDART_INF_F;
-  add_partials<D>(p, 0, shared > 0 ? args.row_parts[b] : 0, d, av, ll, mm);
-  add_partials<D>(p, args.max_parts, args.max_parts + nsplit, d, av, ll, mm);
-  reinterpret_cast<__nv_bfloat16*>(a.out)[(static_cast<size_t>(b) * a.q_heads + hq) * D + d] = __float2bfloat16_rn(ll > 0.f ? av / ll : 0.f);
 }
 
 template <int D, bool kSig = false, typename A>
@@ -911,11 +771,7 @@ static int launch_decode_tc(const A& args, int nsplit, cudaStream_t s) {
   }
   dim3 grid(nsplit, a.kv_heads, a.batch);
   pdl::launch(decode_attn_tc_kernel<DQ, DV, A, kSig>, grid, kDecodeThreads, kSmem, s, 1, mk, mv, mkp, mvp, args);
-  if constexpr (std::is_same<A, XpDecodeSharedArgs>::value) {
-    if (nsplit > 1) pdl::launch(shared_combine_kernel<DV>, dim3(a.q_heads, a.batch), DV, 0, s, 1, args, nsplit);
-  } else {
-    if (nsplit > 1) pdl::launch(decode_combine_kernel<DV, kSig, A>, dim3(a.q_heads, a.batch), DV, 0, s, 1, args, nsplit);
-  }
+  if (nsplit > 1) pdl::launch(decode_combine_kernel<DV, kSig, A>, dim3(a.q_heads, a.batch), DV, 0, s, 1, args, nsplit);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -100 - static_cast<int>(e);
 }
@@ -984,26 +840,4 @@ extern "C" int xp_decode_rows(const XpDecodeRowsArgs* r, void* stream) {
   if (a->head_dim == 128 && r->v_dim == 128) return launch_decode_tc<128, 128>(*r, nsplit, s);
   if (a->head_dim == 192 && r->v_dim == 128) return launch_decode_tc<192, 128>(*r, nsplit, s);
   return -13;
-}
-
-extern "C" int xp_shared_prefix_pieces(const XpDecodeSharedArgs* a, void* stream);   // shared_prefix.cu
-
-extern "C" int xp_decode_shared(const XpDecodeSharedArgs* r, void* stream) {
-  using namespace xpool::attn;
-  const XpDecodeAttnArgs* a = &r->a;
-  if (a->batch <= 0) return 0;
-  if (a->kv_heads <= 0 || a->q_heads % a->kv_heads != 0) return -10;
-  const int nsplit = a->num_splits > 0 ? a->num_splits : 1;
-  if ((r->max_parts > 0 || nsplit > 1) && a->ws == nullptr) return -11;
-  if (r->max_parts > kMergeParts || (reinterpret_cast<uintptr_t>(a->ws) & 15) != 0 || (reinterpret_cast<uintptr_t>(a->out) & 7) != 0) return -11;
-  if (a->q_heads / a->kv_heads > 16 || a->num_pages <= 0 || a->page_size < 16 || (a->page_size & (a->page_size - 1)) != 0 ||
-      a->chunk_tokens % 16 != 0 || (reinterpret_cast<uintptr_t>(a->q) & 15) != 0 || a->batch > 65535)
-    return -12;
-  if (a->head_dim != 64 && a->head_dim != 128) return -13;
-  if (r->max_pieces > 0) {
-    const int rc = xp_shared_prefix_pieces(r, stream);
-    if (rc != 0) return rc;
-  }
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return a->head_dim == 128 ? launch_decode_tc<128, 128>(*r, nsplit, s) : launch_decode_tc<64, 64>(*r, nsplit, s);
 }

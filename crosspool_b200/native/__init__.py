@@ -266,7 +266,7 @@ class DecodeRowsArgs(C.Structure):
 
 class DecodeSharedArgs(C.Structure):
     _fields_ = [("a", DecodeAttnArgs), ("pieces", C.c_void_p), ("n_pieces", C.c_void_p), ("row_prefix", C.c_void_p), ("row_parts", C.c_void_p),
-                ("max_pieces", C.c_int), ("max_parts", C.c_int), ("plan_rows", C.c_int), ("reserved", C.c_int)]
+                ("max_pieces", C.c_int), ("max_parts", C.c_int), ("plan_rows", C.c_int), ("own_slots", C.c_int), ("max_len", C.c_int), ("reserved", C.c_int)]
 
 
 class PrefillAttnArgs(C.Structure):

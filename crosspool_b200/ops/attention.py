@@ -120,7 +120,15 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 
 PREFIX_TOKENS = 16      # prefixes are shared in whole tiles of so many tokens; the rest of one is read by every row
 PIECE_TOKENS = 64       # pieces of a prefix begin at multiples of this
-MAX_PARTS = 32          # pieces of one prefix (partial results that a row's kernel merges)
+MAX_PARTS = 32          # pieces of one prefix
+MAX_SHARED_ROWS = 4096  # rows of a batch
+
+
+def own_slots(rows: int, q_heads: int, kv_heads: int) -> int:
+    """Shares that a row's own tokens may be cut into: the grid's workers (twelve warps on each of 148 SMs) take even shares of all
+    own tokens, and a long row among short ones needs more of them than the rows of an even batch."""
+    units = max(1, rows) * kv_heads * (2 if q_heads // kv_heads > 8 else 1)
+    return min(64, max(8, -(-2 * 12 * 148 // units)))
 
 
 def piece_rows(q_heads: int, kv_heads: int) -> int:
@@ -166,7 +174,7 @@ def fill_shared_plan(sizes: Sequence[int], prefixes: Sequence[int], words: np.nd
             groups.append((at, n, p))
         at += n
     if not groups:
-        words[0] = 0
+        words[0] = words[1] = 0
         return 0, 0
     longest = max(p for _, _, p in groups)
     c = prefix_piece_tokens([(n, p) for _, n, p in groups], kv_heads, per)
@@ -174,7 +182,7 @@ def fill_shared_plan(sizes: Sequence[int], prefixes: Sequence[int], words: np.nd
         if c >= longest:
             raise ValueError(f"{len(groups)} groups do not fit a plan of {max_pieces} pieces and {max_parts} parts")
         c += PIECE_TOKENS
-    count = most = 0
+    count = most = tokens = 0
     for at, n, p in groups:
         k = -(-p // c)
         size = -(-p // (k * PIECE_TOKENS)) * PIECE_TOKENS          # even pieces
@@ -185,33 +193,38 @@ def fill_shared_plan(sizes: Sequence[int], prefixes: Sequence[int], words: np.nd
             for i in range(k):
                 pieces[count] = (at, r, m, i * size, min(p, (i + 1) * size), i, 0, 0)
                 count += 1
-        most = max(most, k)
-    words[0] = count
+        most, tokens = max(most, k), max(tokens, size)
+    words[0], words[1] = count, tokens
     return count, most
 
 
 class SharedPrefixPlan:
     """Which rows of a decode batch share which prefix, in device memory (``words``), and the bounds that a call is launched with:
-    a captured graph may be replayed with other words that keep to them. ``own``: (slices, tokens per slice) of the rows' own tokens."""
+    a captured graph may be replayed with other words that keep to them. ``max_len`` bounds the sequences' lengths."""
 
-    def __init__(self, words: torch.Tensor, rows: int, max_pieces: int, max_parts: int, max_prefix: int, own: tuple[int, int], q_heads: int,
-                 kv_heads: int, head_dim: int):
-        self.words, self.rows, self.max_pieces, self.max_parts, self.max_prefix = words, rows, max_pieces, max_parts, max_prefix
-        self.own, self.q_heads, self.kv_heads, self.head_dim = own, q_heads, kv_heads, head_dim
+    def __init__(self, words: torch.Tensor, rows: int, max_pieces: int, max_parts: int, max_len: int, q_heads: int, kv_heads: int, head_dim: int):
+        if rows > MAX_SHARED_ROWS or rows * -(-max_len // 16) * kv_heads * 2 >= 2 ** 31:
+            raise ValueError(f"{rows} rows of up to {max_len} tokens: up to {MAX_SHARED_ROWS} rows and 2^31 tiles of 16 tokens are supported")
+        self.words, self.rows, self.max_pieces, self.max_parts = words, rows, max_pieces, max_parts
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self.slices = decode_plan(max(rows, 1), kv_heads, max(max_len, 1)) if max_pieces == 0 else (1, 0)   # without prefixes: paged_decode's
         base = words.data_ptr()
         s = native.DecodeSharedArgs()
         s.n_pieces, s.pieces = base, base + 16
         s.row_prefix = base + 16 + 32 * max_pieces
         s.row_parts = s.row_prefix + 4 * rows
         s.max_pieces, s.max_parts, s.plan_rows = max_pieces, max_parts, rows
+        s.max_len = self.max_len = max_len
+        s.own_slots = self.own = own_slots(rows, q_heads, kv_heads)
         s.a.q_heads, s.a.kv_heads, s.a.head_dim = q_heads, kv_heads, head_dim
-        s.a.num_splits, s.a.chunk_tokens = own
+        s.a.num_splits, s.a.chunk_tokens = self.slices
         self._fields = bytes(s)
 
     def workspace_floats(self, batch: int) -> int:
         """Elements of the fp32 workspace of a call over ``batch`` rows."""
-        slots = self.max_parts + (self.own[0] if self.own[0] > 1 else 0)
-        return batch * self.q_heads * slots * (self.head_dim + 2)
+        if self.max_pieces == 0:
+            return batch * self.q_heads * self.slices[0] * (self.head_dim + 2) if self.slices[0] > 1 else 0
+        return batch * self.q_heads * (self.max_parts + self.own) * (self.head_dim + 2) + batch + 4
 
 
 def shared_prefix_plan(sizes: Sequence[int], prefixes: Sequence[int], *, rows: int, q_heads: int, kv_heads: int, head_dim: int, max_len: int,
@@ -229,11 +242,7 @@ def shared_prefix_plan(sizes: Sequence[int], prefixes: Sequence[int], *, rows: i
     host = np.zeros(shared_plan_words(rows, most), dtype=np.int32)
     count, parts = fill_shared_plan(sizes, prefixes, host, rows, most, MAX_PARTS, q_heads=q_heads, kv_heads=kv_heads)
     words = np.concatenate([host[:4 + 8 * count], host[4 + 8 * most:]])
-    # slices for the longest tail of tokens behind a prefix (rows behind the groups may have max_len of them)
-    covered = [p // PREFIX_TOKENS * PREFIX_TOKENS for n, p in zip(sizes, prefixes) if n]
-    own = max_len - min(covered) if covered and sum(sizes) == rows else max_len
-    return SharedPrefixPlan(torch.from_numpy(words).to(device), rows, count, parts, max(prefixes, default=0),
-                            decode_plan(max(rows, 1), kv_heads, max(own, 1)), q_heads, kv_heads, head_dim)
+    return SharedPrefixPlan(torch.from_numpy(words).to(device), rows, count, parts, max_len, q_heads, kv_heads, head_dim)
 
 
 def _check_heads(q_heads: int, kv_heads: int, head_dim: int) -> None:
@@ -263,8 +272,8 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     if block_table.dim() != 2 or block_table.shape[0] < batch or seq_lens.shape != (batch,) or not seq_lens.is_contiguous() \
             or (block_table.shape[1] and block_table.stride(1) != 1):
         raise ValueError(f"block_table {tuple(block_table.shape)} and seq_lens {tuple(seq_lens.shape)} for {batch} rows")
-    if plan.rows > batch or plan.words.device != dev or block_table.shape[1] * page < plan.max_prefix:
-        raise ValueError(f"a plan of {plan.rows} rows and prefixes of up to {plan.max_prefix} tokens for {batch} rows of {block_table.shape[1]} pages")
+    if plan.rows > batch or plan.words.device != dev or block_table.shape[1] * page < plan.max_len:
+        raise ValueError(f"a plan of {plan.rows} rows of up to {plan.max_len} tokens for {batch} rows of {block_table.shape[1]} pages")
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
@@ -279,6 +288,8 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise ValueError(f"the workspace must hold {need} contiguous fp32 elements on the queries' device")
     if not batch:
         return out
+    if batch > MAX_SHARED_ROWS:
+        raise ValueError(f"{batch} rows: up to {MAX_SHARED_ROWS} are supported")
     if not k_cache.shape[0]:
         raise ValueError("a cache of no pages")
     s = native.DecodeSharedArgs.from_buffer_copy(plan._fields)
@@ -293,7 +304,7 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     a.status = status_words(dev).data_ptr()
     with native.on_device(dev):
         native.check(native.kernels().xp_decode_shared(C.byref(s), _stream(dev)), "xp_decode_shared",
-                     1 + (plan.max_pieces > 0) + (plan.own[0] > 1))
+                     1 + (plan.max_pieces > 0 or plan.slices[0] > 1))
     return out
 
 

@@ -165,7 +165,7 @@ def test_graph_replays_with_other_plans():
     rows, hq, hk, d, page = 12, 8, 2, 128, 16
     cases = [([12], [512]), ([4, 8], [256, 64]), ([], []), ([3, 3, 3], [16, 512, 128])]
     words = torch.zeros(A.shared_plan_words(rows, 64), dtype=torch.int32, device="cuda")
-    plan = A.SharedPrefixPlan(words, rows, 64, 8, 512, A.decode_plan(rows, hk, 700), hq, hk, d)
+    plan = A.SharedPrefixPlan(words, rows, 64, 8, 700, hq, hk, d)
     ws = torch.empty(plan.workspace_floats(rows), device="cuda")
 
     def load(i):
@@ -180,7 +180,7 @@ def test_graph_replays_with_other_plans():
     wide = max(s[0][3].shape[1] for s in sets)
     k, v = (torch.zeros(pages, page, hk, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
     q, out = torch.zeros(rows, hq, d, dtype=torch.bfloat16, device="cuda"), torch.zeros(rows, hq, d, dtype=torch.bfloat16, device="cuda")
-    table, lens = torch.zeros(rows, max(wide, 32), dtype=torch.int32, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda")
+    table, lens = torch.zeros(rows, max(wide, 44), dtype=torch.int32, device="cuda"), torch.zeros(rows, dtype=torch.int32, device="cuda")
 
     def fill(i):
         (q1, k1, v1, t1, n1), w = sets[i]
@@ -219,5 +219,5 @@ def test_two_streams_at_once():
 def run_quietly(sizes, prefixes, q, k, v, table, lens):
     from crosspool_b200.ops import attention as A
 
-    plan = A.shared_prefix_plan(sizes, prefixes, rows=q.shape[0], q_heads=q.shape[1], kv_heads=k.shape[2], head_dim=q.shape[2], max_len=1000)
+    plan = A.shared_prefix_plan(sizes, prefixes, rows=q.shape[0], q_heads=q.shape[1], kv_heads=k.shape[2], head_dim=q.shape[2], max_len=700)
     return A.paged_decode_shared(q, k, v, table, lens, plan)
