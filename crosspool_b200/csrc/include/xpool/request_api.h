@@ -17,7 +17,7 @@ extern "C" {
 typedef struct XpPrefixPiece {
   int leader;                 /* row whose block table names the prefix's pages */
   int row0, rows;             /* rows of the piece */
-  int tok0, tok1;             /* tokens [tok0, tok1) of the sequence, tok0 a multiple of 64, tok1 of 16 */
+  int tok0, tok1;             /* tokens [tok0, tok1) of the sequence, tok0 a multiple of 128, tok1 of 16 */
   int part;                   /* index of the partial result of these rows */
   int pad0, pad1;
 } XpPrefixPiece;

@@ -8,13 +8,13 @@
 //
 // Pieces. A plan cuts every prefix into pieces (a range of its tokens, and up to 2 x (128 / G) consecutive rows that read it, G
 // query heads to a KV head). The first CTAs take (piece, KV head) units in turn: two tiles of 128 queries (row of a tile = row * G
-// + head), both multiplied against the same 64-token K/V tiles, so that the tensor pipe works on one while the softmax of the other runs.
+// + head), both multiplied against the same steps of 128 tokens, so that the tensor pipe works on one while the softmax of the other runs.
 //   warps 0-3   softmax of tile A: thread = query = TMEM lane. Reads its row of S with tcgen05.ld, keeps a running maximum and
-//               sum, writes P (bf16) over the start of S as the A operand of the second product, rescales O in tensor memory only
+//               sum, writes P (bf16) over the second half of S as the A operand of the second product, rescales O in tensor memory only
 //               when the maximum grew by more than 2^8 (sum and result carry the same stale maximum), and stores the partial result.
 //   warps 4-7   the same for tile B.
-//   warp 8      TMA producer: Q tiles once a unit, then a ring of K/V tiles through the leader's page table (128-byte swizzle).
-//   warp 9      allocates tensor memory and issues every tcgen05.mma: S_A(t+1), PV_A(t), S_B(t+1), PV_B(t).
+//   warp 8      TMA producer: Q tiles once a unit, then a ring of steps of keys and values through the leader's page table (128-byte swizzle).
+//   warp 9      allocates tensor memory and issues every tcgen05.mma: PV_A(t), S_A(t+1), PV_B(t), S_B(t+1).
 // Own tokens. The 16-token tiles of all rows' own tokens, row by row, KV head by KV head, are one list that is cut into shares for
 // the warps of the grid, wherever a share ends: ragged rows balance, and a row's tokens are in at most own_slots shares. CTAs
 // without pieces begin at once and get larger shares, by as much as the others' pieces take.
@@ -39,22 +39,24 @@ namespace xpool {
 namespace prefix {
 
 constexpr int kRows = 128;       // queries of a tile (UMMA M)
-constexpr int kBN = 64;          // tokens of a K/V tile
-constexpr int kStages = 4;
+// Tokens of a step. Scores in products of 128 columns take as long as in products of 64 (counters: the tensor pipe was busy for
+// 1600 cycles per 64 tokens and two query tiles instead of 1024).
+constexpr int kBN = 128;
+constexpr int kStages = 2;
 constexpr int kWarps = 12;
 constexpr int kThreads = 32 * kWarps;
 constexpr float kRescaleStep = 8.0f;   // log2 units
 constexpr uint32_t kMinShare = 2;      // tiles of a worker's share, at least
-// Time of a unit of pieces, in tiles of own tokens that a CTA streams meanwhile: once, and for each of its K/V tiles.
-constexpr uint32_t kUnitCost = 30, kTileCost = 12;
+// Time of a unit of pieces, in tiles of own tokens that a CTA streams meanwhile: once, and for each of its steps.
+constexpr uint32_t kUnitCost = 40, kTileCost = 16;
 template <int D>
 constexpr int ring_of() { return 256 / D; }   // tiles of a worker's ring: 16 KB
 
 struct __align__(8) Bars {
-  uint64_t q_full, q_empty;
-  uint64_t kv_full[kStages];
-  uint64_t kv_empty[kStages];
-  uint64_t s_full[2][2];
+  uint64_t q_full, q_empty[2];
+  uint64_t k_full[kStages], k_empty[kStages];
+  uint64_t v_full[kStages], v_empty[kStages];
+  uint64_t s_full[2];
   uint64_t p_full[2];
   uint64_t pv_done[2];
   uint64_t own_full[kWarps][4];
@@ -96,18 +98,16 @@ __device__ __forceinline__ int row_units(const XpDecodeAttnArgs& a) { return a.q
 
 // Bounded wait of a converged warp that also gives up when another role of the CTA has; one answer for all lanes.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Bars* b, uint32_t site) {
-  bool ok = sm100::mbar_try_wait(bar, parity);
-  if (!ok) {
-    const uint64_t deadline = sm100::global_timer_ns() + sm100::kPipelineWaitNs;
-    uint32_t spins = 0;
-    while (!(ok = sm100::mbar_try_wait(bar, parity))) {
-      if ((++spins & 0xffu) == 0) {
-        if (b->abort_flag != 0) break;
-        if (sm100::global_timer_ns() > deadline) {
-          b->abort_flag = site;
-          break;
-        }
-      }
+  bool ok = false;
+  uint64_t deadline = 0;                            // the timer is read only once a wait has become a long one
+  for (uint32_t spins = 1; !(ok = sm100::mbar_try_wait(bar, parity)); ++spins) {
+    if ((spins & 0xffu) != 0) continue;
+    if (b->abort_flag != 0) break;
+    const uint64_t now = sm100::global_timer_ns();
+    if (deadline == 0) deadline = now + sm100::kPipelineWaitNs;
+    if (now > deadline) {
+      b->abort_flag = site;
+      break;
     }
   }
   return __all_sync(0xffffffffu, ok) != 0;
@@ -123,6 +123,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// Two weights (not negative) rounded to bf16, ties up. The conversion instruction runs on the unit of the exponentials, an eighth of
+// a warp a cycle, and made it half as busy again; additions and a byte permutation do not. (NaN may be lost here; the sum keeps it.)
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+  return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632);
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -330,6 +335,15 @@ __device__ __forceinline__ void own_worker(const CUtensorMap* tmap_k, const CUte
   }
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
 shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
@@ -342,7 +356,8 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   constexpr int kKTile = kHalves * kKVHalf;
   constexpr int kStage = 2 * kKTile;              // K then V
   constexpr uint32_t kTmemCols = 512;
-  constexpr uint32_t kOCol = 4 * kBN;             // S: two buffers per tile; O_A behind them, then O_B
+  constexpr uint32_t kOCol = 2 * kBN;             // S_A, S_B (P over the second half of either), then O_A, O_B
+  constexpr uint32_t kPCol = kBN / 2;
   extern __shared__ uint8_t smem_dyn[];
   __shared__ Bars bars;
 
@@ -360,16 +375,24 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   const int turns = (n_units + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x), busy = turns > 0 ? (n_units + turns - 1) / turns : 0;
   const bool has_units = static_cast<int>(blockIdx.x) < busy;
 
+  if (threadIdx.x == 32) {
+    sm100::tma_prefetch_desc(&tmap_k16);
+    sm100::tma_prefetch_desc(&tmap_v16);
+    sm100::tma_prefetch_desc(&tmap_q);
+    sm100::tma_prefetch_desc(&tmap_k);
+    sm100::tma_prefetch_desc(&tmap_v);
+  }
   if (threadIdx.x == 0) {
     sm100::mbar_init(&bars.q_full, 1);
-    sm100::mbar_init(&bars.q_empty, 1);
     for (int s = 0; s < kStages; ++s) {
-      sm100::mbar_init(&bars.kv_full[s], 1);
-      sm100::mbar_init(&bars.kv_empty[s], 1);
+      sm100::mbar_init(&bars.k_full[s], 1);
+      sm100::mbar_init(&bars.k_empty[s], 1);
+      sm100::mbar_init(&bars.v_full[s], 1);
+      sm100::mbar_init(&bars.v_empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
-      sm100::mbar_init(&bars.s_full[x][0], 1);
-      sm100::mbar_init(&bars.s_full[x][1], 1);
+      sm100::mbar_init(&bars.q_empty[x], 4);
+      sm100::mbar_init(&bars.s_full[x], 1);
       sm100::mbar_init(&bars.p_full[x], 4);
       sm100::mbar_init(&bars.pv_done[x], 1);
     }
@@ -394,41 +417,41 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   } else if (warp == 8) {
     // ------------------------------------------------------------------ TMA producer
     const int page_shift = 31 - __clz(a.page_size), page_mask = a.page_size - 1;
-    const int boxes = kBN / box_tokens, box_bytes = box_tokens * 128;
+    const int copies = kHalves * (kBN / box_tokens);
     const uint32_t q_bytes = static_cast<uint32_t>(2 * kHalves * np * G * 128);
-    int it = 0, ord = 0;
-    bool ok = true;
+    int it = 0, ord = 0, both = 0;                // stages; units; units of two query tiles
+    bool ok = true, two = false;
     for (int u = blockIdx.x; ok && u < n_units; u += busy, ++ord) {
       const XpPrefixPiece p = args.pieces[u / a.kv_heads];
       const int hk = u % a.kv_heads;
       const int* table = a.block_table + static_cast<size_t>(p.leader) * a.max_blocks;
-      if (ord > 0 && !wait_bar(&bars.q_empty, (ord - 1) & 1, &bars, 1)) break;
+      if (ord > 0 && !wait_bar(&bars.q_empty[0], (ord - 1) & 1, &bars, 1)) break;
+      if (two && !wait_bar(&bars.q_empty[1], (both - 1) & 1, &bars, 1)) break;
+      two = p.rows > np, both += two;
       if (lane == 0) sm100::mbar_arrive_expect_tx(&bars.q_full, q_bytes);
       __syncwarp();
       if (lane < 2 * kHalves) {
         const int x = lane / kHalves, h = lane % kHalves;
         sm100::tma_load_3d_addr(q_s + x * kQTile + h * kQHalf, &tmap_q, sm100::smem_u32(&bars.q_full), h * 64, hk * G, p.row0 + x * np);
       }
-      const int n_tiles = (p.tok1 - p.tok0 + kBN - 1) / kBN;
-      for (int t = 0; t < n_tiles; ++t, ++it) {
+      const int n_steps = (p.tok1 - p.tok0 + kBN - 1) / kBN;
+      for (int t = 0; t < n_steps; ++t, ++it) {
         const int s = it % kStages;
-        if (it >= kStages && !(ok = wait_bar(&bars.kv_empty[s], ((it / kStages) - 1) & 1, &bars, 2))) break;
-        if (lane == 0) sm100::mbar_arrive_expect_tx(&bars.kv_full[s], kStage);
-        __syncwarp();
-        const uint32_t full = sm100::smem_u32(&bars.kv_full[s]), dst = kv_s + s * kStage;
-        if (boxes == 1) {
-          if (lane < 2) {
-            const int tk = p.tok0 + t * kBN;
+        for (int is_v = 0; ok && is_v < 2; ++is_v) {
+          uint64_t* full = is_v ? &bars.v_full[s] : &bars.k_full[s];
+          if (it >= kStages && !(ok = wait_bar(is_v ? &bars.v_empty[s] : &bars.k_empty[s], ((it / kStages) - 1) & 1, &bars, 2))) break;
+          if (lane == 0) sm100::mbar_arrive_expect_tx(full, kKTile);
+          __syncwarp();
+          if (lane < copies) {                     // up to 16: blocks of 64 dims, boxes of tokens
+            const int h = lane % kHalves, j = lane / kHalves;
+            // boxes behind the end repeat the last one
+            const int tk = min(p.tok0 + t * kBN + j * box_tokens, (p.tok1 - 1) & ~(box_tokens - 1));
             const int tok = (table[tk >> page_shift] << page_shift) + (tk & page_mask);
-            sm100::tma_load_4d_addr(dst + lane * kKTile, lane ? &tmap_v : &tmap_k, full, 0, tok, 0, hk);
+            sm100::tma_load_3d_addr(kv_s + s * kStage + is_v * kKTile + h * kKVHalf + j * box_tokens * 128, is_v ? &tmap_v : &tmap_k,
+                                    sm100::smem_u32(full), h * 64, hk, tok);
           }
-        } else if (lane < 2 * boxes * kHalves) {
-          const int h = lane % kHalves, is_v = (lane / kHalves) & 1, j = lane / (2 * kHalves);
-          // boxes behind the end repeat the last one
-          const int tk = min(p.tok0 + t * kBN + j * box_tokens, (p.tok1 - 1) & ~(box_tokens - 1));
-          const int tok = (table[tk >> page_shift] << page_shift) + (tk & page_mask);
-          sm100::tma_load_3d_addr(dst + is_v * kKTile + h * kKVHalf + j * box_bytes, is_v ? &tmap_v : &tmap_k, full, h * 64, hk, tok);
         }
+        if (!ok) break;
       }
     }
   } else if (warp == 9) {
@@ -436,58 +459,55 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const bool leader = sm100::elect_one();
     const uint32_t idesc_s = sm100::umma_idesc_bf16(kRows, kBN);
     const uint32_t idesc_o = sm100::umma_idesc_bf16_bmn(kRows, D);
-    int it = 0, ord = 0, count[2] = {0, 0};       // K/V tiles; units; tiles that query tile A (B) has multiplied
-    auto issue_s = [&](int x, int i, int c) {     // S_x = Q_x K(i)^T into buffer c & 1
+    int it = 0, ord = 0, count[2] = {0, 0};       // stages; units; steps that query tile A (B) has multiplied
+    auto issue_s = [&](int x, int i) {            // S_x = Q_x K(i)^T
       if (!leader) return;
-      const uint32_t d = tmem + static_cast<uint32_t>((x * 2 + (c & 1)) * kBN);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
         const uint64_t da = sm100::umma_desc_sw128(q_s + x * kQTile + (ks >> 2) * kQHalf) + (ks & 3) * 2;
         const uint64_t db = sm100::umma_desc_sw128(kv_s + (i % kStages) * kStage + (ks >> 2) * kKVHalf) + (ks & 3) * 2;
-        sm100::umma_bf16(d, da, db, idesc_s, ks > 0 ? 1u : 0u);
+        sm100::umma_bf16(tmem + static_cast<uint32_t>(x * kBN), da, db, idesc_s, ks > 0 ? 1u : 0u);
       }
-      sm100::umma_commit(&bars.s_full[x][c & 1]);
+      sm100::umma_commit(&bars.s_full[x]);
     };
-    auto issue_pv = [&](int x, int i, int c, bool more) {   // O_x (+)= P_x V(i)
+    auto issue_pv = [&](int x, int i, bool more) {   // O_x (+)= P_x V(i)
       if (!leader) return;
-      const uint32_t d = tmem + kOCol + static_cast<uint32_t>(x * D);
 #pragma unroll
       for (int kk = 0; kk < kBN / 16; ++kk) {
         const uint64_t db = sm100::umma_desc_mn_sw128(kv_s + (i % kStages) * kStage + kKTile + kk * 2048, kKVHalf, 1024);
-        // P sits in the first 32 columns of the S buffer it was computed from, 8 columns per K step
-        sm100::umma_bf16_ts(d, tmem + static_cast<uint32_t>((x * 2 + (c & 1)) * kBN + kk * 8), db, idesc_o, (more || kk > 0) ? 1u : 0u);
+        sm100::umma_bf16_ts(tmem + kOCol + static_cast<uint32_t>(x * D), tmem + static_cast<uint32_t>(x * kBN + kPCol + kk * 8), db, idesc_o,
+                            (more || kk > 0) ? 1u : 0u);
       }
       sm100::umma_commit(&bars.pv_done[x]);
     };
     bool ok = true;
     for (int u = blockIdx.x; ok && u < n_units; u += busy, ++ord) {
       const XpPrefixPiece p = args.pieces[u / a.kv_heads];
-      const int n_tiles = (p.tok1 - p.tok0 + kBN - 1) / kBN, tiles_x = p.rows > np ? 2 : 1;
-      ok = wait_bar(&bars.q_full, ord & 1, &bars, 3) && wait_bar(&bars.kv_full[it % kStages], (it / kStages) & 1, &bars, 4);
+      const int n_steps = (p.tok1 - p.tok0 + kBN - 1) / kBN, tiles_x = p.rows > np ? 2 : 1;
+      ok = wait_bar(&bars.q_full, ord & 1, &bars, 3) && wait_bar(&bars.k_full[it % kStages], (it / kStages) & 1, &bars, 4);
       if (!ok) break;
       sm100::tc_fence_after_sync();
-      for (int x = 0; x < tiles_x; ++x) issue_s(x, it, count[x]);
-      if (n_tiles == 1 && leader) sm100::umma_commit(&bars.q_empty);
-      for (int t = 0; ok && t < n_tiles; ++t) {
-        const bool next = t + 1 < n_tiles;
-        const int i = it + t;
-        if (next) ok = wait_bar(&bars.kv_full[(i + 1) % kStages], ((i + 1) / kStages) & 1, &bars, 5);
+      for (int x = 0; x < tiles_x; ++x) issue_s(x, it);
+      if (leader) sm100::umma_commit(&bars.k_empty[it % kStages]);
+      for (int t = 0; ok && t < n_steps; ++t, ++it) {
         for (int x = 0; ok && x < tiles_x; ++x) {
-          const int c = count[x];
-          if (next) {
-            sm100::tc_fence_after_sync();
-            issue_s(x, i + 1, c + 1);
-            if (t + 2 == n_tiles && x + 1 == tiles_x && leader) sm100::umma_commit(&bars.q_empty);   // the unit's last use of Q
-          }
-          ok = wait_bar(&bars.p_full[x], c & 1, &bars, 6);
+          ok = wait_bar(&bars.p_full[x], count[x] & 1, &bars, 6);
+          if (ok && x == 0) ok = wait_bar(&bars.v_full[it % kStages], (it / kStages) & 1, &bars, 12);
           if (!ok) break;
           sm100::tc_fence_after_sync();
-          issue_pv(x, i, c, t > 0);
-          count[x] = c + 1;
+          issue_pv(x, it, t > 0);
+          if (x + 1 == tiles_x && leader) sm100::umma_commit(&bars.v_empty[it % kStages]);
+          ++count[x];
+          if (t + 1 < n_steps) {
+            // the products run in order: the next scores overwrite the weights that the product before them has read
+            if (x == 0) ok = wait_bar(&bars.k_full[(it + 1) % kStages], ((it + 1) / kStages) & 1, &bars, 5);
+            if (!ok) break;
+            sm100::tc_fence_after_sync();
+            issue_s(x, it + 1);
+            if (x + 1 == tiles_x && leader) sm100::umma_commit(&bars.k_empty[(it + 1) % kStages]);
+          }
         }
-        if (ok && leader) sm100::umma_commit(&bars.kv_empty[i % kStages]);
       }
-      it += n_tiles;
     }
   } else {
     // ------------------------------------------------------------------ softmax and partial results (warps 0-7)
@@ -497,34 +517,43 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t o_t = tmem + lane_off + kOCol + static_cast<uint32_t>(x * D);
     const float sc2 = a.scale * 1.4426950408889634f;
+    const uint32_t s_t = tmem + lane_off + static_cast<uint32_t>(x * kBN);
+    const uint32_t stage = q_s + x * kQTile + (warp & 3) * 4096;   // over the queries of this tile, when they are done with
     int it = 0, c = 0;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < n_units; u += busy) {
       const XpPrefixPiece p = args.pieces[u / a.kv_heads];
-      const int n_tiles = (p.tok1 - p.tok0 + kBN - 1) / kBN;
+      const int n_steps = (p.tok1 - p.tok0 + kBN - 1) / kBN;
       if (x == 0 || p.rows > np) {
         float m_used = -CUDART_INF_F, l = 0.f;
-        for (int t = 0; t < n_tiles; ++t, ++c) {
-          ok = wait_bar(&bars.s_full[x][c & 1], (c >> 1) & 1, &bars, 7);
+        for (int t = 0; t < n_steps; ++t, ++c) {
+          ok = wait_bar(&bars.s_full[x], c & 1, &bars, 7);
           if (!ok) break;
           sm100::tc_fence_after_sync();
-          uint32_t sv[kBN];
-          const uint32_t s_t = tmem + lane_off + static_cast<uint32_t>((x * 2 + (c & 1)) * kBN);
-          sm100::tmem_ld32_issue(s_t, sv);
-          sm100::tmem_ld32_issue(s_t + 32, sv + 32);
-          sm100::tmem_ld_wait_all(sv);
-          sm100::tmem_ld_wait_all(sv + 32);
-          const int nvis = p.tok1 - p.tok0 - t * kBN;       // tokens of the prefix in this tile (a uniform number)
-          if (nvis < kBN) {
+          uint32_t lo[kBN / 2], hi[kBN / 2];
+          sm100::tmem_ld32_issue(s_t, lo);
+          sm100::tmem_ld32_issue(s_t + 32, lo + 32);
+          sm100::tmem_ld32_issue(s_t + 64, hi);
+          sm100::tmem_ld32_issue(s_t + 96, hi + 32);
+          sm100::tmem_ld_wait_all(lo);
+          sm100::tmem_ld_wait_all(lo + 32);
+          sm100::tmem_ld_wait_all(hi);
+          sm100::tmem_ld_wait_all(hi + 32);
+          const int nvis = p.tok1 - p.tok0 - t * kBN;       // tokens of the prefix in this step (a uniform number)
+          auto cut = [&](uint32_t (&v)[kBN / 2], int n) {
+            if (n < kBN / 2) {
 #pragma unroll
-            for (int j = 0; j < kBN; ++j)
-              if (j >= nvis) sv[j] = 0xff800000u;           // -inf: selected, never computed with
-          }
+              for (int j = 0; j < kBN / 2; ++j)
+                if (j >= n) v[j] = 0xff800000u;             // -inf: selected, never computed with
+            }
+          };
+          cut(lo, nvis);
+          cut(hi, nvis - kBN / 2);
           float mx4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-          for (int j = 0; j < kBN; j += 8) {
+          for (int j = 0; j < kBN / 2; j += 4) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], __uint_as_float(sv[j + 2 * e]), __uint_as_float(sv[j + 2 * e + 1]));
+            for (int e = 0; e < 4; ++e) mx4[e] = max3(mx4[e], __uint_as_float(lo[j + e]), __uint_as_float(hi[j + e]));
           }
           const float m_new = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sc2;
           float factor = 1.f;
@@ -535,39 +564,30 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             }
           }
           const float m_sub = m_used == -CUDART_INF_F ? 0.f : m_used;
+          // P as the tensor core's A operand: two bf16 to a column, over the second half of S
           float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t pk[kBN / 2];
+          auto weights = [&](const uint32_t* v, uint32_t to) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int j = 0; j < kBN; j += 2) {
-            const float p0 = sm100::ex2_approx(fmaf(__uint_as_float(sv[j]), sc2, -m_sub));
-            const float p1 = sm100::ex2_approx(fmaf(__uint_as_float(sv[j + 1]), sc2, -m_sub));
-            sum4[(j >> 1) & 3] += p0 + p1;
-            pk[j >> 1] = pack2(p0, p1);
-          }
-          l = l * factor + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
-          const bool rescale = t > 0 && __any_sync(0xffffffffu, factor != 1.f);
-          if (rescale) {
-            // the previous second product must have retired: it accumulates into O
-            ok = wait_bar(&bars.pv_done[x], (c - 1) & 1, &bars, 8);
-            if (!ok) break;
-            sm100::tc_fence_after_sync();
-#pragma unroll 1
-            for (int e = 0; e < D; e += 32) {
-              uint32_t ov[32];
-              sm100::tmem_ld32_issue(o_t + e, ov);
-              sm100::tmem_ld_wait_all(ov);
-#pragma unroll
-              for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * factor);
-              sm100::tmem_st32(o_t + e, ov);
+            for (int j = 0; j < 32; j += 2) {
+              const float p0 = sm100::ex2_approx(fmaf(__uint_as_float(v[j]), sc2, -m_sub));
+              const float p1 = sm100::ex2_approx(fmaf(__uint_as_float(v[j + 1]), sc2, -m_sub));
+              sum4[(j >> 1) & 3] += p0 + p1;
+              pk[j >> 1] = pack_weights(p0, p1);
             }
-            sm100::tmem_st_wait();
-          }
-          // P as the tensor core's A operand: 32 columns of two bf16 each, over the start of the S buffer
-          sm100::tmem_st32(s_t, pk);
+            tmem_st16(to, pk);
+          };
+          weights(lo, s_t + kPCol);
+          weights(lo + 32, s_t + kPCol + 16);
+          weights(hi, s_t + kPCol + 32);
+          weights(hi + 32, s_t + kPCol + 48);
+          l = l * factor + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
           if (nvis < kBN && x == 0) {
             // cache slots behind the prefix may hold anything: zero those V rows (a weight of zero times NaN). Tile A's product
             // is issued before tile B's, and both read this stage.
             const uint32_t v_s = kv_s + ((it + t) % kStages) * kStage + kKTile;
+            ok = wait_bar(&bars.v_full[(it + t) % kStages], ((it + t) / kStages) & 1, &bars, 13);
+            if (!ok) break;
             for (int i = row; i < (kBN - nvis) * (D / 8); i += kRows) {
               const int R = nvis + i / (D / 8), cc = i % (D / 8);
               const uint32_t off = (cc >> 3) * kKVHalf + R * 128 + (((cc & 7) ^ (R & 7)) << 4);
@@ -575,39 +595,66 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             }
             sm100::fence_proxy_async_smem();
           }
+          if (t > 0) {
+            // the previous second product accumulates into O; it has retired before these scores were complete
+            ok = wait_bar(&bars.pv_done[x], (c - 1) & 1, &bars, 8);
+            if (!ok) break;
+            if (__any_sync(0xffffffffu, factor != 1.f)) {
+              sm100::tc_fence_after_sync();
+#pragma unroll 1
+              for (int e = 0; e < D; e += 32) {
+                uint32_t ov[32];
+                sm100::tmem_ld32_issue(o_t + e, ov);
+                sm100::tmem_ld_wait_all(ov);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * factor);
+                sm100::tmem_st32(o_t + e, ov);
+              }
+            }
+          }
           sm100::tmem_st_wait();
           sm100::tc_fence_before_sync();
-          // every phase of pv_done is consumed in order, before the arrival below lets the next one complete
-          if (t > 0 && !rescale) {
-            ok = wait_bar(&bars.pv_done[x], (c - 1) & 1, &bars, 9);
-            if (!ok) break;
-          }
           __syncwarp();
           if (lane == 0) sm100::mbar_arrive(&bars.p_full[x]);
         }
         if (ok) ok = wait_bar(&bars.pv_done[x], (c - 1) & 1, &bars, 10);
         if (ok) {
+          // The partial result goes out through shared memory, 128 bytes of a row at a time: stored from the lanes that hold the
+          // rows, 256 rows of 512 bytes kept the store unit for 4 us.
           sm100::tc_fence_after_sync();
           const int r = x * np + pos;
           const bool stored = pos < np && r < p.rows;
-          const int hq = (u % a.kv_heads) * G + head;
-          const Partials to(args, D, p.row0 + (stored ? r : 0), min(hq, a.q_heads - 1));
+          const Partials to(args, D, p.row0 + (stored ? r : 0), min((u % a.kv_heads) * G + head, a.q_heads - 1));
+          const unsigned long long mine = stored ? reinterpret_cast<unsigned long long>(to.sums + static_cast<size_t>(p.part) * D) : 0ull;
+          if (stored) to.pairs[p.part] = make_float2(m_used, l);
 #pragma unroll 1
           for (int e = 0; e < D; e += 32) {
             uint32_t ov[32];
             sm100::tmem_ld32_issue(o_t + e, ov);
             sm100::tmem_ld_wait_all(ov);
-            if (stored) {
-              uint4* o = reinterpret_cast<uint4*>(to.sums + static_cast<size_t>(p.part) * D + e);
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) o[j / 4] = make_uint4(ov[j], ov[j + 1], ov[j + 2], ov[j + 3]);
+            for (int j = 0; j < 8; ++j)
+              asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((j ^ (lane & 7)) << 4)), "r"(ov[4 * j]), "r"(ov[4 * j + 1]),
+                           "r"(ov[4 * j + 2]), "r"(ov[4 * j + 3])
+                           : "memory");
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int rr = j * 4 + (lane >> 3), cc = lane & 7;
+              const unsigned long long o = __shfl_sync(0xffffffffu, mine, rr);
+              uint4 v;
+              asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(stage + rr * 128 + ((cc ^ (rr & 7)) << 4)));
+              if (o != 0) reinterpret_cast<uint4*>(o)[e / 4 + cc] = v;
             }
+            __syncwarp();
           }
-          if (stored) to.pairs[p.part] = make_float2(m_used, l);
           sm100::tc_fence_before_sync();       // O has been read before the next unit's first arrival at p_full
+          sm100::fence_proxy_async_smem();     // the next queries are copied over the staged rows
+          __syncwarp();
+          if (lane == 0) sm100::mbar_arrive(&bars.q_empty[x]);
         }
       }
-      it += n_tiles;
+      it += n_steps;
     }
   }
   // ------------------------------------------------------------------ own tokens, over the memory of the pieces' tiles
@@ -656,8 +703,9 @@ shared_merge_kernel(XpDecodeSharedArgs args, int G) {
   __shared__ float wt[16][kMost + 1];               // weights, then 1 / sum of weights
   const XpDecodeAttnArgs& a = args.a;
   const int hk = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int shared = shared_tokens(args, b), parts = shared > 0 ? args.row_parts[b] : 0, tiles = (row_tokens(args, b) - shared + 15) >> 4;
   const uint32_t* words = share_words(args, D);
+  const int shared = shared_tokens(args, b), most_parts = b < args.plan_rows ? args.row_parts[b] : 0;
+  const int parts = shared > 0 ? most_parts : 0, tiles = (row_tokens(args, b) - shared + 15) >> 4;
   const Shares cut{words[0], words[1], words[2]};
   const uint32_t units = row_units(a), row0 = words[4 + b] * units;
   // shares that hold tiles of a unit of this row
@@ -688,7 +736,7 @@ shared_merge_kernel(XpDecodeSharedArgs args, int G) {
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) wt[g][kMost] = sum > 0.f ? 1.f / sum : 0.f;
+    if (lane == 0) wt[g][kMost] = sum == 0.f ? 0.f : 1.f / sum;      // a row without tokens gives zeros
   }
   __syncthreads();
   for (int i = threadIdx.x * 4; i < G * D; i += kMergeThreads * 4) {
@@ -725,13 +773,10 @@ static int launch(const XpDecodeSharedArgs& args, cudaStream_t s) {
   const XpDecodeAttnArgs& a = args.a;
   const int G = a.q_heads / a.kv_heads;
   const uint64_t tokens = static_cast<uint64_t>(a.num_pages) * a.page_size;
-  const int box_tokens = a.page_size >= kBN ? kBN : 16;   // one copy brings a whole K (or V) tile, or 16 tokens and 64 dims
+  const int box_tokens = a.page_size >= 64 ? 64 : 16;     // a copy brings so many tokens and 64 dims
   CUtensorMap mq, mk, mv, mk16, mv16;
   if (tmap::cache().get_kv(&mk16, a.k_cache, tokens, a.kv_heads, D) != 0 || tmap::cache().get_kv(&mv16, a.v_cache, tokens, a.kv_heads, D) != 0) return -20;
-  mk = mk16, mv = mv16;
-  if (box_tokens == kBN && (tmap::cache().get_kv4(&mk, a.k_cache, tokens, a.kv_heads, D, kBN) != 0 ||
-                            tmap::cache().get_kv4(&mv, a.v_cache, tokens, a.kv_heads, D, kBN) != 0))
-    return -20;
+  if (tmap::cache().get_kv(&mk, a.k_cache, tokens, a.kv_heads, D, box_tokens) != 0 || tmap::cache().get_kv(&mv, a.v_cache, tokens, a.kv_heads, D, box_tokens) != 0) return -20;
   if (tmap::cache().get_q(&mq, a.q, static_cast<uint64_t>(a.batch), a.q_heads, D, G, kRows / G) != 0) return -20;
   constexpr int kTiles = 2 * (D / 64) * kRows * 128 + kStages * 2 * (D / 64) * kBN * 128, kRings = kWarps * ring_of<D>() * 16 * D * 4;
   constexpr int kSmem = (kTiles > kRings ? kTiles : kRings) + (2 * XP_PREFIX_ROWS + 1) * 4 + 1024;

@@ -119,7 +119,7 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
 # ---------------------------------------------------------------------------------------------- shared prefixes
 
 PREFIX_TOKENS = 16      # prefixes are shared in whole tiles of so many tokens; the rest of one is read by every row
-PIECE_TOKENS = 64       # pieces of a prefix begin at multiples of this
+PIECE_TOKENS = 128      # pieces of a prefix begin at multiples of this
 MAX_PARTS = 32          # pieces of one prefix
 MAX_SHARED_ROWS = 4096  # rows of a batch
 

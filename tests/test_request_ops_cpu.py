@@ -34,7 +34,7 @@ def test_pieces_cover_every_prefix_once(sizes, prefixes, rows, hq, hk):
     starts = np.cumsum([0] + list(sizes))
     for leader, row0, n, t0, t1, part, *_ in pieces.tolist():
         assert leader in starts and leader <= row0 and row0 + n <= starts[starts > leader][0]
-        assert 0 < n <= per and t0 % 64 == 0 and t1 % 16 == 0 and t0 < t1 <= want[row0]
+        assert 0 < n <= per and t0 % A.PIECE_TOKENS == 0 and t1 % 16 == 0 and t0 < t1 <= want[row0]
         for r in range(row0, row0 + n):
             assert part not in [x[2] for x in seen[r]] and part < parts[r]
             seen[r].add((t0, t1, part))
