@@ -57,7 +57,7 @@ struct __align__(8) Bars {
   uint64_t k_full[kStages], k_empty[kStages];
   uint64_t v_full[kStages], v_empty[kStages];
   uint64_t s_full[2];
-  uint64_t p_full[2];
+  uint64_t p_half[2], p_full[2];
   uint64_t pv_done[2];
   uint64_t own_full[kWarps][4];
   uint32_t tmem_base;
@@ -127,6 +127,27 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // a warp a cycle, and made it half as busy again; additions and a byte permutation do not. (NaN may be lost here; the sum keeps it.)
 __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
   return __byte_perm(__float_as_uint(lo) + 0x8000u, __float_as_uint(hi) + 0x8000u, 0x7632);
+}
+// Two fp32 numbers in one register pair, computed by one instruction.
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float2 parts_of(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
@@ -335,6 +356,13 @@ __device__ __forceinline__ void own_worker(const CUtensorMap* tmap_k, const CUte
   }
 }
 
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -393,6 +421,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
     for (int x = 0; x < 2; ++x) {
       sm100::mbar_init(&bars.q_empty[x], 4);
       sm100::mbar_init(&bars.s_full[x], 1);
+      sm100::mbar_init(&bars.p_half[x], 4);
       sm100::mbar_init(&bars.p_full[x], 4);
       sm100::mbar_init(&bars.pv_done[x], 1);
     }
@@ -470,15 +499,15 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       }
       sm100::umma_commit(&bars.s_full[x]);
     };
-    auto issue_pv = [&](int x, int i, bool more) {   // O_x (+)= P_x V(i)
+    auto issue_pv = [&](int x, int i, int half, bool more) {   // O_x (+)= P_x V(i), tokens of one half of the step
       if (!leader) return;
 #pragma unroll
-      for (int kk = 0; kk < kBN / 16; ++kk) {
+      for (int kk = half * (kBN / 32); kk < (half + 1) * (kBN / 32); ++kk) {
         const uint64_t db = sm100::umma_desc_mn_sw128(kv_s + (i % kStages) * kStage + kKTile + kk * 2048, kKVHalf, 1024);
         sm100::umma_bf16_ts(tmem + kOCol + static_cast<uint32_t>(x * D), tmem + static_cast<uint32_t>(x * kBN + kPCol + kk * 8), db, idesc_o,
                             (more || kk > 0) ? 1u : 0u);
       }
-      sm100::umma_commit(&bars.pv_done[x]);
+      if (half) sm100::umma_commit(&bars.pv_done[x]);
     };
     bool ok = true;
     for (int u = blockIdx.x; ok && u < n_units; u += busy, ++ord) {
@@ -491,11 +520,15 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
       if (leader) sm100::umma_commit(&bars.k_empty[it % kStages]);
       for (int t = 0; ok && t < n_steps; ++t, ++it) {
         for (int x = 0; ok && x < tiles_x; ++x) {
-          ok = wait_bar(&bars.p_full[x], count[x] & 1, &bars, 6);
+          ok = wait_bar(&bars.p_half[x], count[x] & 1, &bars, 6);
           if (ok && x == 0) ok = wait_bar(&bars.v_full[it % kStages], (it / kStages) & 1, &bars, 12);
           if (!ok) break;
           sm100::tc_fence_after_sync();
-          issue_pv(x, it, t > 0);
+          issue_pv(x, it, 0, t > 0);
+          ok = wait_bar(&bars.p_full[x], count[x] & 1, &bars, 14);
+          if (!ok) break;
+          sm100::tc_fence_after_sync();
+          issue_pv(x, it, 1, true);
           if (x + 1 == tiles_x && leader) sm100::umma_commit(&bars.v_empty[it % kStages]);
           ++count[x];
           if (t + 1 < n_steps) {
@@ -564,24 +597,23 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             }
           }
           const float m_sub = m_used == -CUDART_INF_F ? 0.f : m_used;
-          // P as the tensor core's A operand: two bf16 to a column, over the second half of S
-          float sum4[4] = {0.f, 0.f, 0.f, 0.f};
-          auto weights = [&](const uint32_t* v, uint32_t to) {
-            uint32_t pk[16];
+          if (t > 0) {
+            // the previous second product accumulates into O; it has retired before these scores were complete
+            ok = wait_bar(&bars.pv_done[x], (c - 1) & 1, &bars, 8);
+            if (!ok) break;
+            if (__any_sync(0xffffffffu, factor != 1.f)) {
+              sm100::tc_fence_after_sync();
+#pragma unroll 1
+              for (int e = 0; e < D; e += 16) {
+                uint32_t ov[16];
+                sm100::tmem_ld16_issue(o_t + e, ov);
+                tmem_ld_wait16(ov);
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float p0 = sm100::ex2_approx(fmaf(__uint_as_float(v[j]), sc2, -m_sub));
-              const float p1 = sm100::ex2_approx(fmaf(__uint_as_float(v[j + 1]), sc2, -m_sub));
-              sum4[(j >> 1) & 3] += p0 + p1;
-              pk[j >> 1] = pack_weights(p0, p1);
+                for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * factor);
+                tmem_st16(o_t + e, ov);
+              }
             }
-            tmem_st16(to, pk);
-          };
-          weights(lo, s_t + kPCol);
-          weights(lo + 32, s_t + kPCol + 16);
-          weights(hi, s_t + kPCol + 32);
-          weights(hi + 32, s_t + kPCol + 48);
-          l = l * factor + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+          }
           if (nvis < kBN && x == 0) {
             // cache slots behind the prefix may hold anything: zero those V rows (a weight of zero times NaN). Tile A's product
             // is issued before tile B's, and both read this stage.
@@ -595,27 +627,36 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
             }
             sm100::fence_proxy_async_smem();
           }
-          if (t > 0) {
-            // the previous second product accumulates into O; it has retired before these scores were complete
-            ok = wait_bar(&bars.pv_done[x], (c - 1) & 1, &bars, 8);
-            if (!ok) break;
-            if (__any_sync(0xffffffffu, factor != 1.f)) {
-              sm100::tc_fence_after_sync();
-#pragma unroll 1
-              for (int e = 0; e < D; e += 32) {
-                uint32_t ov[32];
-                sm100::tmem_ld32_issue(o_t + e, ov);
-                sm100::tmem_ld_wait_all(ov);
+          // P as the tensor core's A operand: two bf16 to a column, over the second half of S. The second product begins with the
+          // step's first half while the weights of the second are computed.
+          const uint64_t scale_pair = pair_of(__float_as_uint(sc2), __float_as_uint(sc2));
+          const uint64_t off_pair = pair_of(__float_as_uint(-m_sub), __float_as_uint(-m_sub));
+          uint64_t sum2[2] = {0, 0};
+          auto weights = [&](const uint32_t* v, uint32_t to) {
+            uint32_t pk[16];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * factor);
-                sm100::tmem_st32(o_t + e, ov);
-              }
+            for (int j = 0; j < 32; j += 2) {
+              const float2 e = parts_of(fma2(pair_of(v[j], v[j + 1]), scale_pair, off_pair));
+              const float p0 = sm100::ex2_approx(e.x), p1 = sm100::ex2_approx(e.y);
+              sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], pair_of(__float_as_uint(p0), __float_as_uint(p1)));
+              pk[j >> 1] = pack_weights(p0, p1);
             }
-          }
-          sm100::tmem_st_wait();
-          sm100::tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) sm100::mbar_arrive(&bars.p_full[x]);
+            tmem_st16(to, pk);
+          };
+          auto hand_over = [&](uint64_t* bar) {
+            sm100::tmem_st_wait();
+            sm100::tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(bar);
+          };
+          weights(lo, s_t + kPCol);
+          weights(lo + 32, s_t + kPCol + 16);
+          hand_over(&bars.p_half[x]);
+          weights(hi, s_t + kPCol + 32);
+          weights(hi + 32, s_t + kPCol + 48);
+          hand_over(&bars.p_full[x]);
+          const float2 sum = parts_of(add2(sum2[0], sum2[1]));
+          l = l * factor + (sum.x + sum.y);
         }
         if (ok) ok = wait_bar(&bars.pv_done[x], (c - 1) & 1, &bars, 10);
         if (ok) {
