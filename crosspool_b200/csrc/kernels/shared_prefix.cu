@@ -48,7 +48,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr float kRescaleStep = 8.0f;   // log2 units
 constexpr uint32_t kMinShare = 2;      // tiles of a worker's share, at least
 // Time of a unit of pieces, in tiles of own tokens that a CTA streams meanwhile: once, and for each of its steps.
-constexpr uint32_t kUnitCost = 40, kTileCost = 16;
+constexpr uint32_t kUnitCost = 35, kTileCost = 19;
 template <int D>
 constexpr int ring_of() { return 256 / D; }   // tiles of a worker's ring: 16 KB
 
@@ -62,7 +62,7 @@ struct __align__(8) Bars {
   uint64_t own_full[kWarps][4];
   uint32_t tmem_base;
   volatile uint32_t abort_flag;
-  uint32_t own_sum[kWarps], own_max[kWarps];
+  uint32_t own_sum[2], own_max[2];
 };
 
 // Where the partial results of head hq of row b lie.
@@ -155,12 +155,14 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return r;
 }
 
-// For every row its first tile (first[batch]: their number), and the tiles it shares * 16 + the tokens of its last tile - 1.
-// Returns the most tiles of a row. All threads of the CTA.
-__device__ __forceinline__ uint32_t scan_rows(const XpDecodeSharedArgs& args, Bars& bars, uint32_t* first, uint32_t* place) {
-  const int batch = args.a.batch, tid = threadIdx.x, lane = tid & 31, each = (batch + kThreads - 1) / kThreads;
+// For every row its first tile (first[batch]: their number), and the tokens it shares | the tokens of its last tile - 1. bars.own_max:
+// the most tiles of a row. Two warps, which have no part in the pieces.
+constexpr int kScanThreads = 64;
+__device__ __forceinline__ void scan_rows(const XpDecodeSharedArgs& args, Bars& bars, uint32_t* first, uint32_t* place, int tid) {
+  const int batch = args.a.batch, lane = tid & 31, each = (batch + kScanThreads - 1) / kScanThreads;
   const int b0 = min(batch, tid * each), b1 = min(batch, b0 + each);
   uint32_t sum = 0, most = 0;
+#pragma unroll 4
   for (int b = b0; b < b1; ++b) {
     const int shared = shared_tokens(args, b), own = row_tokens(args, b) - shared;
     const uint32_t n = static_cast<uint32_t>(own + 15) >> 4;
@@ -176,21 +178,14 @@ __device__ __forceinline__ uint32_t scan_rows(const XpDecodeSharedArgs& args, Ba
   }
   if (lane == 31) bars.own_sum[tid >> 5] = before;
   if (lane == 0) bars.own_max[tid >> 5] = most;
-  __syncthreads();
-  uint32_t at = before - sum;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < (tid >> 5)) at += bars.own_sum[w];
-    most = max(most, bars.own_max[w]);
-  }
+  asm volatile("bar.sync 1, %0;" ::"n"(kScanThreads) : "memory");
+  uint32_t at = before - sum + (tid >= 32 ? bars.own_sum[0] : 0u);
   for (int b = b0; b < b1; ++b) {
     const uint32_t n = first[b];
     first[b] = at;
     at += n;
   }
-  if (tid == kThreads - 1) first[batch] = at;
-  __syncthreads();
-  return most;
+  if (tid == kScanThreads - 1) first[batch] = at;
 }
 
 // Shares of `total` tiles for `busy` CTAs that have spent the time of `cost` tiles on pieces and `idle` CTAs that have not.
@@ -441,8 +436,10 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   const uint32_t tmem = bars.tmem_base;
   pdl::release();
 
-  if (!has_units || warp > 9) {
-    // no part in the pieces
+  if (warp > 9) {
+    scan_rows(args, bars, first, place, threadIdx.x - 320);
+  } else if (!has_units) {
+    // nothing before the own tokens
   } else if (warp == 8) {
     // ------------------------------------------------------------------ TMA producer
     const int page_shift = 31 - __clz(a.page_size), page_mask = a.page_size - 1;
@@ -708,7 +705,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_co
   }
   const bool failed = bars.abort_flag != 0;         // uniform: every role is behind the barrier
   if (!failed) {
-    const uint32_t most = scan_rows(args, bars, first, place);
+    const uint32_t most = max(bars.own_max[0], bars.own_max[1]);
     const uint32_t idle = gridDim.x - busy, cost = turns * (kUnitCost + kTileCost * ((args.n_pieces[1] + kBN - 1) / kBN));
     const Shares shares = make_shares(first[a.batch] * row_units(a), most, args.own_slots, busy, idle, cost);
     if (blockIdx.x == gridDim.x - 1) {
@@ -745,10 +742,25 @@ shared_merge_kernel(XpDecodeSharedArgs args, int G) {
   const XpDecodeAttnArgs& a = args.a;
   const int hk = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t* words = share_words(args, D);
+  // Everything that does not hang on another load is requested at once: the shares, the pairs of all slots (those that were not
+  // written are dropped), and below the sums of the pieces.
+  const uint32_t words_free = words[0], words_large = words[1], words_small = words[2], row_first = words[4 + b];
   const int shared = shared_tokens(args, b), most_parts = b < args.plan_rows ? args.row_parts[b] : 0;
   const int parts = shared > 0 ? most_parts : 0, tiles = (row_tokens(args, b) - shared + 15) >> 4;
-  const Shares cut{words[0], words[1], words[2]};
-  const uint32_t units = row_units(a), row0 = words[4 + b] * units;
+  const int slots = args.max_parts + args.own_slots;
+  float2 pair[4][3];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int g = warp + k * (kMergeThreads / 32);
+    const Partials p(args, D, b, hk * G + min(g, G - 1));
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const int i = j * 32 + lane;
+      pair[k][j] = g < G && i < slots ? p.pairs[i] : make_float2(-CUDART_INF_F, 0.f);
+    }
+  }
+  const Shares cut{words_free, words_large, words_small};
+  const uint32_t units = row_units(a), row0 = row_first * units;
   // shares that hold tiles of a unit of this row
   auto shares = [&](int unit) {
     if (tiles == 0) return 0;
@@ -756,24 +768,26 @@ shared_merge_kernel(XpDecodeSharedArgs args, int G) {
     return static_cast<int>(cut.worker(start + tiles - 1) - cut.worker(start)) + 1;
   };
   const int own0 = shares(units == a.kv_heads ? hk : 2 * hk), own1 = units == a.kv_heads ? 0 : shares(2 * hk + 1);
-  for (int g = warp; g < G; g += kMergeThreads / 32) {
-    const Partials p(args, D, b, hk * G + g);
-    const int n = parts + (g < 8 ? own0 : own1);
-    float2 pair[3];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int g = warp + k * (kMergeThreads / 32), own = g < 8 ? own0 : own1;
+    if (g >= G) break;
     float top = -CUDART_INF_F, sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const int i = k * 32 + lane;
-      pair[k] = i < n ? p.pairs[i < parts ? i : args.max_parts + i - parts] : make_float2(-CUDART_INF_F, 0.f);
-      top = fmaxf(top, pair[k].x);
+    for (int j = 0; j < 3; ++j) {
+      const int i = j * 32 + lane;
+      const bool used = i < args.max_parts ? i < parts : i < args.max_parts + own;
+      if (!used) pair[k][j] = make_float2(-CUDART_INF_F, 0.f);
+      top = fmaxf(top, pair[k][j].x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const float c = pair[k].x == -CUDART_INF_F ? 0.f : exp2f(pair[k].x - top);
-      if (k * 32 + lane < n) wt[g][k * 32 + lane] = c;
-      sum = fmaf(pair[k].y, c, sum);
+    for (int j = 0; j < 3; ++j) {
+      const int i = j * 32 + lane;
+      const float c = pair[k][j].x == -CUDART_INF_F ? 0.f : exp2f(pair[k][j].x - top);
+      if (i < slots) wt[g][i] = c;
+      sum = fmaf(pair[k][j].y, c, sum);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -786,8 +800,9 @@ shared_merge_kernel(XpDecodeSharedArgs args, int G) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int s = 0; s < n; ++s) {
-      const float4 o = *reinterpret_cast<const float4*>(p.sums + static_cast<size_t>(s < parts ? s : args.max_parts + s - parts) * D + d);
-      const float c = wt[g][s];
+      const int at = s < parts ? s : args.max_parts + s - parts;
+      const float4 o = *reinterpret_cast<const float4*>(p.sums + static_cast<size_t>(at) * D + d);
+      const float c = wt[g][at];
       v[0] = fmaf(o.x, c, v[0]), v[1] = fmaf(o.y, c, v[1]), v[2] = fmaf(o.z, c, v[2]), v[3] = fmaf(o.w, c, v[3]);
     }
     const float c = wt[g][kMost];

@@ -136,22 +136,30 @@ def piece_rows(q_heads: int, kv_heads: int) -> int:
     return 2 * (128 // (q_heads // kv_heads))
 
 
-def prefix_piece_tokens(groups: Sequence[tuple[int, int]], kv_heads: int, rows_per_piece: int, num_sms: int = 148) -> int:
-    """Tokens of a prefix that a CTA takes at once, for ``groups`` of (rows, prefix tokens): the split that fills the SMs with the
-    least time of the slowest one. A piece costs as long as about 128 more tokens take (its queries, the first copies, its result)."""
+def prefix_piece_tokens(groups: Sequence[tuple[int, int]], kv_heads: int, rows_per_piece: int, own_tokens: int = 0, head_dim: int = 128,
+                        q_heads: int = 0, num_sms: int = 148) -> int:
+    """Tokens of a prefix that a CTA takes at once, for ``groups`` of (rows, prefix tokens) and about ``own_tokens`` behind them: the
+    split with the least estimated time. The SMs that take pieces need the longest unit's time and stream own tokens afterwards,
+    the others stream from the start; every part of a prefix is one more result to store and merge. Microseconds, as measured on
+    B200 with heads of 128: a unit 3.5 and 1.9 per 128 tokens; 80 KB a us and SM streamed, 5.7 MB in all."""
     tiles = [(-(-n // rows_per_piece), p) for n, p in groups]
-    best, best_cost = PIECE_TOKENS, None
+    own = own_tokens * kv_heads * head_dim * 4
+    rows = sum(n for n, _ in groups)
     longest = max(p for _, p in tiles)
-    c = PIECE_TOKENS
+    best, best_cost, c = PIECE_TOKENS, None, PIECE_TOKENS
     while True:
-        units = kv_heads * sum(t * -(-p // c) for t, p in tiles)
         parts = -(-longest // c)
-        cost = -(-units // num_sms) * (min(c, longest) + 128) + 8 * parts
-        if parts <= MAX_PARTS and (best_cost is None or cost < best_cost):
-            best, best_cost = c, cost
+        if parts <= MAX_PARTS:
+            units = kv_heads * sum(t * -(-p // c) for t, p in tiles)
+            turns = -(-units // num_sms)
+            busy, piece = -(-units // turns), turns * (3.5 + 1.9 * -(-min(c, longest) // PIECE_TOKENS))
+            left = own - (num_sms - busy) * piece * 80e3                # streamed by all SMs behind the pieces
+            cost = max(piece + (4.0 + left / 5.3e6 if left > 0 else 0.0), own / 5.7e6) + parts * (0.15 + rows * max(q_heads, kv_heads) * (head_dim + 2) * 8 / 5e6)
+            if best_cost is None or cost < best_cost:
+                best, best_cost = c, cost
         if c >= longest:
             return best
-        c += max(PIECE_TOKENS, c // 4 // PIECE_TOKENS * PIECE_TOKENS)
+        c += max(PIECE_TOKENS, c // 8 // PIECE_TOKENS * PIECE_TOKENS)
 
 
 def shared_plan_words(rows: int, max_pieces: int) -> int:
@@ -160,9 +168,10 @@ def shared_plan_words(rows: int, max_pieces: int) -> int:
 
 
 def fill_shared_plan(sizes: Sequence[int], prefixes: Sequence[int], words: np.ndarray, rows: int, max_pieces: int, max_parts: int, *,
-                     q_heads: int, kv_heads: int) -> tuple[int, int]:
+                     q_heads: int, kv_heads: int, head_dim: int = 128, own_tokens: int = 0) -> tuple[int, int]:
     """Writes the plan of consecutive groups of rows (``sizes``) with ``prefixes`` tokens shared in each to ``words``; returns its
-    number of pieces and the most pieces of a row. Prefixes are cut so that neither exceeds its bound."""
+    number of pieces and the most pieces of a row. Prefixes are cut so that neither exceeds its bound. ``own_tokens``: about how many
+    tokens all rows have behind their prefixes."""
     per = piece_rows(q_heads, kv_heads)
     pieces = words[4:4 + 8 * max_pieces].reshape(max_pieces, 8)
     shared, parts = words[4 + 8 * max_pieces:][:rows], words[4 + 8 * max_pieces + rows:][:rows]
@@ -177,7 +186,7 @@ def fill_shared_plan(sizes: Sequence[int], prefixes: Sequence[int], words: np.nd
         words[0] = words[1] = 0
         return 0, 0
     longest = max(p for _, _, p in groups)
-    c = prefix_piece_tokens([(n, p) for _, n, p in groups], kv_heads, per)
+    c = prefix_piece_tokens([(n, p) for _, n, p in groups], kv_heads, per, own_tokens, head_dim, q_heads)
     while -(-longest // c) > max_parts or sum(-(-n // per) * -(-p // c) for _, n, p in groups) > max_pieces:
         if c >= longest:
             raise ValueError(f"{len(groups)} groups do not fit a plan of {max_pieces} pieces and {max_parts} parts")
@@ -240,7 +249,9 @@ def shared_prefix_plan(sizes: Sequence[int], prefixes: Sequence[int], *, rows: i
     per = piece_rows(q_heads, kv_heads)
     most = sum(-(-n // per) * -(-p // PIECE_TOKENS) for n, p in zip(sizes, prefixes))
     host = np.zeros(shared_plan_words(rows, most), dtype=np.int32)
-    count, parts = fill_shared_plan(sizes, prefixes, host, rows, most, MAX_PARTS, q_heads=q_heads, kv_heads=kv_heads)
+    # the longest tail behind a prefix is about what every row may have, and half of it what a row has
+    own = rows * (max_len - max(prefixes, default=0)) // 2
+    count, parts = fill_shared_plan(sizes, prefixes, host, rows, most, MAX_PARTS, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, own_tokens=own)
     words = np.concatenate([host[:4 + 8 * count], host[4 + 8 * most:]])
     return SharedPrefixPlan(torch.from_numpy(words).to(device), rows, count, parts, max_len, q_heads, kv_heads, head_dim)
 
