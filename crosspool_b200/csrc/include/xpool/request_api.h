@@ -96,6 +96,7 @@ typedef struct XpLogitArgs {
   float* values;              /* [rows] optional: the adjusted logit of the selected token */
   int rows, vocab, ld, ld_out, f32, out_f32;
 } XpLogitArgs;
+#define XP_LOGIT_VOCAB (1 << 20)
 int xp_logit_controls(const XpLogitArgs* a, void* stream);
 
 #ifdef __cplusplus

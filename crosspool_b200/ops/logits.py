@@ -15,6 +15,7 @@ import torch
 from .. import native
 
 _INT, _FLOAT = torch.int32, torch.float32
+MAX_VOCAB = 1 << 20
 
 
 @dataclass(frozen=True)
@@ -95,6 +96,8 @@ def _args(logits: torch.Tensor, c: LogitControls) -> "native.LogitArgs":
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
         raise ValueError("logits must be bf16 or fp32 [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
+    if vocab > MAX_VOCAB:
+        raise ValueError(f"{vocab} tokens: up to {MAX_VOCAB} are supported")
     if c._rows is not None and c._rows < rows:
         raise ValueError(f"controls of {c._rows} rows for {rows} rows of logits")
     if c._device is not None and c._device != logits.device:

@@ -181,6 +181,29 @@ def test_rows_with_a_pitch_and_nothing_else_written():
     assert torch.equal(L.select_tokens(wide[:, 3:1006], c), L.select_tokens(x, c))
 
 
+@pytest.mark.parametrize("select", [False, True])
+def test_histories_of_more_different_tokens_than_are_counted_at_once(select):
+    from crosspool_b200.ops import logits as L
+
+    g = torch.Generator().manual_seed(4)
+    x = (2 * torch.randn(3, 30000, generator=g)).cuda()
+    toks = torch.cat([torch.randperm(30000, generator=g)[:9000], torch.randint(0, 400, (3000,), generator=g)]).int()
+    history = torch.stack([toks, toks.flip(0), toks]).cuda()
+    t = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    ids = toks[::40].contiguous()
+    vals = torch.randn(len(ids), generator=g)
+    c = L.LogitControls(history=history, lens=t(12000, 12000, 5), prompt_lens=t(4000, 0, 0), repetition=torch.full((3,), 1.3, device="cuda"),
+                        frequency=torch.full((3,), 0.2, device="cuda"), presence=torch.full((3,), 0.4, device="cuda"), bias_ids=ids.cuda(),
+                        bias_values=vals.cuda(), bias_starts=t(0, len(ids), len(ids), len(ids)))
+    want = torch.stack([controls(x[r].cpu(), history[r, :n].tolist(), p, 1.3, 0.2, 0.4, list(zip(ids.tolist(), vals.tolist())) if r == 0 else (),
+                                 dtype=torch.float32) for r, (n, p) in enumerate(((12000, 4000), (12000, 0), (5, 0)))])
+    if select:
+        assert L.select_tokens(x, c).tolist() == want.argmax(1).tolist()
+    else:
+        y = x.clone()
+        assert torch.equal(L.adjust_logits(x, c).cpu(), want) and torch.equal(L.adjust_logits(y, c, out=y).cpu(), want)
+
+
 def test_many_biases_of_few_tokens():
     from crosspool_b200.ops import logits as L
 
