@@ -28,11 +28,12 @@
 namespace xpool {
 namespace controls {
 
-constexpr int kSlots = 4096;                       // tokens of a share that can be counted at once: kSlots - kRoom
-constexpr int kRoom = 1024;                        // slots left so that a search ends: one per thread of the largest CTA
+constexpr int kSlots = 4096;                       // tokens of a share that can be counted at once
+constexpr int kSearch = 64;                        // slots that a token is searched in; one that finds no room is counted in another round
 constexpr uint32_t kEmpty = 0xffffffffu;
 constexpr uint32_t kInPrompt = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3fffffffu;
 constexpr int kMaxRanks = 8;
+constexpr int kBatch = 4;                          // loads of a thread in flight (kSlots is a multiple of 1024 * kBatch)
 constexpr int kUnit = 1024;                        // shares are multiples of so many tokens
 
 __device__ __forceinline__ uint32_t hash3(uint32_t a, uint32_t b, uint32_t c) {
@@ -56,30 +57,28 @@ struct Row {
   __device__ __forceinline__ int token(int i) const { return i == len - 1 && latest >= 0 ? latest : history[i]; }
 };
 
+// (loads that do not hang on one another stand side by side: a chain of them is a microsecond of a small batch)
 __device__ __forceinline__ Row load_row(const XpLogitArgs& a, int r) {
   const XpLogitControls& c = a.c;
   Row w;
-  w.history = nullptr, w.len = 0, w.prompt = 0, w.latest = -1;
-  if (c.history != nullptr) {
-    const int slot = c.history_rows != nullptr ? c.history_rows[r] : r;
-    if (slot >= 0 && slot < c.history_slots) {
-      w.history = c.history + static_cast<size_t>(slot) * c.ld_history;
-      w.len = min(max(c.lens[r], 0), c.history_cap);
-      w.prompt = c.prompt_lens != nullptr ? c.prompt_lens[r] : 0;
-      if (c.latest != nullptr && w.len > 0) w.latest = c.latest[r];
-    }
-  }
-  w.bias0 = w.bias1 = 0;
-  if (c.bias_starts != nullptr) {
-    w.bias0 = min(max(c.bias_starts[r], 0), c.bias_total);
-    w.bias1 = min(max(c.bias_starts[r + 1], w.bias0), c.bias_total);
-  }
+  const int slot = c.history_rows != nullptr ? c.history_rows[r] : r;
+  const int len = c.history != nullptr ? c.lens[r] : 0;
+  const int prompt = c.prompt_lens != nullptr ? c.prompt_lens[r] : 0;
+  const int latest = c.latest != nullptr ? c.latest[r] : -1;
+  const int bias0 = c.bias_starts != nullptr ? c.bias_starts[r] : 0, bias1 = c.bias_starts != nullptr ? c.bias_starts[r + 1] : 0;
   const int m = c.mask_index != nullptr ? c.mask_index[r] : -1;
-  w.mask = m >= 0 && m < c.mask_count ? c.masks + static_cast<size_t>(m) * c.ld_mask : nullptr;
+  const float t = a.temps != nullptr ? a.temps[r] : 0.f;
   w.repetition = c.repetition != nullptr ? c.repetition[r] : 1.f;
   w.frequency = c.frequency != nullptr ? c.frequency[r] : 0.f;
   w.presence = c.presence != nullptr ? c.presence[r] : 0.f;
-  const float t = a.temps != nullptr ? a.temps[r] : 0.f;
+  const bool known = slot >= 0 && slot < c.history_slots;
+  w.history = known ? c.history + static_cast<size_t>(slot) * c.ld_history : nullptr;
+  w.len = known ? min(max(len, 0), c.history_cap) : 0;
+  w.prompt = prompt;
+  w.latest = w.len > 0 ? latest : -1;
+  w.bias0 = min(max(bias0, 0), c.bias_total);
+  w.bias1 = min(max(bias1, w.bias0), c.bias_total);
+  w.mask = m >= 0 && m < c.mask_count ? c.masks + static_cast<size_t>(m) * c.ld_mask : nullptr;
   w.noisy = t > 0.f;
   w.inv_t = w.noisy ? 1.f / t : 1.f;
   w.seed = w.noisy ? a.seeds[2 * r] : 0, w.step = w.noisy ? a.seeds[2 * r + 1] : 0;
@@ -114,20 +113,46 @@ struct Best {
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Occurrences of marked tokens, found by linear search from a hashed place.
+// The largest of those of 16 bytes of logits whose bits are set (-inf if none is).
+__device__ __forceinline__ float largest(const uint4& v, uint32_t use, float) {
+  const float low = -CUDART_INF_F;
+  const float x = use & 1u ? __uint_as_float(v.x) : low, y = use & 2u ? __uint_as_float(v.y) : low;
+  const float z = use & 4u ? __uint_as_float(v.z) : low, w = use & 8u ? __uint_as_float(v.w) : low;
+  return fmaxf(fmaxf(x, y), fmaxf(z, w));
+}
+// (bf16: four bits become the signs of four bytes, and those two pairs of half-word masks)
+__device__ __forceinline__ float largest(const uint4& v, uint32_t use, __nv_bfloat16) {
+  uint32_t r[4] = {v.x, v.y, v.z, v.w};
+  if (use != 0xffu) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t signs = (((use >> (4 * h)) & 15u) * 0x00204081u & 0x01010101u) << 7;
+      uint32_t m0, m1;                               // (the intrinsic leaves out the mode that spreads a byte's sign)
+      asm("prmt.b32 %0, %1, 0, 0x9988;" : "=r"(m0) : "r"(signs));
+      asm("prmt.b32 %0, %1, 0, 0xbbaa;" : "=r"(m1) : "r"(signs));
+      r[2 * h] = (r[2 * h] & m0) | (0xff80ff80u & ~m0);
+      r[2 * h + 1] = (r[2 * h + 1] & m1) | (0xff80ff80u & ~m1);
+    }
+  }
+  const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(r);
+  const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
+// Occurrences of marked tokens, found by linear search from a hashed place: the factor is odd, so kSlots neighbouring tokens have
+// places of their own.
 struct Table {
   uint32_t* keys;
   uint32_t* words;
-  __device__ __forceinline__ static int place(uint32_t id) { return static_cast<int>((id * 2654435761u) >> 20); }
-  // the slot of a token, which is entered where it is not there; the caller keeps kRoom slots empty
-  __device__ __forceinline__ int enter(uint32_t id, bool& is_new) const {
-    for (int s = place(id);; s = (s + 1) & (kSlots - 1)) {
+  __device__ __forceinline__ static int place(uint32_t id) { return static_cast<int>((id * 2654435761u) & (kSlots - 1)); }
+  // the slot of a token, which is entered where it is not there; -1: no room
+  __device__ __forceinline__ int enter(uint32_t id) const {
+    int s = place(id);
+    for (int i = 0; i < kSearch; ++i, s = (s + 1) & (kSlots - 1)) {
       const uint32_t k = atomicCAS(&keys[s], kEmpty, id);
-      if (k == kEmpty || k == id) {
-        is_new = k == kEmpty;
-        return s;
-      }
+      if (k == kEmpty || k == id) return s;
     }
+    return -1;
   }
   __device__ __forceinline__ uint32_t word(uint32_t id) const {
     for (int s = place(id);; s = (s + 1) & (kSlots - 1))
@@ -136,14 +161,13 @@ struct Table {
 };
 
 template <typename T, typename O, bool kSelect, int kThreads>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
   namespace cg = cooperative_groups;
   constexpr int N = 16 / sizeof(T), kWarps = kThreads / 32;
-  static_assert(kThreads <= kRoom, "a search may not end");
   __shared__ float keys_s[kMaxRanks * kWarps], vals_s[kMaxRanks * kWarps];
   __shared__ int toks_s[kMaxRanks * kWarps];
-  __shared__ int entered, repeats;
+  __shared__ int repeats;
   extern __shared__ __align__(16) uint32_t dyn[];
   // the first CTA's shared memory is written once that CTA is known to have started
   auto started = cg::this_cluster().barrier_arrive();
@@ -167,33 +191,59 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
     return k;
   };
 
+  // The next loads of a thread are always in flight: while marks are made, and while loaded logits are worked on.
+  const int whole = wide ? n / N : 0;
+  uint4 ahead[kBatch];
+  uint32_t bits[kBatch];                           // the mask's, of the same tokens
+  const uint8_t* mask8 = reinterpret_cast<const uint8_t*>(w.mask) + (lo >> 3);
+  auto fetch = [&](int c) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (c + j * kThreads < whole) {
+        ahead[j] = reinterpret_cast<const uint4*>(row + lo)[c + j * kThreads];
+        bits[j] = w.mask != nullptr ? mask8[(c + j * kThreads) * N >> 3] : 0xffu;
+      }
+  };
+  fetch(threadIdx.x);
+
   // ---- marks and counts of the tokens that the controls touch
   // tokens [t0, t1): returns whether they found room
   auto count = [&](int t0, int t1, bool mark) {
-    if (threadIdx.x == 0) entered = 0, repeats = 0;
+    int ids[kBatch];
+    auto get = [&](int i0) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kThreads;
+        ids[j] = i < w.len ? w.token(i) : -1;
+      }
+    };
+    get(threadIdx.x);
+    if (threadIdx.x == 0) repeats = 0;
     for (int i = threadIdx.x * 4; i < kSlots; i += kThreads * 4) {
       *reinterpret_cast<uint4*>(table.keys + i) = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
       *reinterpret_cast<uint4*>(table.words + i) = make_uint4(0, 0, 0, 0);
     }
     if (mark)
-      for (int i = threadIdx.x; i < (n + 31) / 32; i += kThreads) marks[i] = 0;
+      for (int i = threadIdx.x * 4; i < (n + 31) / 32; i += kThreads * 4) *reinterpret_cast<uint4*>(marks + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
     bool full = false;
     auto enter = [&](int id, uint32_t what) -> uint32_t {
       if (mark) atomicOr(&marks[(id - lo) >> 5], 1u << ((id - lo) & 31));
-      if (full || *reinterpret_cast<volatile int*>(&entered) > kSlots - kRoom) {
+      const int s = full ? -1 : table.enter(static_cast<uint32_t>(id));
+      if (s < 0) {
         full = true;
         return 0u;
       }
-      bool is_new;
-      const int s = table.enter(static_cast<uint32_t>(id), is_new);
-      if (is_new) atomicAdd(&entered, 1);
       return what == 1u ? atomicAdd(&table.words[s], 1u) : atomicOr(&table.words[s], what);
     };
-#pragma unroll 4
-    for (int i = threadIdx.x; i < w.len; i += kThreads) {
-      const int id = w.token(i);
-      if (id >= t0 && id < t1) enter(id, i < w.prompt ? kInPrompt : 1u);
+    for (int i = threadIdx.x; i < w.len; i += kThreads * kBatch) {
+      int now[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) now[j] = ids[j];
+      if (i + kThreads * kBatch < w.len) get(i + kThreads * kBatch);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (now[j] >= t0 && now[j] < t1) enter(now[j], i + j * kThreads < w.prompt ? kInPrompt : 1u);
     }
     for (int e = w.bias0 + threadIdx.x; e < w.bias1; e += kThreads) {
       const int id = a.c.bias_ids[e];
@@ -204,58 +254,60 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
   const bool fits = !touched || count(lo, hi, true);
 
   // ---- the stream: tokens without marks
-  auto stream = [&](int i0, const T (&v)[N], O (&o)[N]) {
-    uint32_t skip = 0u, allowed = ~0u;
-    const uint32_t ones = (1u << N) - 1u;
-    if (touched) skip = marks[(i0 - lo) >> 5] >> ((i0 - lo) & 31) & ones;
-    if (w.mask != nullptr) allowed = w.mask[i0 >> 5] >> (i0 & 31);
+  int at = -1;                                     // first token of the vector that holds the best one
+  auto stream = [&](int i0, const uint4& raw, uint32_t byte) {
+    const T* v = reinterpret_cast<const T*>(&raw);
+    constexpr uint32_t ones = (1u << N) - 1u;
+    const uint32_t skip = touched ? marks[(i0 - lo) >> 5] >> ((i0 - lo) & 31) & ones : 0u, allowed = byte >> (i0 & 7);
+    const uint32_t use = allowed & ~skip & ones;
     if constexpr (kSelect) {
-      float f[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) f[j] = as_float(v[j]);
-      if (touched || w.mask != nullptr) {
-        const uint32_t use = allowed & ~skip;
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = use >> j & 1u ? f[j] : -CUDART_INF_F;
-      }
       if (w.noisy) {
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (!(skip >> j & 1u)) best.offer(key_of(f[j], i0 + j), f[j], i0 + j);
-      } else {
-        float top = f[0];
-#pragma unroll
-        for (int j = 1; j < N; ++j) top = fmaxf(top, f[j]);
-        if (top > best.key) {
-#pragma unroll
-          for (int j = N - 1; j >= 0; --j)
-            if (f[j] == top) best.token = i0 + j;
-          best.key = best.value = top;
-        } else if (best.token == 0x7fffffff) {       // nothing but -inf so far: the lowest token counts
-#pragma unroll
-          for (int j = N - 1; j >= 0; --j)
-            if (!(skip >> j & 1u)) best.token = i0 + j;
+        for (int j = 0; j < N; ++j) {
+          const float f = allowed >> j & 1u ? as_float(v[j]) : -CUDART_INF_F;
+          if (!(skip >> j & 1u)) best.offer(key_of(f, i0 + j), f, i0 + j);
         }
+        return;
       }
+      // only the value and the vector's place; which of its tokens it is, is looked up once, at the end
+      const float top = largest(raw, use, T());
+      at = top > best.key || at < 0 ? i0 : at;
+      best.key = fmaxf(best.key, top);
     } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float f = (allowed | skip) >> j & 1u ? as_float(v[j]) : -CUDART_INF_F;      // marked tokens stay as they are for now
-        elem::st(o + j, f);
+      O* to = out + i0;
+      if (sizeof(O) == sizeof(T) && (allowed & ones) == ones) {
+        *reinterpret_cast<uint4*>(to) = raw;
+        return;
       }
+      __align__(16) O o[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) elem::st(o + j, (allowed | skip) >> j & 1u ? as_float(v[j]) : -CUDART_INF_F);   // marked tokens stay as they are for now
+      if constexpr (sizeof(O) * N == 8) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(o);
+#pragma unroll
+      for (int j = 0; j < static_cast<int>(sizeof(O)) * N / 16; ++j) reinterpret_cast<uint4*>(to)[j] = reinterpret_cast<const uint4*>(o)[j];
     }
   };
-  const int whole = wide ? n / N : 0;
-#pragma unroll 4
-  for (int c = threadIdx.x; c < whole; c += kThreads) {
-    __align__(16) T v[N];
-    __align__(16) O o[N];
-    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(row + lo + c * N);
-    stream(lo + c * N, v, o);
-    if constexpr (!kSelect) {
+  for (int c = threadIdx.x; c < whole; c += kThreads * kBatch) {
+    uint4 now[kBatch];
+    uint32_t byte[kBatch];
 #pragma unroll
-      for (int j = 0; j < static_cast<int>(sizeof(O)) * N / 16; ++j) reinterpret_cast<uint4*>(out + lo + c * N)[j] = reinterpret_cast<const uint4*>(o)[j];
-      if constexpr (sizeof(O) * N == 8) *reinterpret_cast<uint2*>(out + lo + c * N) = *reinterpret_cast<const uint2*>(o);
+    for (int j = 0; j < kBatch; ++j) now[j] = ahead[j], byte[j] = bits[j];
+    fetch(c + kThreads * kBatch);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (c + j * kThreads < whole) stream(lo + (c + j * kThreads) * N, now[j], byte[j]);
+  }
+  if constexpr (kSelect) {
+    if (at >= 0 && !w.noisy) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(row + at);
+      const T* v = reinterpret_cast<const T*>(&raw);
+      const uint32_t skip = touched ? marks[(at - lo) >> 5] >> ((at - lo) & 31) : 0u, allowed = w.mask != nullptr ? w.mask[at >> 5] >> (at & 31) : ~0u;
+      best.value = best.key;
+#pragma unroll
+      for (int j = N - 1; j >= 0; --j) {
+        const float f = allowed >> j & 1u ? as_float(v[j]) : -CUDART_INF_F;
+        if (!(skip >> j & 1u) && f == best.key) best.token = at + j;
+      }
     }
   }
   for (int i = lo + whole * N + threadIdx.x; i < hi; i += kThreads) {
@@ -276,9 +328,20 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
     else elem::st(out + i, v);
   };
   auto marked = [&](int t0, int t1) {
-    for (int s = threadIdx.x; s < kSlots; s += kThreads) {
-      const uint32_t id = table.keys[s], word = table.words[s];
-      if (id != kEmpty && !(word & kBiased)) finish(static_cast<int>(id), penalised(as_float(row[id]), word, w));
+#pragma unroll 1
+    for (int s0 = threadIdx.x; s0 < kSlots; s0 += kThreads * kBatch) {
+      uint32_t id[kBatch];
+      T raw[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        id[j] = table.keys[s0 + j * kThreads];
+        if (id[j] != kEmpty) raw[j] = row[id[j]];
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const uint32_t word = table.words[s0 + j * kThreads];
+        if (id[j] != kEmpty && !(word & kBiased)) finish(static_cast<int>(id[j]), penalised(as_float(raw[j]), word, w));
+      }
     }
     // biased tokens: the thread of a token's first entry adds up all of them
     for (int e = w.bias0 + threadIdx.x; e < w.bias1; e += kThreads) {
@@ -300,9 +363,9 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
     if (fits) {
       marked(lo, hi);
     } else {
-      // more tokens than the table holds: ranges of the vocabulary that cannot have more, one after the other
-      for (int t0 = lo; t0 < hi; t0 += kSlots - kRoom) {
-        const int t1 = min(t0 + kSlots - kRoom, hi);
+      // more tokens than the table holds: as many neighbouring ones as there are slots, one range after the other
+      for (int t0 = lo; t0 < hi; t0 += kSlots) {
+        const int t1 = min(t0 + kSlots, hi);
         __syncthreads();
         count(t0, t1, false);
         marked(t0, t1);
@@ -352,7 +415,7 @@ static int launch(const XpLogitArgs& a, int ranks, cudaStream_t s) {
   auto aligned = [](const void* p, int64_t ld, int e) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * e % 16 == 0; };
   const int wide = aligned(a.logits, a.ld, es) && aligned(a.out, a.out == nullptr ? 0 : a.ld_out, eo);
   const int share = ((a.vocab + ranks - 1) / ranks + kUnit - 1) / kUnit * kUnit;
-  const int smem = 2 * kSlots * 4 + (share + 31) / 32 * 4;
+  const int smem = 2 * kSlots * 4 + share / 8;
   if (a.out == nullptr) return a.f32 ? go<logit_controls_kernel<float, float, true, kThreads>, kThreads>(a, wide, ranks, share, smem, s)
                                      : go<logit_controls_kernel<bf16, float, true, kThreads>, kThreads>(a, wide, ranks, share, smem, s);
   if (a.out_f32) return a.f32 ? go<logit_controls_kernel<float, float, false, kThreads>, kThreads>(a, wide, ranks, share, smem, s)
@@ -373,7 +436,9 @@ extern "C" int xp_logit_controls(const XpLogitArgs* a, void* stream) {
   if (a->c.bias_starts != nullptr && a->c.bias_total > 0 && (a->c.bias_ids == nullptr || a->c.bias_values == nullptr)) return -12;
   if (a->temps != nullptr && a->seeds == nullptr) return -13;
   if (a->vocab > XP_LOGIT_VOCAB || a->rows > (1 << 27)) return -14;
-  int ranks = a->rows <= 32 ? 8 : a->rows <= 256 ? 4 : 2;
+  // About 256 CTAs of 512 threads, of which an SM holds two. us, CTAs a row 1 / 2 / 4 / 8: 256 rows of 151936 with histories and masks
+  // 33 / 39 / 55 / 86, 64 rows 22 / 16 / 16 / 24, 16 rows 20 / 14 / 11 / 11, 3 rows 17 / 12 / 9 / 8.
+  int ranks = a->rows <= 32 ? 8 : a->rows <= 64 ? 4 : a->rows <= 128 ? 2 : 1;
   while (ranks > 1 && a->vocab / ranks < 4 * kUnit) ranks >>= 1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return a->vocab / ranks <= 4 * kUnit ? launch<256>(*a, ranks, s) : launch<512>(*a, ranks, s);
