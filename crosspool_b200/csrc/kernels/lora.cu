@@ -1,54 +1,248 @@
 // Low-rank adapters of many requests beside a shared projection: out[r] = y[r] + scale (B (A x[r])), every row with the A, B and
-// scale of its own adapter. First form: a CTA per row; warps take the rank's dot products over k, threads the features.
-#include "xpool/elem.cuh"
+// scale of its own adapter. A plan's items are up to 16 rows of one adapter; a cluster of CTAs takes an item:
+//
+//   h = x A^T      the CTAs share k, the warps of a CTA its blocks of 32; partial sums meet in shared memory, then in the
+//                  distributed shared memory of the cluster, always in the same order
+//   out = y + scale h B^T    the CTAs share the features, their warps blocks of 32
+//
+// Both products by mma.m16n8k16 with the rows as M. An adapter is read once for 16 rows or fewer: 32 flop a byte at most, far
+// below what the tensor pipe needs, so what counts is bytes in flight and the one exchange between the products. Fragments are
+// loaded from global memory straight to registers: the order of a sum's terms is free, so a lane's operand of two steps of k are 8
+// neighbouring elements (16 bytes) of a row of x or A, and the columns of four tiles of features are dealt so that a lane holds 8
+// neighbouring features of y and out. While the first product runs, B and y are brought to the L2.
+//
+// h enters the second product as a bf16 pair (high and low part, 16 mantissa bits): its rounding to bf16 alone would be as large as
+// the result's. Sums are fp32.
+#include "xpool/mma_sync.cuh"
 #include "xpool/pdl.cuh"
 #include "xpool/request_api.h"
 
 namespace xpool {
 namespace lora {
 
-constexpr int kThreads = 256;
+using bf16 = __nv_bfloat16;
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kMaxRank = 128;
+constexpr int kTiles = 8;        // tiles of 8 ranks that a pass of the first product takes
+constexpr int kItemRows = 16;
+constexpr int kPitch = kTiles * 8 + 4;               // fp32 row of a warp's partial sums
+
+__device__ __forceinline__ uint4 load16(const bf16* p, bool ok) { return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u); }
+__device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {      // whole 16 bytes
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+// Shared memory: partial sums of the warps, the CTA's sums h [16][parts * rank], and the whole h as fragments, 8 words per lane and 16 ranks.
+__host__ __device__ constexpr int smem_bytes(int all_ranks) { return kWarps * kItemRows * kPitch * 4 + kItemRows * all_ranks * 4 + all_ranks / 16 * 32 * 8 * 4; }
 
 __global__ void __launch_bounds__(kThreads)
-lora_kernel(XpLoraArgs a) {
+lora_kernel(XpLoraArgs a, int ranks) {
+  // the CTAs of a cluster read each other's sums; none leaves before the last has
+  sm100::cluster_sync();
   pdl::wait();
   pdl::release();
-  __shared__ float h[XP_LORA_PARTS * kMaxRank];
-  __shared__ int mine[2];
-  if (threadIdx.x == 0) mine[0] = -2;
-  __syncthreads();
-  for (int i = threadIdx.x; i < min(*a.n_items, a.max_items); i += kThreads) {
-    const XpLoraItem it = a.items[i];
-    if (static_cast<int>(blockIdx.x) >= it.first && static_cast<int>(blockIdx.x) < it.first + it.rows) mine[0] = it.slot;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* part = reinterpret_cast<float*>(smem);
+  float* sums = part + kWarps * kItemRows * kPitch;
+  uint4* frags = reinterpret_cast<uint4*>(sums + kItemRows * a.parts * a.rank);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int rank = blockIdx.x % ranks, first_item = blockIdx.x / ranks, step = gridDim.x / ranks;
+  const int n_items = min(*a.n_items, a.max_items);
+  bool pending = false;                              // the cluster's CTAs have read each other's sums, or are about to
+
+  for (int it = first_item; it < n_items; it += step) {
+    const XpLoraItem item = a.items[it];
+    const int slot = item.slot, rk = slot >= 0 && slot < a.slots ? a.ranks[slot] : 0;
+    // rows of this lane: g and g + 8 of the item
+    const bool on0 = g < item.rows, on1 = g + 8 < item.rows;
+    const int r0 = on0 ? a.perm[item.first + g] : 0, r1 = on1 ? a.perm[item.first + g + 8] : 0;
+    const bf16* y = reinterpret_cast<const bf16*>(a.y);
+    bf16* out = reinterpret_cast<bf16*>(a.out);
+    // features of this CTA, in blocks of 32 that do not cross parts
+    int blocks = 0;
+#pragma unroll
+    for (int p = 0; p < XP_LORA_PARTS; ++p)
+      if (p < a.parts) blocks += (a.part_end[p] - (p ? a.part_end[p - 1] : 0) + 31) >> 5;
+    const int b0 = static_cast<int>(static_cast<long long>(blocks) * rank / ranks), b1 = static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / ranks);
+    auto locate = [&](int b, int& p, int& f, int& end) {      // part of a block, its first feature, the part's end
+      int begin = 0;
+      p = 0;
+      while (true) {
+        const int n = (a.part_end[p] - begin + 31) >> 5;
+        if (b < n || p + 1 == a.parts) break;
+        b -= n, begin = a.part_end[p], ++p;
+      }
+      f = begin + b * 32, end = a.part_end[p];
+    };
+    if (rk == 0) {                                   // no adapter: the rows are copied
+      if (a.out != a.y) {
+        for (int b = b0 + warp; b < b1; b += kWarps) {
+          int p, f, end;
+          locate(b, p, f, end);
+          f += q * 8;
+          if (f >= end) continue;
+          if (on0) *reinterpret_cast<uint4*>(out + static_cast<size_t>(r0) * a.ld_out + f) = load16(y + static_cast<size_t>(r0) * a.ld_y + f, true);
+          if (on1) *reinterpret_cast<uint4*>(out + static_cast<size_t>(r1) * a.ld_out + f) = load16(y + static_cast<size_t>(r1) * a.ld_y + f, true);
+        }
+      }
+      continue;                                      // (the same for all CTAs of the cluster)
+    }
+    const bf16* bw = reinterpret_cast<const bf16*>(a.b) + static_cast<size_t>(slot) * a.n * a.rank;
+    if (b1 > b0 && warp == 0) {
+      int p, f, end, f1;
+      locate(b1 - 1, p, f1, end);
+      f1 = min(f1 + 32, end);
+      locate(b0, p, f, end);
+      const uint32_t bytes = static_cast<uint32_t>(f1 - f) * a.rank * 2;
+      for (uint32_t at = lane * 4096u; at < bytes; at += 32 * 4096u)
+        prefetch_l2(reinterpret_cast<const uint8_t*>(bw + static_cast<size_t>(f) * a.rank) + at, min(4096u, bytes - at));
+      if (lane < item.rows) prefetch_l2(y + static_cast<size_t>(a.perm[item.first + lane]) * a.ld_y + f, static_cast<uint32_t>(f1 - f) * 2);
+    }
+
+    // ---- h = x A^T, this CTA's share of k
+    const int kblocks = (a.k + 31) >> 5;
+    const int k0 = static_cast<int>(static_cast<long long>(kblocks) * rank / ranks), k1 = static_cast<int>(static_cast<long long>(kblocks) * (rank + 1) / ranks);
+    const bf16* x = reinterpret_cast<const bf16*>(a.x);
+    const bf16* aw = reinterpret_cast<const bf16*>(a.a) + static_cast<size_t>(slot) * a.parts * a.rank * a.k;
+    const int all = a.parts * rk;                    // columns of h, part after part
+    for (int c0 = 0; c0 < all; c0 += kTiles * 8) {
+      const int tiles = min(kTiles, (all - c0) >> 3);
+      float acc[kTiles][4];
+      const bf16* wrow[kTiles];
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+        const int c = c0 + min(t, tiles - 1) * 8 + g;
+        wrow[t] = aw + (static_cast<size_t>(c / rk) * a.rank + c % rk) * a.k;
+      }
+#pragma unroll 2
+      for (int kb = k0 + warp; kb < k1; kb += kWarps) {
+        const int k = kb * 32 + q * 8;
+        const bool in = k < a.k;
+        const uint4 x0 = load16(x + static_cast<size_t>(r0) * a.ldx + k, in && on0), x1 = load16(x + static_cast<size_t>(r1) * a.ldx + k, in && on1);
+        uint4 w[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+          if (t < tiles) w[t] = load16(wrow[t] + k, in);
+        const uint32_t lo[4] = {x0.x, x1.x, x0.y, x1.y}, hi[4] = {x0.z, x1.z, x0.w, x1.w};
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+          if (t < tiles) {
+            frag::mma(acc[t], lo, w[t].x, w[t].y);
+            frag::mma(acc[t], hi, w[t].z, w[t].w);
+          }
+      }
+      float* mine = part + (warp * kItemRows + g) * kPitch + q * 2;
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+        if (t < tiles) {
+          *reinterpret_cast<float2*>(mine + t * 8) = make_float2(acc[t][0], acc[t][1]);
+          *reinterpret_cast<float2*>(mine + 8 * kPitch + t * 8) = make_float2(acc[t][2], acc[t][3]);
+        }
+      __syncthreads();
+      if (c0 == 0 && pending) cluster_wait();        // the others have read the sums of the item before
+      for (int i = threadIdx.x; i < kItemRows * tiles * 8; i += kThreads) {
+        const int r = i / (tiles * 8), c = i % (tiles * 8);
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) s += part[(w * kItemRows + r) * kPitch + c];
+        sums[r * all + c0 + c] = s;
+      }
+      __syncthreads();
+    }
+    cluster_arrive();
+    cluster_wait();
+    // ---- the whole h, as fragments: lane (g, q) of a block of 16 ranks holds ranks 4 q .. 4 q + 3 of rows g and g + 8
+    const uint32_t sums_addr = sm100::smem_u32(sums);
+    for (int i = threadIdx.x; i < all / 16 * 32; i += kThreads) {
+      const int kb = i >> 5, l = i & 31, row = l >> 2, c = kb * 16 + (l & 3) * 4;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      for (int s = 0; s < ranks; ++s) {
+        const uint32_t at = sm100::map_rank(sums_addr, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += ld_cluster(at + static_cast<uint32_t>((row + (e >> 2) * 8) * all + c + (e & 3)) * 4u);
+      }
+      uint4 hi, lo;
+      frag::split2(v[0], v[1], hi.x, lo.x);
+      frag::split2(v[4], v[5], hi.y, lo.y);
+      frag::split2(v[2], v[3], hi.z, lo.z);
+      frag::split2(v[6], v[7], hi.w, lo.w);
+      frags[i * 2] = hi, frags[i * 2 + 1] = lo;
+    }
+    cluster_arrive();                                // waited for before the sums are written again, and before the CTA ends
+    pending = true;
+    __syncthreads();
+
+    // ---- out = y + scale h B^T
+    const float scale = a.scale[slot];
+    for (int b = b0 + warp; b < b1; b += kWarps) {
+      int p, f, end;
+      locate(b, p, f, end);
+      const int fl = f + q * 8;                      // this lane's features of y and out
+      const bool in = fl < end;
+      const uint4 y0 = load16(y + static_cast<size_t>(r0) * a.ld_y + fl, in && on0), y1 = load16(y + static_cast<size_t>(r1) * a.ld_y + fl, in && on1);
+      // column g of tile t is feature (g / 2) * 8 + 2 t + g % 2 of the block
+      const int fg = f + (g >> 1) * 8 + (g & 1);
+      const bool ing = f + (g >> 1) * 8 < end;
+      const bf16* brow = bw + static_cast<size_t>(ing ? fg : f) * a.rank + q * 4;
+      float acc[4][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+      const uint4* h = frags + (p * (rk >> 4) * 32 + lane) * 2;
+#pragma unroll 2
+      for (int kb = 0; kb < rk >> 4; ++kb) {
+        uint2 w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint2*>(brow + t * 2 * a.rank + kb * 16);
+        const uint4 hv = h[kb * 64], lv = h[kb * 64 + 1];
+        const uint32_t hi[4] = {hv.x, hv.y, hv.z, hv.w}, lo[4] = {lv.x, lv.y, lv.z, lv.w};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          frag::mma(acc[t], hi, w[t].x, w[t].y);
+          frag::mma(acc[t], lo, w[t].x, w[t].y);
+        }
+      }
+      auto finish = [&](const uint4& v, int row, int half) {
+        const uint32_t in_words[4] = {v.x, v.y, v.z, v.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const float2 yv = frag::unpack2(in_words[t]);
+          const __nv_bfloat162 r = __floats2bfloat162_rn(fmaf(scale, acc[t][half * 2], yv.x), fmaf(scale, acc[t][half * 2 + 1], yv.y));
+          o[t] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+        *reinterpret_cast<uint4*>(out + static_cast<size_t>(row) * a.ld_out + fl) = make_uint4(o[0], o[1], o[2], o[3]);
+      };
+      if (in && on0) finish(y0, r0, 0);
+      if (in && on1) finish(y1, r1, 1);
+    }
+    __syncthreads();                                 // the fragments have been read
   }
-  __syncthreads();
-  const int slot = mine[0];
-  const int r = a.perm[blockIdx.x];
-  if (slot < -1 || slot >= a.slots || r < 0 || r >= a.rows) return;
-  using bf16 = __nv_bfloat16;
-  const bf16* x = reinterpret_cast<const bf16*>(a.x) + static_cast<size_t>(r) * a.ldx;
-  const bf16* y = reinterpret_cast<const bf16*>(a.y) + static_cast<size_t>(r) * a.ld_y;
-  bf16* out = reinterpret_cast<bf16*>(a.out) + static_cast<size_t>(r) * a.ld_out;
-  const int rank = slot >= 0 ? a.ranks[slot] : 0;
-  const float scale = slot >= 0 ? a.scale[slot] : 0.f;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int j = warp; j < a.parts * rank; j += kThreads / 32) {
-    const bf16* row = reinterpret_cast<const bf16*>(a.a) + ((static_cast<size_t>(slot) * a.parts + j / rank) * a.rank + j % rank) * a.k;
-    float s = 0.f;
-    for (int c = lane; c < a.k; c += 32) s += elem::ld(x + c) * elem::ld(row + c);
-    s = elem::warp_sum(s);
-    if (lane == 0) h[j] = s;
+  if (pending) cluster_wait();
+}
+
+static int launch(const XpLoraArgs& a, int ranks, cudaStream_t s) {
+  const int smem = smem_bytes(a.parts * a.rank);
+  static uint64_t allowed = 0;                       // devices on which the kernel may have the shared memory
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return -21;
+  if ((allowed >> (dev & 63) & 1) == 0) {
+    if (cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(XP_LORA_PARTS * kMaxRank)) != cudaSuccess) return -21;
+    allowed |= 1ull << (dev & 63);
   }
-  __syncthreads();
-  for (int c = threadIdx.x; c < a.n; c += kThreads) {
-    int part = 0;
-    while (c >= a.part_end[part]) ++part;
-    const bf16* row = reinterpret_cast<const bf16*>(a.b) + (static_cast<size_t>(max(slot, 0)) * a.n + c) * a.rank;
-    float s = 0.f;
-    for (int j = 0; j < rank; ++j) s += h[part * rank + j] * elem::ld(row + j);
-    elem::st(out + c, elem::ld(y + c) + scale * s);
-  }
+  const int most = 148 * 4 / ranks;
+  pdl::launch(lora_kernel, static_cast<unsigned>((a.max_items < most ? a.max_items : most) * ranks), kThreads, smem, s, ranks, a, ranks);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : -100 - static_cast<int>(e);
 }
 
 }  // namespace lora
@@ -56,10 +250,13 @@ lora_kernel(XpLoraArgs a) {
 
 extern "C" int xp_lora(const XpLoraArgs* a, void* stream) {
   using namespace xpool::lora;
-  if (a->rows <= 0) return 0;
-  if (a->parts < 1 || a->parts > XP_LORA_PARTS || a->rank < 16 || a->rank > kMaxRank || a->rank % 16 != 0 || a->k <= 0 || a->n <= 0) return -10;
+  if (a->rows <= 0 || a->max_items <= 0) return 0;
+  if (a->parts < 1 || a->parts > XP_LORA_PARTS || a->rank < 16 || a->rank > kMaxRank || a->rank % 16 != 0 || a->k <= 0 || a->k % 8 != 0 || a->n <= 0) return -10;
+  for (int p = 0; p < a->parts; ++p)
+    if (a->part_end[p] % 8 != 0 || a->part_end[p] <= (p ? a->part_end[p - 1] : 0)) return -11;
   if (a->part_end[a->parts - 1] != a->n) return -11;
-  xpool::pdl::launch(lora_kernel, a->rows, kThreads, 0, reinterpret_cast<cudaStream_t>(stream), 1, *a);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : -100 - static_cast<int>(e);
+  auto odd = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
+  if (odd(a->x) || odd(a->y) || odd(a->out) || odd(a->a) || odd(a->b) || (a->rows > 1 && (a->ldx % 8 != 0 || a->ld_y % 8 != 0 || a->ld_out % 8 != 0))) return -12;
+  int ranks = a->max_items <= 37 ? 8 : a->max_items <= 74 ? 4 : a->max_items <= 148 ? 2 : 1;
+  return launch(*a, ranks, reinterpret_cast<cudaStream_t>(stream));
 }
