@@ -56,7 +56,7 @@ typedef struct XpLoraArgs {
   const void* y;              /* bf16 [rows, ld_y] */
   void* out;                  /* bf16 [rows, ld_out]; may be y */
   const void* a;              /* bf16 [slots, parts, rank, k] */
-  const void* b;              /* bf16 [slots, n, rank] */
+  const void* b;              /* bf16, n * rank elements per slot, of which [n, ranks[slot]] are used, without gaps */
   const float* scale;         /* [slots] */
   const int* ranks;           /* [slots] rank in use, rounded up to 16; what lies behind it is zero */
   const XpLoraItem* items;

@@ -23,7 +23,7 @@ namespace lora {
 using bf16 = __nv_bfloat16;
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kMaxRank = 128;
-constexpr int kTiles = 8;        // tiles of 8 ranks that a pass of the first product takes
+constexpr int kTiles = 8;        // tiles of 8 ranks that a warp of the first product takes, at most
 constexpr int kItemRows = 16;
 constexpr int kPitch = kTiles * 8 + 4;               // fp32 row of a warp's partial sums
 
@@ -33,19 +33,18 @@ __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {    
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ void add4(float4& s, const float4& v) { s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w; }
 
 // Shared memory: partial sums of the warps, the CTA's sums h [16][parts * rank], and the whole h as fragments, 8 words per lane and 16 ranks.
 __host__ __device__ constexpr int smem_bytes(int all_ranks) { return kWarps * kItemRows * kPitch * 4 + kItemRows * all_ranks * 4 + all_ranks / 16 * 32 * 8 * 4; }
 
 __global__ void __launch_bounds__(kThreads)
 lora_kernel(XpLoraArgs a, int ranks) {
-  // the CTAs of a cluster read each other's sums; none leaves before the last has
-  sm100::cluster_sync();
   pdl::wait();
   pdl::release();
   extern __shared__ __align__(16) uint8_t smem[];
@@ -54,11 +53,12 @@ lora_kernel(XpLoraArgs a, int ranks) {
   uint4* frags = reinterpret_cast<uint4*>(sums + kItemRows * a.parts * a.rank);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = blockIdx.x % ranks, first_item = blockIdx.x / ranks, step = gridDim.x / ranks;
+  XpLoraItem item = a.items[first_item];            // (the grid has no more clusters than items)
   const int n_items = min(*a.n_items, a.max_items);
   bool pending = false;                              // the cluster's CTAs have read each other's sums, or are about to
 
   for (int it = first_item; it < n_items; it += step) {
-    const XpLoraItem item = a.items[it];
+    if (it != first_item) item = a.items[it];
     const int slot = item.slot, rk = slot >= 0 && slot < a.slots ? a.ranks[slot] : 0;
     // rows of this lane: g and g + 8 of the item
     const bool on0 = g < item.rows, on1 = g + 8 < item.rows;
@@ -100,9 +100,9 @@ lora_kernel(XpLoraArgs a, int ranks) {
       locate(b1 - 1, p, f1, end);
       f1 = min(f1 + 32, end);
       locate(b0, p, f, end);
-      const uint32_t bytes = static_cast<uint32_t>(f1 - f) * a.rank * 2;
+      const uint32_t bytes = static_cast<uint32_t>(f1 - f) * rk * 2;
       for (uint32_t at = lane * 4096u; at < bytes; at += 32 * 4096u)
-        prefetch_l2(reinterpret_cast<const uint8_t*>(bw + static_cast<size_t>(f) * a.rank) + at, min(4096u, bytes - at));
+        prefetch_l2(reinterpret_cast<const uint8_t*>(bw + static_cast<size_t>(f) * rk) + at, min(4096u, bytes - at));
       if (lane < item.rows) prefetch_l2(y + static_cast<size_t>(a.perm[item.first + lane]) * a.ld_y + f, static_cast<uint32_t>(f1 - f) * 2);
     }
 
@@ -111,19 +111,21 @@ lora_kernel(XpLoraArgs a, int ranks) {
     const int k0 = static_cast<int>(static_cast<long long>(kblocks) * rank / ranks), k1 = static_cast<int>(static_cast<long long>(kblocks) * (rank + 1) / ranks);
     const bf16* x = reinterpret_cast<const bf16*>(a.x);
     const bf16* aw = reinterpret_cast<const bf16*>(a.a) + static_cast<size_t>(slot) * a.parts * a.rank * a.k;
-    const int all = a.parts * rk;                    // columns of h, part after part
-    for (int c0 = 0; c0 < all; c0 += kTiles * 8) {
-      const int tiles = min(kTiles, (all - c0) >> 3);
+    // The warps share the columns of h in groups of up to 64, and those of a group its blocks of k.
+    const int all = a.parts * rk, n_tiles = all >> 3;   // columns of h, part after part
+    const int groups = n_tiles <= kTiles ? 1 : n_tiles <= 2 * kTiles ? 2 : n_tiles <= 4 * kTiles ? 4 : 8, each = kWarps / groups;
+    const int per = (n_tiles + groups - 1) / groups, t0 = warp / each * per, tiles = max(0, min(per, n_tiles - t0));
+    if (tiles > 0) {
       float acc[kTiles][4];
       const bf16* wrow[kTiles];
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-        const int c = c0 + min(t, tiles - 1) * 8 + g;
+        const int c = (t0 + min(t, tiles - 1)) * 8 + g;
         wrow[t] = aw + (static_cast<size_t>(c / rk) * a.rank + c % rk) * a.k;
       }
 #pragma unroll 2
-      for (int kb = k0 + warp; kb < k1; kb += kWarps) {
+      for (int kb = k0 + warp % each; kb < k1; kb += each) {
         const int k = kb * 32 + q * 8;
         const bool in = k < a.k;
         const uint4 x0 = load16(x + static_cast<size_t>(r0) * a.ldx + k, in && on0), x1 = load16(x + static_cast<size_t>(r1) * a.ldx + k, in && on1);
@@ -146,36 +148,32 @@ lora_kernel(XpLoraArgs a, int ranks) {
           *reinterpret_cast<float2*>(mine + t * 8) = make_float2(acc[t][0], acc[t][1]);
           *reinterpret_cast<float2*>(mine + 8 * kPitch + t * 8) = make_float2(acc[t][2], acc[t][3]);
         }
-      __syncthreads();
-      if (c0 == 0 && pending) cluster_wait();        // the others have read the sums of the item before
-      for (int i = threadIdx.x; i < kItemRows * tiles * 8; i += kThreads) {
-        const int r = i / (tiles * 8), c = i % (tiles * 8);
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) s += part[(w * kItemRows + r) * kPitch + c];
-        sums[r * all + c0 + c] = s;
-      }
-      __syncthreads();
     }
-    cluster_arrive();
-    cluster_wait();
+    __syncthreads();
+    if (pending) cluster_wait();                     // the others have read the sums of the item before
+    for (int i = threadIdx.x; i < kItemRows * all / 4; i += kThreads) {
+      const int r = i / (all / 4), c = i % (all / 4) * 4, gr = (c >> 3) / per;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = gr * each; w < (gr + 1) * each; ++w) add4(s, *reinterpret_cast<const float4*>(part + (w * kItemRows + r) * kPitch + c - gr * per * 8));
+      *reinterpret_cast<float4*>(sums + r * all + c) = s;
+    }
+    sm100::cluster_sync();
     // ---- the whole h, as fragments: lane (g, q) of a block of 16 ranks holds ranks 4 q .. 4 q + 3 of rows g and g + 8
     const uint32_t sums_addr = sm100::smem_u32(sums);
     for (int i = threadIdx.x; i < all / 16 * 32; i += kThreads) {
       const int kb = i >> 5, l = i & 31, row = l >> 2, c = kb * 16 + (l & 3) * 4;
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+#pragma unroll 4
       for (int s = 0; s < ranks; ++s) {
-        const uint32_t at = sm100::map_rank(sums_addr, s);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] += ld_cluster(at + static_cast<uint32_t>((row + (e >> 2) * 8) * all + c + (e & 3)) * 4u);
+        const uint32_t at = sm100::map_rank(sums_addr, s) + static_cast<uint32_t>(row * all + c) * 4u;
+        add4(u, ld_cluster(at));
+        add4(v, ld_cluster(at + 32u * all));
       }
       uint4 hi, lo;
-      frag::split2(v[0], v[1], hi.x, lo.x);
-      frag::split2(v[4], v[5], hi.y, lo.y);
-      frag::split2(v[2], v[3], hi.z, lo.z);
-      frag::split2(v[6], v[7], hi.w, lo.w);
+      frag::split2(u.x, u.y, hi.x, lo.x);
+      frag::split2(v.x, v.y, hi.y, lo.y);
+      frag::split2(u.z, u.w, hi.z, lo.z);
+      frag::split2(v.z, v.w, hi.w, lo.w);
       frags[i * 2] = hi, frags[i * 2 + 1] = lo;
     }
     cluster_arrive();                                // waited for before the sums are written again, and before the CTA ends
@@ -193,7 +191,7 @@ lora_kernel(XpLoraArgs a, int ranks) {
       // column g of tile t is feature (g / 2) * 8 + 2 t + g % 2 of the block
       const int fg = f + (g >> 1) * 8 + (g & 1);
       const bool ing = f + (g >> 1) * 8 < end;
-      const bf16* brow = bw + static_cast<size_t>(ing ? fg : f) * a.rank + q * 4;
+      const bf16* brow = bw + static_cast<size_t>(ing ? fg : f) * rk + q * 4;
       float acc[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
@@ -202,7 +200,7 @@ lora_kernel(XpLoraArgs a, int ranks) {
       for (int kb = 0; kb < rk >> 4; ++kb) {
         uint2 w[4];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint2*>(brow + t * 2 * a.rank + kb * 16);
+        for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint2*>(brow + t * 2 * rk + kb * 16);
         const uint4 hv = h[kb * 64], lv = h[kb * 64 + 1];
         const uint32_t hi[4] = {hv.x, hv.y, hv.z, hv.w}, lo[4] = {lv.x, lv.y, lv.z, lv.w};
 #pragma unroll

@@ -21,9 +21,10 @@ ITEM_ROWS = 16        # rows of one adapter that a cluster of CTAs takes at once
 
 
 class AdapterStack:
-    """The adapters of one projection, slot by slot: ``a`` ``[slots, parts, rank, in]`` and ``b`` ``[slots, out, rank]`` in bf16,
-    a scale and a rank per slot. ``out_features``: a number, or one per part of a fused projection (q, k and v: each part has an
-    ``A`` of its own). Ranks are padded with zeros to ``rank``, the next multiple of 16 of ``max_rank``."""
+    """The adapters of one projection, slot by slot in bf16: ``a`` ``[slots, parts, rank, in]``, ``b`` with room for ``[out, rank]``
+    in each slot, a scale and a rank per slot. ``out_features``: a number, or one per part of a fused projection (q, k and v: each
+    part has an ``A`` of its own). A slot's rank is its adapter's, padded with zeros to a multiple of 16 (``rank`` at most); its
+    ``B`` lies without gaps, ``[out, slot's rank]``, so that low ranks cost no more bytes than they have."""
 
     def __init__(self, slots: int, in_features: int, out_features: int | Sequence[int], max_rank: int, device: str | torch.device = "cuda"):
         self.parts = (int(out_features),) if isinstance(out_features, int) else tuple(int(n) for n in out_features)
@@ -34,7 +35,7 @@ class AdapterStack:
         self.slots, self.in_features, self.out_features = slots, in_features, sum(self.parts)
         self.rank = (max_rank + 15) // 16 * 16
         self.a = torch.zeros(slots, len(self.parts), self.rank, in_features, dtype=torch.bfloat16, device=device)
-        self.b = torch.zeros(slots, self.out_features, self.rank, dtype=torch.bfloat16, device=device)
+        self.b = torch.zeros(slots, self.out_features * self.rank, dtype=torch.bfloat16, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
         self.ranks = torch.zeros(slots, dtype=torch.int32, device=device)
         self.device = self.a.device
@@ -68,14 +69,15 @@ class AdapterStack:
             used = max(used, r)
         self.a[slot].zero_()
         self.b[slot].zero_()
-        at = 0
+        r16, at = (used + 15) // 16 * 16, 0
+        b16 = self.b[slot, :self.out_features * r16].view(self.out_features, r16)
         for i, (n, x, y) in enumerate(zip(self.parts, pa, pb)):
             if x is not None:
                 self.a[slot, i, :x.shape[0]].copy_(x)
-                self.b[slot, at:at + n, :x.shape[0]].copy_(y)
+                b16[at:at + n, :x.shape[0]].copy_(y)
             at += n
         self.scale[slot:slot + 1].fill_(float(scale))
-        self.ranks[slot:slot + 1].fill_((used + 15) // 16 * 16)
+        self.ranks[slot:slot + 1].fill_(r16)
 
     def clear(self, slot: int) -> None:
         """Empties ``slot``: rows that name it keep ``y``."""

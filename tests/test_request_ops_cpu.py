@@ -112,7 +112,7 @@ def test_stacks_and_adapters_that_are_refused():
         with pytest.raises(ValueError):
             lora.AdapterStack(*args, device="cpu")
     s = lora.AdapterStack(2, 64, (32, 16), 20, device="cpu")
-    assert s.rank == 32 and s.a.shape == (2, 2, 32, 64) and s.b.shape == (2, 48, 32)
+    assert s.rank == 32 and s.a.shape == (2, 2, 32, 64) and s.b.shape == (2, 48 * 32)
     z = torch.zeros
     for slot, a, b in ((2, [z(4, 64), z(4, 64)], [z(32, 4), z(16, 4)]), (-1, [None, None], [None, None]), (0, z(4, 64), z(48, 4)),
                        (0, [z(4, 64), z(4, 64)], [z(32, 4), z(32, 4)]), (0, [z(4, 64), None], [z(32, 4), z(16, 4)]),
