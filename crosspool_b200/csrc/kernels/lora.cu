@@ -13,6 +13,10 @@
 //
 // h enters the second product as a bf16 pair (high and low part, 16 mantissa bits): its rounding to bf16 alone would be as large as
 // the result's. Sums are fp32.
+#include <cooperative_groups.h>
+
+#include <utility>
+
 #include "xpool/mma_sync.cuh"
 #include "xpool/pdl.cuh"
 #include "xpool/request_api.h"
@@ -23,39 +27,48 @@ namespace lora {
 using bf16 = __nv_bfloat16;
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kMaxRank = 128;
-constexpr int kTiles = 8;        // tiles of 8 ranks that a warp of the first product takes, at most
 constexpr int kItemRows = 16;
-constexpr int kPitch = kTiles * 8 + 4;               // fp32 row of a warp's partial sums
+constexpr int kMaxCluster = 8;
+constexpr int kPitch = 64 + 4;                       // fp32 row of a warp's partial sums
 
 __device__ __forceinline__ uint4 load16(const bf16* p, bool ok) { return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u); }
 __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {      // whole 16 bytes
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
+// 16 bytes to the shared memory of a CTA of the cluster
+__device__ __forceinline__ void st_cluster(uint32_t addr, const float4& v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ void add4(float4& s, const float4& v) { s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w; }
 
-// Shared memory: partial sums of the warps, the CTA's sums h [16][parts * rank], and the whole h as fragments, 8 words per lane and 16 ranks.
-__host__ __device__ constexpr int smem_bytes(int all_ranks) { return kWarps * kItemRows * kPitch * 4 + kItemRows * all_ranks * 4 + all_ranks / 16 * 32 * 8 * 4; }
+// Shared memory: partial sums of the warps; the sums of all CTAs for the blocks of 16 ranks that this CTA adds up, [blocks][CTA]
+// [16 rows][16 ranks]; the whole h as fragments, 8 words per lane and block.
+__host__ __device__ constexpr int smem_bytes(int all_ranks, int ranks) {
+  return kWarps * kItemRows * kPitch * 4 + (all_ranks / 16 + ranks - 1) / ranks * ranks * 1024 + all_ranks / 16 * 1024;
+}
 
-__global__ void __launch_bounds__(kThreads)
+// kTiles: tiles of 8 ranks that a warp of the first product takes, at most. Four are enough for 256 columns of h and leave the
+// registers for three CTAs to an SM.
+template <int kTiles>
+__global__ void __launch_bounds__(kThreads, kTiles == 4 ? 3 : 2)
 lora_kernel(XpLoraArgs a, int ranks) {
+  namespace cg = cooperative_groups;
+  // another CTA's shared memory is written once that CTA is known to have started
+  auto started = cg::this_cluster().barrier_arrive();
   pdl::wait();
   pdl::release();
   extern __shared__ __align__(16) uint8_t smem[];
   float* part = reinterpret_cast<float*>(smem);
   float* sums = part + kWarps * kItemRows * kPitch;
-  uint4* frags = reinterpret_cast<uint4*>(sums + kItemRows * a.parts * a.rank);
+  uint4* frags = reinterpret_cast<uint4*>(sums + (a.parts * a.rank / 16 + ranks - 1) / ranks * ranks * 256);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = blockIdx.x % ranks, first_item = blockIdx.x / ranks, step = gridDim.x / ranks;
   XpLoraItem item = a.items[first_item];            // (the grid has no more clusters than items)
   const int n_items = min(*a.n_items, a.max_items);
-  bool pending = false;                              // the cluster's CTAs have read each other's sums, or are about to
+  bool met = false;                                  // the CTAs of the cluster have all started
 
   for (int it = first_item; it < n_items; it += step) {
     if (it != first_item) item = a.items[it];
@@ -111,7 +124,7 @@ lora_kernel(XpLoraArgs a, int ranks) {
     const int k0 = static_cast<int>(static_cast<long long>(kblocks) * rank / ranks), k1 = static_cast<int>(static_cast<long long>(kblocks) * (rank + 1) / ranks);
     const bf16* x = reinterpret_cast<const bf16*>(a.x);
     const bf16* aw = reinterpret_cast<const bf16*>(a.a) + static_cast<size_t>(slot) * a.parts * a.rank * a.k;
-    // The warps share the columns of h in groups of up to 64, and those of a group its blocks of k.
+    // The warps share the columns of h in groups of kTiles tiles, and those of a group its blocks of k.
     const int all = a.parts * rk, n_tiles = all >> 3;   // columns of h, part after part
     const int groups = n_tiles <= kTiles ? 1 : n_tiles <= 2 * kTiles ? 2 : n_tiles <= 4 * kTiles ? 4 : 8, each = kWarps / groups;
     const int per = (n_tiles + groups - 1) / groups, t0 = warp / each * per, tiles = max(0, min(per, n_tiles - t0));
@@ -150,35 +163,41 @@ lora_kernel(XpLoraArgs a, int ranks) {
         }
     }
     __syncthreads();
-    if (pending) cluster_wait();                     // the others have read the sums of the item before
+    if (!met) {
+      cg::this_cluster().barrier_wait(std::move(started));
+      met = true;
+    }
+    // ---- the cluster's sums: every block of 16 ranks has a CTA that adds up what all have of it and hands the fragments round
+    const uint32_t sums_addr = sm100::smem_u32(sums), frags_addr = sm100::smem_u32(frags);
     for (int i = threadIdx.x; i < kItemRows * all / 4; i += kThreads) {
-      const int r = i / (all / 4), c = i % (all / 4) * 4, gr = (c >> 3) / per;
+      const int r = i / (all / 4), c = i % (all / 4) * 4, gr = (c >> 3) / per, kb = c >> 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int w = gr * each; w < (gr + 1) * each; ++w) add4(s, *reinterpret_cast<const float4*>(part + (w * kItemRows + r) * kPitch + c - gr * per * 8));
-      *reinterpret_cast<float4*>(sums + r * all + c) = s;
+      st_cluster(sm100::map_rank(sums_addr, kb % ranks) + static_cast<uint32_t>((kb / ranks * ranks + rank) * 1024 + r * 64 + (c & 15) * 4), s);
     }
     sm100::cluster_sync();
-    // ---- the whole h, as fragments: lane (g, q) of a block of 16 ranks holds ranks 4 q .. 4 q + 3 of rows g and g + 8
-    const uint32_t sums_addr = sm100::smem_u32(sums);
-    for (int i = threadIdx.x; i < all / 16 * 32; i += kThreads) {
-      const int kb = i >> 5, l = i & 31, row = l >> 2, c = kb * 16 + (l & 3) * 4;
+    for (int i = threadIdx.x; i < (all / 16 - rank + ranks - 1) / ranks * 32; i += kThreads) {
+      // lane (g, q) of a block holds ranks 4 q .. 4 q + 3 of rows g and g + 8
+      const int kb = i >> 5, l = i & 31;
+      const float* from = sums + kb * ranks * 256 + (l >> 2) * 16 + (l & 3) * 4;
       float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
-#pragma unroll 4
       for (int s = 0; s < ranks; ++s) {
-        const uint32_t at = sm100::map_rank(sums_addr, s) + static_cast<uint32_t>(row * all + c) * 4u;
-        add4(u, ld_cluster(at));
-        add4(v, ld_cluster(at + 32u * all));
+        add4(u, *reinterpret_cast<const float4*>(from + s * 256));
+        add4(v, *reinterpret_cast<const float4*>(from + s * 256 + 128));
       }
       uint4 hi, lo;
       frag::split2(u.x, u.y, hi.x, lo.x);
       frag::split2(v.x, v.y, hi.y, lo.y);
       frag::split2(u.z, u.w, hi.z, lo.z);
       frag::split2(v.z, v.w, hi.w, lo.w);
-      frags[i * 2] = hi, frags[i * 2 + 1] = lo;
+      const uint32_t to = frags_addr + static_cast<uint32_t>((kb * ranks + rank) * 32 + l) * 32u;
+      for (int s = 0; s < ranks; ++s) {
+        const uint32_t at = sm100::map_rank(to, s);
+        st_cluster(at, hi);
+        st_cluster(at + 16, lo);
+      }
     }
-    cluster_arrive();                                // waited for before the sums are written again, and before the CTA ends
-    pending = true;
-    __syncthreads();
+    sm100::cluster_sync();                           // nobody reads or writes another CTA's memory behind this
 
     // ---- out = y + scale h B^T
     const float scale = a.scale[slot];
@@ -223,22 +242,22 @@ lora_kernel(XpLoraArgs a, int ranks) {
       if (in && on0) finish(y0, r0, 0);
       if (in && on1) finish(y1, r1, 1);
     }
-    __syncthreads();                                 // the fragments have been read
   }
-  if (pending) cluster_wait();
+  if (!met) cg::this_cluster().barrier_wait(std::move(started));
 }
 
+template <int kTiles>
 static int launch(const XpLoraArgs& a, int ranks, cudaStream_t s) {
-  const int smem = smem_bytes(a.parts * a.rank);
+  const int smem = smem_bytes(a.parts * a.rank, ranks);
   static uint64_t allowed = 0;                       // devices on which the kernel may have the shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -21;
   if ((allowed >> (dev & 63) & 1) == 0) {
-    if (cudaFuncSetAttribute(lora_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(XP_LORA_PARTS * kMaxRank)) != cudaSuccess) return -21;
+    if (cudaFuncSetAttribute(lora_kernel<kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(XP_LORA_PARTS * kMaxRank, kMaxCluster)) != cudaSuccess) return -21;
     allowed |= 1ull << (dev & 63);
   }
   const int most = 148 * 4 / ranks;
-  pdl::launch(lora_kernel, static_cast<unsigned>((a.max_items < most ? a.max_items : most) * ranks), kThreads, smem, s, ranks, a, ranks);
+  pdl::launch(lora_kernel<kTiles>, static_cast<unsigned>((a.max_items < most ? a.max_items : most) * ranks), kThreads, smem, s, ranks, a, ranks);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -100 - static_cast<int>(e);
 }
@@ -256,5 +275,6 @@ extern "C" int xp_lora(const XpLoraArgs* a, void* stream) {
   auto odd = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
   if (odd(a->x) || odd(a->y) || odd(a->out) || odd(a->a) || odd(a->b) || (a->rows > 1 && (a->ldx % 8 != 0 || a->ld_y % 8 != 0 || a->ld_out % 8 != 0))) return -12;
   int ranks = a->max_items <= 37 ? 8 : a->max_items <= 74 ? 4 : a->max_items <= 148 ? 2 : 1;
-  return launch(*a, ranks, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return a->parts * a->rank <= 256 ? launch<4>(*a, ranks, s) : launch<8>(*a, ranks, s);
 }
