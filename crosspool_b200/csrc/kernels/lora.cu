@@ -31,7 +31,29 @@ constexpr int kItemRows = 16;
 constexpr int kMaxCluster = 8;
 constexpr int kPitch = 64 + 4;                       // fp32 row of a warp's partial sums
 
-__device__ __forceinline__ uint4 load16(const bf16* p, bool ok) { return ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u); }
+// 16 or 8 bytes to shared memory; zeros when not ok
+__device__ __forceinline__ void copy16(uint32_t dst, const bf16* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const bf16* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// waits until at most `left` of the groups issued last are in flight
+__device__ __forceinline__ void landed(int left) {
+  if (left >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (left == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (left == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {      // whole 16 bytes
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
@@ -44,16 +66,20 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, const uint4& v) {
 }
 __device__ __forceinline__ void add4(float4& s, const float4& v) { s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w; }
 
-// Shared memory: partial sums of the warps; the sums of all CTAs for the blocks of 16 ranks that this CTA adds up, [blocks][CTA]
+// A warp's ring, and its partial sums between the products. 10 KB: four blocks of k of three tiles, and two CTAs to an SM.
+template <int kTiles>
+constexpr int region_bytes() { return kTiles == 4 ? 10240 : 15360; }
+static_assert(kItemRows * kPitch * 4 <= region_bytes<4>() && (2 + 8) * 512 * 3 <= region_bytes<8>() && 1024 + kMaxRank * 64 <= region_bytes<4>(), "region");
+
+// Shared memory: the warps' regions; the sums of all CTAs for the blocks of 16 ranks that this CTA adds up, [blocks][CTA]
 // [16 rows][16 ranks]; the whole h as fragments, 8 words per lane and block.
-__host__ __device__ constexpr int smem_bytes(int all_ranks, int ranks) {
-  return kWarps * kItemRows * kPitch * 4 + (all_ranks / 16 + ranks - 1) / ranks * ranks * 1024 + all_ranks / 16 * 1024;
+__host__ __device__ constexpr int smem_bytes(int all_ranks, int ranks, int region) {
+  return kWarps * region + (all_ranks / 16 + ranks - 1) / ranks * ranks * 1024 + all_ranks / 16 * 1024;
 }
 
-// kTiles: tiles of 8 ranks that a warp of the first product takes, at most. Four are enough for 256 columns of h and leave the
-// registers for three CTAs to an SM.
+// kTiles: tiles of 8 ranks that a warp of the first product takes, at most; four are enough for 256 columns of h.
 template <int kTiles>
-__global__ void __launch_bounds__(kThreads, kTiles == 4 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, 2)
 lora_kernel(XpLoraArgs a, int ranks) {
   namespace cg = cooperative_groups;
   // another CTA's shared memory is written once that CTA is known to have started
@@ -61,10 +87,11 @@ lora_kernel(XpLoraArgs a, int ranks) {
   pdl::wait();
   pdl::release();
   extern __shared__ __align__(16) uint8_t smem[];
-  float* part = reinterpret_cast<float*>(smem);
-  float* sums = part + kWarps * kItemRows * kPitch;
+  constexpr int kRegion = region_bytes<kTiles>();
+  float* sums = reinterpret_cast<float*>(smem + kWarps * kRegion);
   uint4* frags = reinterpret_cast<uint4*>(sums + (a.parts * a.rank / 16 + ranks - 1) / ranks * ranks * 256);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const uint32_t ring = sm100::smem_u32(smem) + warp * kRegion + lane * 16;
   const int rank = blockIdx.x % ranks, first_item = blockIdx.x / ranks, step = gridDim.x / ranks;
   XpLoraItem item = a.items[first_item];            // (the grid has no more clusters than items)
   const int n_items = min(*a.n_items, a.max_items);
@@ -101,8 +128,8 @@ lora_kernel(XpLoraArgs a, int ranks) {
           locate(b, p, f, end);
           f += q * 8;
           if (f >= end) continue;
-          if (on0) *reinterpret_cast<uint4*>(out + static_cast<size_t>(r0) * a.ld_out + f) = load16(y + static_cast<size_t>(r0) * a.ld_y + f, true);
-          if (on1) *reinterpret_cast<uint4*>(out + static_cast<size_t>(r1) * a.ld_out + f) = load16(y + static_cast<size_t>(r1) * a.ld_y + f, true);
+          if (on0) *reinterpret_cast<uint4*>(out + static_cast<size_t>(r0) * a.ld_out + f) = *reinterpret_cast<const uint4*>(y + static_cast<size_t>(r0) * a.ld_y + f);
+          if (on1) *reinterpret_cast<uint4*>(out + static_cast<size_t>(r1) * a.ld_out + f) = *reinterpret_cast<const uint4*>(y + static_cast<size_t>(r1) * a.ld_y + f);
         }
       }
       continue;                                      // (the same for all CTAs of the cluster)
@@ -137,24 +164,44 @@ lora_kernel(XpLoraArgs a, int ranks) {
         const int c = (t0 + min(t, tiles - 1)) * 8 + g;
         wrow[t] = aw + (static_cast<size_t>(c / rk) * a.rank + c % rk) * a.k;
       }
-#pragma unroll 2
-      for (int kb = k0 + warp % each; kb < k1; kb += each) {
+      const uint32_t stage = (2 + tiles) * 512;
+      const int depth = min(4, static_cast<int>(kRegion / stage));
+      const bf16* x0 = x + static_cast<size_t>(r0) * a.ldx;
+      const bf16* x1 = x + static_cast<size_t>(r1) * a.ldx;
+      auto issue = [&](int kb, int s) {
         const int k = kb * 32 + q * 8;
-        const bool in = k < a.k;
-        const uint4 x0 = load16(x + static_cast<size_t>(r0) * a.ldx + k, in && on0), x1 = load16(x + static_cast<size_t>(r1) * a.ldx + k, in && on1);
-        uint4 w[kTiles];
+        const bool in = kb < k1 && k < a.k;
+        const int at = in ? k : 0;
+        if (kb < k1) {
+          copy16(ring + s * stage, x0 + at, in && on0);
+          copy16(ring + s * stage + 512, x1 + at, in && on1);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-          if (t < tiles) w[t] = load16(wrow[t] + k, in);
-        const uint32_t lo[4] = {x0.x, x1.x, x0.y, x1.y}, hi[4] = {x0.z, x1.z, x0.w, x1.w};
+          for (int t = 0; t < kTiles; ++t)
+            if (t < tiles) copy16(ring + s * stage + 1024 + t * 512, wrow[t] + at, in);
+        }
+        issued();
+      };
+      const int kb0 = k0 + warp % each;
+      for (int i = 0; i < depth; ++i) issue(kb0 + i * each, i);
+      int s = 0;
+      for (int kb = kb0; kb < k1; kb += each) {
+        landed(depth - 1);
+        const uint32_t at = ring + s * stage;
+        const uint4 u = lds16(at), v = lds16(at + 512);
+        const uint32_t lo[4] = {u.x, v.x, u.y, v.y}, hi[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
           if (t < tiles) {
-            frag::mma(acc[t], lo, w[t].x, w[t].y);
-            frag::mma(acc[t], hi, w[t].z, w[t].w);
+            const uint4 w = lds16(at + 1024 + t * 512);
+            frag::mma(acc[t], lo, w.x, w.y);
+            frag::mma(acc[t], hi, w.z, w.w);
           }
+        issue(kb + depth * each, s);
+        s = s + 1 == depth ? 0 : s + 1;
       }
-      float* mine = part + (warp * kItemRows + g) * kPitch + q * 2;
+      landed(0);
+      __syncwarp();                                  // the partial sums lie over all lanes' copies
+      float* mine = reinterpret_cast<float*>(smem + warp * kRegion) + g * kPitch + q * 2;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
         if (t < tiles) {
@@ -172,10 +219,34 @@ lora_kernel(XpLoraArgs a, int ranks) {
     for (int i = threadIdx.x; i < kItemRows * all / 4; i += kThreads) {
       const int r = i / (all / 4), c = i % (all / 4) * 4, gr = (c >> 3) / per, kb = c >> 4;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int w = gr * each; w < (gr + 1) * each; ++w) add4(s, *reinterpret_cast<const float4*>(part + (w * kItemRows + r) * kPitch + c - gr * per * 8));
+      for (int w = gr * each; w < (gr + 1) * each; ++w) add4(s, *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + w * kRegion) + r * kPitch + c - gr * per * 8));
       st_cluster(sm100::map_rank(sums_addr, kb % ranks) + static_cast<uint32_t>((kb / ranks * ranks + rank) * 1024 + r * 64 + (c & 15) * 4), s);
     }
     sm100::cluster_sync();
+    // ---- the first blocks of the second product are on their way
+    const uint32_t stage = 1024 + rk * 64;             // y, and 8 bytes per tile and block of ranks
+    const int depth = min(4, static_cast<int>(kRegion / stage));
+    const uint32_t ring8 = ring - lane * 8;
+    auto issue = [&](int b, int s) {
+      if (b < b1) {
+        int p, f, end;
+        locate(b, p, f, end);
+        const int fl = f + q * 8;                      // this lane's features of y and out
+        const bool in = fl < end;
+        copy16(ring + s * stage, y + static_cast<size_t>(r0) * a.ld_y + (in ? fl : f), in && on0);
+        copy16(ring + s * stage + 512, y + static_cast<size_t>(r1) * a.ld_y + (in ? fl : f), in && on1);
+        // column g of tile t is feature (g / 2) * 8 + 2 t + g % 2 of the block
+        const bool ing = f + (g >> 1) * 8 < end;
+        const bf16* brow = bw + static_cast<size_t>(ing ? f + (g >> 1) * 8 + (g & 1) : f) * rk + q * 4;
+#pragma unroll 2
+        for (int kb = 0; kb < rk >> 4; ++kb) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) copy8(ring8 + s * stage + 1024 + (kb * 4 + t) * 256, brow + t * 2 * rk + kb * 16);
+        }
+      }
+      issued();
+    };
+    for (int i = 0; i < depth; ++i) issue(b0 + warp + i * kWarps, i);
     for (int i = threadIdx.x; i < (all / 16 - rank + ranks - 1) / ranks * 32; i += kThreads) {
       // lane (g, q) of a block holds ranks 4 q .. 4 q + 3 of rows g and g + 8
       const int kb = i >> 5, l = i & 31;
@@ -201,33 +272,32 @@ lora_kernel(XpLoraArgs a, int ranks) {
 
     // ---- out = y + scale h B^T
     const float scale = a.scale[slot];
+    int s = 0;
     for (int b = b0 + warp; b < b1; b += kWarps) {
       int p, f, end;
       locate(b, p, f, end);
-      const int fl = f + q * 8;                      // this lane's features of y and out
+      const int fl = f + q * 8;
       const bool in = fl < end;
-      const uint4 y0 = load16(y + static_cast<size_t>(r0) * a.ld_y + fl, in && on0), y1 = load16(y + static_cast<size_t>(r1) * a.ld_y + fl, in && on1);
-      // column g of tile t is feature (g / 2) * 8 + 2 t + g % 2 of the block
-      const int fg = f + (g >> 1) * 8 + (g & 1);
-      const bool ing = f + (g >> 1) * 8 < end;
-      const bf16* brow = bw + static_cast<size_t>(ing ? fg : f) * rk + q * 4;
+      landed(depth - 1);
+      const uint32_t at = ring + s * stage, at8 = ring8 + s * stage + 1024;
+      const uint4 y0 = lds16(at), y1 = lds16(at + 512);
       float acc[4][4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
       const uint4* h = frags + (p * (rk >> 4) * 32 + lane) * 2;
 #pragma unroll 2
       for (int kb = 0; kb < rk >> 4; ++kb) {
-        uint2 w[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) w[t] = *reinterpret_cast<const uint2*>(brow + t * 2 * rk + kb * 16);
         const uint4 hv = h[kb * 64], lv = h[kb * 64 + 1];
         const uint32_t hi[4] = {hv.x, hv.y, hv.z, hv.w}, lo[4] = {lv.x, lv.y, lv.z, lv.w};
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-          frag::mma(acc[t], hi, w[t].x, w[t].y);
-          frag::mma(acc[t], lo, w[t].x, w[t].y);
+          const uint2 w = lds8(at8 + (kb * 4 + t) * 256);
+          frag::mma(acc[t], hi, w.x, w.y);
+          frag::mma(acc[t], lo, w.x, w.y);
         }
       }
+      issue(b + depth * kWarps, s);
+      s = s + 1 == depth ? 0 : s + 1;
       auto finish = [&](const uint4& v, int row, int half) {
         const uint32_t in_words[4] = {v.x, v.y, v.z, v.w};
         uint32_t o[4];
@@ -242,18 +312,19 @@ lora_kernel(XpLoraArgs a, int ranks) {
       if (in && on0) finish(y0, r0, 0);
       if (in && on1) finish(y1, r1, 1);
     }
+    __syncwarp();                                    // the next item's stages lie otherwise
   }
   if (!met) cg::this_cluster().barrier_wait(std::move(started));
 }
 
 template <int kTiles>
 static int launch(const XpLoraArgs& a, int ranks, cudaStream_t s) {
-  const int smem = smem_bytes(a.parts * a.rank, ranks);
+  const int smem = smem_bytes(a.parts * a.rank, ranks, region_bytes<kTiles>());
   static uint64_t allowed = 0;                       // devices on which the kernel may have the shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -21;
   if ((allowed >> (dev & 63) & 1) == 0) {
-    if (cudaFuncSetAttribute(lora_kernel<kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(XP_LORA_PARTS * kMaxRank, kMaxCluster)) != cudaSuccess) return -21;
+    if (cudaFuncSetAttribute(lora_kernel<kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(kTiles * 64, kMaxCluster, region_bytes<kTiles>())) != cudaSuccess) return -21;
     allowed |= 1ull << (dev & 63);
   }
   const int most = 148 * 4 / ranks;
