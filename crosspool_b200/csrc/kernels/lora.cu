@@ -345,7 +345,10 @@ extern "C" int xp_lora(const XpLoraArgs* a, void* stream) {
   if (a->part_end[a->parts - 1] != a->n) return -11;
   auto odd = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
   if (odd(a->x) || odd(a->y) || odd(a->out) || odd(a->a) || odd(a->b) || (a->rows > 1 && (a->ldx % 8 != 0 || a->ld_y % 8 != 0 || a->ld_out % 8 != 0))) return -12;
-  int ranks = a->max_items <= 37 ? 8 : a->max_items <= 74 ? 4 : a->max_items <= 148 ? 2 : 1;
+  // Clusters as large as the SMs hold beside one another (two CTAs to an SM). us with 1 / 2 / 4 / 8 CTAs an item: 4 items of rank 16
+  // beside 1024 -> 4096 17 / 12 / 9 / 7; 39 items of ranks 8 to 64 beside 4096 -> 6144 77 / 44 / 36 / 31; 126 items of ranks 16 and 32
+  // beside 4096 -> 4096 27 / 23 / 26 / 33, of rank 128 73 / 67 / 61 / 71.
+  int ranks = a->max_items <= 48 ? 8 : a->max_items <= 80 ? 4 : a->max_items <= 296 ? 2 : 1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return a->parts * a->rank <= 256 ? launch<4>(*a, ranks, s) : launch<8>(*a, ranks, s);
 }
