@@ -52,6 +52,8 @@ def _parser() -> argparse.ArgumentParser:
         if name == "serve":
             g.add_argument("--host", default="127.0.0.1")
             g.add_argument("--port", type=int, required=True)
+            g.add_argument("--controls", action="store_true", help="requests may bring penalties and biases on tokens")
+            g.add_argument("--shared-prefix", action="store_true", help="cache prompt pages and read shared ones once a decode step")
         else:
             g.add_argument("--ids", action="append", required=True, help="one prompt: token ids with commas between them (repeatable)")
             g.add_argument("--max-new-tokens", type=int, default=16)

@@ -23,10 +23,11 @@ import torch
 from ..models.config import ModelConfig
 from ..models.weights import AttentionWeights
 from ..ops import attention as A
-from ..ops import gemm, norm
+from ..ops import gemm, logits, lora, norm
 from ..utils import nvtx
 from ..utils.dtype import decode_dtype
 from .kv_cache import OutOfPages, PagedKvCache
+from .request_options import AdapterRows, ControlRows, PrefixRows, TokenControls
 
 MODE_PREFILL, MODE_DECODE = 1, 2
 
@@ -59,6 +60,10 @@ class EngineConfig:
     dtype: str = "bfloat16"     # activations, weights and cache; "float32" (layered decoders only) runs true 32-bit products
     mixed_batches: bool = False  # a prefill chunk takes the running sequences' next tokens along in the same forward pass
     sampling: bool = False      # per-request temperature sampling (Gumbel-max kernel) instead of greedy argmax
+    controls: bool = False      # per-request penalties, biases and grammar masks (``add_request(controls=...)``)
+    shared_prefix: bool = False  # decode attention reads prompt pages that running sequences share once for all of them
+    adapters: int = 0           # low-rank adapters of the attention projections that may be loaded at once (``load_adapter``)
+    adapter_rank: int = 16      # their largest rank
 
 
 @dataclass
@@ -76,6 +81,8 @@ class Sequence:
     temperature: float = 0.0         # 0: greedy (needs EngineConfig.sampling for anything else)
     seed: int = 0
     refill_len: int = 0              # > 0 after a retraction: prompt + generated tokens to recompute before decoding on
+    controls: TokenControls | None = None
+    adapter: str | None = None       # name of a loaded adapter
 
     @property
     def fill_len(self) -> int:
@@ -144,6 +151,11 @@ def _parts_kw(parts) -> dict:
 
 
 class AttentionEngine:
+    control_rows: ControlRows | None = None    # EngineConfig.controls
+    prefix_rows: PrefixRows | None = None      # EngineConfig.shared_prefix
+    adapter_rows: AdapterRows | None = None    # EngineConfig.adapters
+    _lora_plan = None                          # adapters of the pass that is being enqueued
+
     def __init__(self, cfg: ModelConfig, weights: AttentionWeights, port: FfnPort, ecfg: EngineConfig | None = None,
                  device: str | torch.device = "cuda", kv: PagedKvCache | None = None, tp=None):
         """``tp``: a connected ``parallel.atn_tp.TpGroup`` when this engine is one attention TP rank;
@@ -162,8 +174,14 @@ class AttentionEngine:
                 raise ValueError("prefix sharing needs a cache of pages; this model carries a recurrent state per sequence")
             if e.prefix_cache and not cfg.pages_shareable(e.page_size):
                 raise ValueError(f"prefix sharing needs whole blocks per page; this model pools blocks that do not fill {e.page_size} tokens in eights")
+            if e.shared_prefix or e.adapters:
+                raise UnsupportedAttention(f"{cfg.architecture}: shared-prefix attention and adapters are for rotary grouped-query decoders")
         elif e.dtype != "bfloat16":
             raise ValueError(f"{cfg.architecture} runs in bfloat16 on the GPU engine")
+        if e.adapters and tp is not None:
+            raise ValueError("adapters need whole attention projections (no attention TP)")
+        if e.shared_prefix and (e.page_size < 16 or e.page_size & (e.page_size - 1)):
+            raise ValueError(f"shared-prefix attention needs pages of a power of two of at least 16 tokens, not {e.page_size}")
         self.cfg, self.w, self.port = cfg, weights, port
         self.tp = tp
         self.ecfg = e
@@ -180,6 +198,14 @@ class AttentionEngine:
         self._buckets = e.decode_buckets or capacity_buckets(e.max_batch)
         self.body = None              # layered decoders: engine/layered.py
         self._alloc_buffers()
+        rows = max(e.max_batch, self.max_seqs)
+        if e.controls:
+            self.control_rows = ControlRows(rows, e.max_batch, e.max_seq_len, cfg.vocab_size, self.device)
+        if e.shared_prefix:
+            self.prefix_rows = PrefixRows(cfg, e, self._buckets, e.max_seq_len, self.device)
+        if e.adapters:
+            self.adapter_rows = AdapterRows(cfg, e.adapters, e.adapter_rank, e.max_batch, e.prefill_chunk, self.device)
+        self._b_batch: list[Sequence] = []
         self.waiting: deque[Sequence] = deque()
         self.running: list[Sequence] = []
         self.prefilling: list[Sequence] = []
@@ -310,8 +336,27 @@ class AttentionEngine:
                 m[4 * cap:4 * cap + B * self.max_blocks].view(B, self.max_blocks))
 
     # ------------------------------------------------------------------ request API
+    def load_adapter(self, name: str, layers: list[dict], scale: float = 1.0) -> None:
+        """Loads a low-rank adapter of the attention projections (``layers[l]``: {``q``, ``k``, ``v``, ``o``: (A, B)}); requests name
+        it in ``add_request(adapter=name)``. Needs ``EngineConfig(adapters=...)``."""
+        if self.adapter_rows is None:
+            raise ValueError("adapters need EngineConfig(adapters=...)")
+        with torch.cuda.stream(self.stream):
+            self.adapter_rows.load(name, layers, scale)
+            self.stream.synchronize()        # the caller may free its tensors
+
+    def unload_adapter(self, name: str) -> None:
+        """Frees the adapter's slot; refused while requests use it."""
+        if self.adapter_rows is None or name not in self.adapter_rows.names:
+            raise ValueError(f"no adapter {name!r} is loaded")
+        if any(s.adapter == name for s in (*self.waiting, *self.prefilling, *self.running)):
+            raise ValueError(f"adapter {name!r} is in use")
+        with torch.cuda.stream(self.stream):
+            self.adapter_rows.unload(name)
+
     def add_request(self, prompt: list[int], max_new_tokens: int, arrival: float | None = None,
-                    deadline: float = 0.0, temperature: float = 0.0, seed: int = 0) -> Sequence:
+                    deadline: float = 0.0, temperature: float = 0.0, seed: int = 0, controls: TokenControls | None = None,
+                    adapter: str | None = None) -> Sequence:
         if len(prompt) == 0:
             raise ValueError("empty prompt")
         if max_new_tokens < 1:
@@ -322,8 +367,14 @@ class AttentionEngine:
             raise ValueError(f"token id outside [0, {self.cfg.vocab_size})")
         if temperature > 0 and not self.ecfg.sampling:
             raise ValueError("temperature sampling needs EngineConfig(sampling=True)")
+        if controls is not None:
+            if not self.ecfg.controls:
+                raise ValueError("controls need EngineConfig(controls=True)")
+            controls.check(self.cfg.vocab_size, ControlRows.MOST_BIASES)
+        if adapter is not None and (self.adapter_rows is None or adapter not in self.adapter_rows.names):
+            raise ValueError(f"no adapter {adapter!r} is loaded")
         s = Sequence(self._next_id, list(prompt), max_new_tokens, arrival if arrival is not None else time.monotonic(),
-                     deadline, temperature=float(temperature), seed=int(seed) & 0x7FFFFFFF)
+                     deadline, temperature=float(temperature), seed=int(seed) & 0x7FFFFFFF, controls=controls, adapter=adapter)
         self._next_id += 1
         self.waiting.append(s)
         return s
@@ -347,6 +398,24 @@ class AttentionEngine:
         self.samp_temps[:n].copy_(h[:n, 0], non_blocking=True)
         self.samp_seeds[:n].copy_(hi[:n, 1:3], non_blocking=True)
 
+    def _stage_options(self, seqs: list["Sequence"], samples: list[bool], index: list[int] | None, rows: int) -> int:
+        """Controls of the rows that are sampled and adapters of all rows, on the engine stream before the pass; returns the
+        number of the adapter plan's items."""
+        if self.control_rows is not None:
+            self.control_rows.stage(seqs, samples)
+        if self.adapter_rows is None:
+            return 0
+        n = self.adapter_rows.fill(index, rows)
+        self.adapter_rows.copy(rows)
+        return n
+
+    def _adapter_slot(self, s: "Sequence") -> int:
+        return self.adapter_rows.names[s.adapter] if s.adapter is not None else -1
+
+    def _prefix_space(self, s: "Sequence"):
+        """Cached prefixes hold the keys and values of one adapter (as it was loaded)."""
+        return None if s.adapter is None else (s.adapter, self.adapter_rows.generation[s.adapter])
+
     # ------------------------------------------------------------------ model forward
     def _layers(self, rows: int, mode: int, attn_fn) -> None:
         """Runs all decoder layers over the first ``rows`` rows of the static buffers. ``resid``
@@ -362,10 +431,15 @@ class AttentionEngine:
                 norm.add_rmsnorm(weight=lw.input_norm, eps=cfg.rms_norm_eps, resid=resid, out=x, w_static=True, **_parts_kw(parts),
                                  **self.port.wait_args())
             gemm.linear(x, lw.qkv, out=self.qkv[:rows], bias=lw.qkv_bias, w_static=True)
+            if self._lora_plan is not None:
+                lora.lora_add(self.qkv[:rows], x, self.adapter_rows.qkv[l], self._lora_plan, out=self.qkv[:rows])
             attn_fn(l, lw, rows)
             tgt = self.port.publish_targets(l, rows, mode)
             if self.tp is None:
-                gemm.linear(self.attn_out[:rows].view(rows, cfg.q_size), lw.o, out=self.o[:rows], w_static=True)
+                heads = self.attn_out[:rows].view(rows, cfg.q_size)
+                gemm.linear(heads, lw.o, out=self.o[:rows], w_static=True)
+                if self._lora_plan is not None:
+                    lora.lora_add(self.o[:rows], heads, self.adapter_rows.o[l], self._lora_plan, out=self.o[:rows])
                 o_parts = dict(parts=[self.o[:rows]])
             else:
                 # this rank's heads give a partial; all ranks' partials are folded by the norm below
@@ -449,7 +523,10 @@ class AttentionEngine:
         self._sample(n_sel)
 
     def _sample(self, n_sel: int) -> None:
-        if self.ecfg.sampling:
+        if self.control_rows is not None:
+            draw = (self.samp_temps[:n_sel], self.samp_seeds[:n_sel]) if self.ecfg.sampling else (None, None)
+            logits.select_tokens(self.logits[:n_sel], self.control_rows.controls, *draw, out=self.tokens[:n_sel])
+        elif self.ecfg.sampling:
             A.sample(self.logits[:n_sel], self.samp_temps[:n_sel], self.samp_seeds[:n_sel], out=self.tokens[:n_sel])
         else:
             A.argmax(self.logits[:n_sel], out=self.tokens[:n_sel])
@@ -473,13 +550,19 @@ class AttentionEngine:
             A.rope_kv_write(self.qkv[:rows], self.q[:rows], self.kv.k[l], self.kv.v[l], pos, slots,
                             q_heads=cfg.num_q_heads, kv_heads=cfg.num_kv_heads, head_dim=cfg.head_dim,
                             theta=cfg.rope_theta, q_norm=lw.q_norm, k_norm=lw.k_norm, eps=cfg.rms_norm_eps)
+            if self.prefix_rows is not None:
+                A.paged_decode_shared(self.q[:rows], self.kv.k[l], self.kv.v[l], table, lens, self.prefix_rows.plans[B],
+                                      out=self.attn_out[:rows], ws=self.prefix_rows.ws)
+                return
             A.paged_decode(self.q[:rows], self.kv.k[l], self.kv.v[l], table, lens, out=self.attn_out[:rows],
                            num_splits=splits, ws=self.attn_ws, chunk_tokens=chunk)
 
+        self._lora_plan = self.adapter_rows.plan(B, B) if self.adapter_rows is not None else None
         self._layers(B, MODE_DECODE, attn)
+        self._lora_plan = None
         self._head(B, B, None)
 
-    def _prefill_forward(self, rows: int, n_seqs: int, max_q: int) -> None:
+    def _prefill_forward(self, rows: int, n_seqs: int, max_q: int, adapter_items: int = 0) -> None:
         cfg, P, S = self.cfg, self.ecfg.prefill_chunk, self.max_seqs
         m = self.pre_meta
         ids, pos, slots = m[0:rows], m[P:P + rows], m[2 * P:2 * P + rows]
@@ -502,8 +585,11 @@ class AttentionEngine:
                                cfg.rope_theta, l0.q_norm, l0.k_norm, cfg.rms_norm_eps)
             return rope, A.prefill_args(self.q[:rows], self.kv.k[0], self.kv.v[0], table, q_starts, q_lens, ctx_lens, max_q, self.attn_out[:rows])
 
-        if not self._plain_layers(rows, attn_args):
+        if adapter_items:
+            self._lora_plan = self.adapter_rows.plan(rows, adapter_items)
+        if adapter_items or not self._plain_layers(rows, attn_args):
             self._layers(rows, MODE_PREFILL, attn)
+        self._lora_plan = None
         self._head(rows, n_seqs, last_idx)
 
     def _ragged_forward(self, chosen: list[tuple[Sequence, int]], rows: int) -> None:
@@ -648,7 +734,7 @@ class AttentionEngine:
             if len(self.running) + len(self.prefilling) >= e.max_batch:
                 break
             s = self.waiting[0]
-            shared = self.prefix.match(s.prompt) if self.prefix is not None else []
+            shared = self.prefix.match(s.prompt, self._prefix_space(s)) if self.prefix is not None else []
             need = (s.fill_len + 1 + e.page_size - 1) // e.page_size - len(shared)
             if need > self.kv.allocator.free_pages and self.prefix is not None:
                 freed = self.prefix.evict(need - self.kv.allocator.free_pages)
@@ -698,6 +784,8 @@ class AttentionEngine:
         with torch.cuda.stream(self.stream):
             self.pre_meta.copy_(self.pre_meta_host, non_blocking=True)
             self._stage_sampling([s for s, _ in chosen])
+            index = [self._adapter_slot(s) for s, n in chosen for _ in range(n)] if self.adapter_rows is not None else None
+            items = self._stage_options([s for s, _ in chosen], [s in self._riding or s.computed + n >= s.fill_len for s, n in chosen], index, rows)
             self._announce(rows, MODE_PREFILL)
             if self.body is not None:
                 n = len(chosen)
@@ -705,7 +793,7 @@ class AttentionEngine:
                 self.body.head(rows, self.pre_meta[3 * P + 3 * S:3 * P + 3 * S + n], n, self.sel, self.logits)
                 self._sample(n)
             else:
-                self._prefill_forward(rows, len(chosen), max(n for _, n in chosen))
+                self._prefill_forward(rows, len(chosen), max(n for _, n in chosen), items)
             self.tokens_host[:len(chosen)].copy_(self.tokens[:len(chosen)], non_blocking=True)
             self._step_event.record(self.stream)
         self._pre_inflight = chosen
@@ -825,7 +913,7 @@ class AttentionEngine:
             if s.prefill_done:
                 if self.prefix is not None:
                     # full prompt pages become shareable; the sequence keeps them pinned while it runs
-                    taken = self.prefix.insert(s.prompt, self.kv.tables[s.seq_id])
+                    taken = self.prefix.insert(s.prompt, self.kv.tables[s.seq_id], self._prefix_space(s))
                     s.shared_pages = list(getattr(s, "shared_pages", [])) + taken
                 tok = int(th[i])
                 s.generated.append(tok)
@@ -844,6 +932,8 @@ class AttentionEngine:
     def _release_pages(self, s: Sequence) -> None:
         """Returns the sequence's private pages to the allocator; pages of the prefix cache are only unpinned."""
         shared = getattr(s, "shared_pages", None)
+        if self.control_rows is not None:
+            self.control_rows.release(s.seq_id)
         if self.prefix is not None and shared:
             keep = set(shared)
             t = self.kv.tables.pop(s.seq_id, [])
@@ -869,6 +959,7 @@ class AttentionEngine:
         batch = self.running[:e.max_batch]
         key = tuple(s.seq_id for s in batch)
         if key and key == self._b_key:
+            batch = self._b_batch
             n = len(batch)
             pos = self._b_pos
             pos += 1
@@ -900,7 +991,12 @@ class AttentionEngine:
         if not batch:
             self._b_key = None
             return None
-        return batch, self._fill_decode(batch)
+        key = tuple(s.seq_id for s in batch)
+        if self.prefix_rows is not None:
+            batch = self.prefix_rows.order(batch, [self.kv.tables[s.seq_id] for s in batch], self._bucket(len(batch)))
+        B = self._fill_decode(batch)
+        self._b_key, self._b_batch = key, batch
+        return batch, B
 
     def _fill_decode(self, batch: list[Sequence]) -> int:
         """Writes the whole pinned decode metadata for ``batch``; returns the row bucket."""
@@ -940,6 +1036,9 @@ class AttentionEngine:
         with torch.cuda.stream(self.stream):
             self.dec_meta.copy_(self.dec_meta_host, non_blocking=True)
             self._stage_sampling(batch)
+            self._stage_options(batch, [True] * n, [self._adapter_slot(s) for s in batch] if self.adapter_rows is not None else None, B)
+            if self.prefix_rows is not None:
+                self.prefix_rows.copy()
             self._replay_decode(B)
             self.tokens_host[:n].copy_(self.tokens[:n], non_blocking=True)
             self._step_event.record(self.stream)

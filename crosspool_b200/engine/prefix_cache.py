@@ -29,6 +29,7 @@ class PrefixCache:
     def __init__(self, page_size: int):
         self.page_size = page_size
         self.root = _Node(-1, None)
+        self._spaces: dict = {}      # roots of prefixes that are cached apart (keys and values of an adapter)
         self._clock = itertools.count(1)
         self._by_page: dict[int, _Node] = {}
         self.hits = self.lookups = self.hit_tokens = 0
@@ -45,11 +46,17 @@ class PrefixCache:
         for i in range(0, limit - limit % ps, ps):
             yield tuple(tokens[i:i + ps])
 
-    def match(self, tokens: list[int]) -> list[int]:
+    def _root(self, space) -> _Node:
+        if space is None:
+            return self.root
+        self._spaces = {k: n for k, n in self._spaces.items() if n.children or k == space}
+        return self._spaces.setdefault(space, _Node(-1, None))
+
+    def match(self, tokens: list[int], space=None) -> list[int]:
         """Pages of the longest cached prefix, leaving at least one token to compute; every returned
-        page is pinned until :meth:`release` is called with it."""
+        page is pinned until :meth:`release` is called with it. ``space``: prefixes inserted with another one do not count."""
         self.lookups += 1
-        node, out, now = self.root, [], next(self._clock)
+        node, out, now = self._root(space), [], next(self._clock)
         for key in self._pages(tokens, len(tokens) - 1):
             nxt = node.children.get(key)
             if nxt is None:
@@ -63,11 +70,11 @@ class PrefixCache:
             self.hit_tokens += len(out) * self.page_size
         return out
 
-    def insert(self, tokens: list[int], pages: list[int]) -> list[int]:
+    def insert(self, tokens: list[int], pages: list[int], space=None) -> list[int]:
         """Registers the full pages of a computed prompt (``pages`` is the sequence's block table).
         Returns the pages the cache took ownership of (they must not be freed with the sequence);
         pages that duplicate an existing entry stay with the sequence."""
-        node, taken, now = self.root, [], next(self._clock)
+        node, taken, now = self._root(space), [], next(self._clock)
         for i, key in enumerate(self._pages(tokens, len(tokens))):
             if i >= len(pages):
                 break

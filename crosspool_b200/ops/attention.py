@@ -314,7 +314,7 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
 
     a.status = status_words(dev).data_ptr()
     with native.on_device(dev):
-        native.check(native.kernels().xp_decode_shared(C.byref(s), _stream(dev)), "xp_decode_shared",
+        native.check(native.kernels().xp_decode_shared(C.byref(s), native.stream_of(dev)), "xp_decode_shared",
                      1 + (plan.max_pieces > 0 or plan.slices[0] > 1))
     return out
 

@@ -111,7 +111,7 @@ def _args(logits: torch.Tensor, c: LogitControls) -> "native.LogitArgs":
 
 def _launch(s, dev) -> None:
     with native.on_device(dev):
-        native.check(native.kernels().xp_logit_controls(C.byref(s), torch.cuda.current_stream(dev).cuda_stream), "xp_logit_controls")
+        native.check(native.kernels().xp_logit_controls(C.byref(s), native.stream_of(dev)), "xp_logit_controls")
 
 
 def adjust_logits(logits: torch.Tensor, controls: LogitControls, *, out: torch.Tensor | None = None) -> torch.Tensor:

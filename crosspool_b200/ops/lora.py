@@ -163,5 +163,5 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: Adapte
     s.rows, s.max_items = rows, plan.max_items
     s.ldx, s.ld_y, s.ld_out = x.stride(0), y.stride(0), out.stride(0)
     with native.on_device(dev):
-        native.check(native.kernels().xp_lora(C.byref(s), torch.cuda.current_stream(dev).cuda_stream), "xp_lora")
+        native.check(native.kernels().xp_lora(C.byref(s), native.stream_of(dev)), "xp_lora")
     return out

@@ -7,8 +7,9 @@ import json
 
 
 def build(model: str, *, dtype: str = "bfloat16", gpu: int = 0, max_batch: int = 64, max_seq_len: int = 8192, kv_tokens: int = 0,
-          page_size: int = 64, sampling: bool = True):
-    """A warmed-up single-Instance :class:`Deployment` of a checkpoint directory or preset."""
+          page_size: int = 64, sampling: bool = True, controls: bool = False, shared_prefix: bool = False):
+    """A warmed-up single-Instance :class:`Deployment` of a checkpoint directory or preset. ``controls``: requests may bring
+    penalties and biases; ``shared_prefix``: prompt pages are cached, and read once a decode step for all requests that share them."""
     import torch
 
     from ..deployment import build_loopback
@@ -16,6 +17,7 @@ def build(model: str, *, dtype: str = "bfloat16", gpu: int = 0, max_batch: int =
 
     torch.cuda.set_device(gpu)
     ecfg = EngineConfig(max_batch=max_batch, max_seq_len=max_seq_len, page_size=page_size, dtype=dtype, sampling=sampling,
+                        controls=controls, shared_prefix=shared_prefix, prefix_cache=shared_prefix,
                         num_pages=(kv_tokens + page_size - 1) // page_size)
     dep = build_loopback([(model, model, 0)], ecfg, device=f"cuda:{gpu}")
     dep.warmup()
@@ -24,7 +26,7 @@ def build(model: str, *, dtype: str = "bfloat16", gpu: int = 0, max_batch: int =
 
 def _from_args(ns, sampling: bool):
     return build(ns.model, dtype=ns.dtype, gpu=ns.gpu, max_batch=ns.max_batch, max_seq_len=ns.max_seq_len, kv_tokens=ns.kv_tokens,
-                 sampling=sampling)
+                 sampling=sampling, controls=getattr(ns, "controls", False), shared_prefix=getattr(ns, "shared_prefix", False))
 
 
 def serve(ns) -> int:

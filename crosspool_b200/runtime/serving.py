@@ -40,6 +40,7 @@ class Pending:
     # set by an asyncio consumer: tokens are then also handed to its event loop, so that it never has to poll
     aio_loop: object = None
     aio_queue: object = None
+    options: dict = field(default_factory=dict)   # further arguments of add_request: controls, adapter
     tag: object = None   # opaque to the loop; an in-process consumer (``EngineLoop.sink``) finds its own record here
 
     def deliver(self, item) -> None:
@@ -89,9 +90,10 @@ class EngineLoop:
         self.metrics = None      # runtime/metrics.py::InstanceMetrics once an HTTP endpoint serves GET /metrics
 
     def submit(self, model_id: str, prompt: list[int], max_new_tokens: int, temperature: float = 0.0, seed: int = 0,
-               aio: bool = False, queued: bool = True, tag: object = None) -> Pending:
-        """``aio``: called from a running event loop that will ``await p.aio_queue.get()``."""
-        p = Pending(model_id, prompt, max_new_tokens, time.monotonic(), temperature, seed, tag=tag)
+               aio: bool = False, queued: bool = True, tag: object = None, options: dict | None = None) -> Pending:
+        """``aio``: called from a running event loop that will ``await p.aio_queue.get()``. ``options``: ``controls`` and
+        ``adapter`` of the engine's ``add_request``."""
+        p = Pending(model_id, prompt, max_new_tokens, time.monotonic(), temperature, seed, options=dict(options or {}), tag=tag)
         if not queued:
             p.out = None
         if aio:
@@ -107,7 +109,7 @@ class EngineLoop:
                 return
             try:
                 kw = {"temperature": p.temperature, "seed": p.seed} if p.temperature > 0 else {}
-                seq = self.dep.add_request(p.model_id, p.prompt, p.max_new_tokens, arrival=p.arrival, **kw)
+                seq = self.dep.add_request(p.model_id, p.prompt, p.max_new_tokens, arrival=p.arrival, **kw, **p.options)
                 self._by_seq[(p.model_id, seq.seq_id)] = p
             except Exception as e:  # bad request: answer it, keep serving
                 p.deliver(e)
@@ -184,6 +186,23 @@ class GenerateRequest(BaseModel):
     stream: bool = False
     temperature: float = 0.0
     seed: int = 0
+    # of engines with controls (EngineConfig.controls) and adapters
+    repetition_penalty: float = 1.0
+    frequency_penalty: float = 0.0
+    presence_penalty: float = 0.0
+    logit_bias: dict[int, float] = {}
+    adapter: Optional[str] = None
+
+    def options(self) -> dict:
+        """Arguments of the engine's ``add_request`` beside the prompt, none for a plain request."""
+        out: dict = {}
+        if self.repetition_penalty != 1.0 or self.frequency_penalty or self.presence_penalty or self.logit_bias:
+            from ..engine.request_options import TokenControls
+
+            out["controls"] = TokenControls(self.repetition_penalty, self.frequency_penalty, self.presence_penalty, dict(self.logit_bias))
+        if self.adapter is not None:
+            out["adapter"] = self.adapter
+        return out
 
 
 def load_tokenizers(checkpoints: dict[str, str | None]) -> dict:
@@ -249,7 +268,7 @@ def create_serving_app(loop: EngineLoop, models: list[str], tokenizer=None):
             if req.text is None or tok_model is None:
                 raise HTTPException(status_code=422, detail="input_ids required (no tokenizer configured)")
             ids = tok_model.encode(req.text)
-        p = loop.submit(model, list(ids), req.max_new_tokens, req.temperature, req.seed, aio=True)
+        p = loop.submit(model, list(ids), req.max_new_tokens, req.temperature, req.seed, aio=True, options=req.options())
         if req.stream:
             async def sse():
                 n = 0

@@ -49,7 +49,7 @@ class TpEngineLoop(EngineLoop):
                             p.deliver(RuntimeError(f"{p.model_id} is served by its tensor-parallel leader, not by this rank"))
                 reqs, stop = self._exchange(
                     [{"model": p.model_id, "prompt": p.prompt, "max_new_tokens": p.max_new_tokens, "temperature": p.temperature,
-                      "seed": p.seed} for p in mine] if self.leader else None, self._stop.is_set())
+                      "seed": p.seed, "options": p.options} for p in mine] if self.leader else None, self._stop.is_set())
                 if stop:
                     for p in local:
                         p.deliver(RuntimeError("the engine loop is stopping"))
@@ -59,7 +59,7 @@ class TpEngineLoop(EngineLoop):
                         continue       # an Instance that only the leader's device hosts
                     kw = {"temperature": r["temperature"], "seed": r["seed"]} if r["temperature"] > 0 else {}
                     try:
-                        seq = self.dep.add_request(r["model"], r["prompt"], r["max_new_tokens"], **kw)
+                        seq = self.dep.add_request(r["model"], r["prompt"], r["max_new_tokens"], **kw, **r["options"])
                         if self.leader:
                             self._by_seq[(r["model"], seq.seq_id)] = mine[i]
                     except Exception as e:   # every rank refuses the same request the same way
@@ -68,7 +68,7 @@ class TpEngineLoop(EngineLoop):
                 for p in local:
                     kw = {"temperature": p.temperature, "seed": p.seed} if p.temperature > 0 else {}
                     try:
-                        seq = self.dep.add_request(p.model_id, p.prompt, p.max_new_tokens, **kw)
+                        seq = self.dep.add_request(p.model_id, p.prompt, p.max_new_tokens, **kw, **p.options)
                         self._by_seq[(p.model_id, seq.seq_id)] = p
                     except Exception as e:
                         p.deliver(e)
