@@ -160,7 +160,8 @@ struct Table {
   }
 };
 
-template <typename T, typename O, bool kSelect, int kThreads>
+// kOdd: rows whose pitch is no whole 16 bytes (their vectors' bits in masks and marks begin anywhere in a word).
+template <typename T, typename O, bool kSelect, bool kOdd, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads)
 logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
   namespace cg = cooperative_groups;
@@ -192,16 +193,28 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
   };
 
   // The next loads of a thread are always in flight: while marks are made, and while loaded logits are worked on.
-  const int whole = wide ? n / N : 0;
+  // Rows of an odd vocabulary begin anywhere: vectors begin behind the `head` tokens before the first whole 16 bytes.
+  const int head = kOdd ? min(n, static_cast<int>((N - static_cast<size_t>(r) * a.ld % N) % N)) : 0, whole = wide ? (n - head) / N : 0, lov = lo + head;
   uint4 ahead[kBatch];
-  uint32_t bits[kBatch];                           // the mask's, of the same tokens
-  const uint8_t* mask8 = reinterpret_cast<const uint8_t*>(w.mask) + (lo >> 3);
+  // ... the mask's bits of the same tokens: a byte, or the two words that they lie in; shifted when they are used, or the loads
+  // would be waited for here
+  uint32_t bits[kBatch], more[kOdd ? kBatch : 1];
+  auto bits_at = [](const uint32_t* p, int at, int last) {     // 32 bits from a place on; `last`: the last word that is there
+    return __funnelshift_r(p[at >> 5], p[min((at >> 5) + 1, last)], at & 31);
+  };
   auto fetch = [&](int c) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
       if (c + j * kThreads < whole) {
-        ahead[j] = reinterpret_cast<const uint4*>(row + lo)[c + j * kThreads];
-        bits[j] = w.mask != nullptr ? mask8[(c + j * kThreads) * N >> 3] : 0xffu;
+        ahead[j] = reinterpret_cast<const uint4*>(row + lov)[c + j * kThreads];
+        const int i0 = lov + (c + j * kThreads) * N;
+        bits[j] = ~0u;
+        if constexpr (kOdd) {
+          more[j] = ~0u;
+          if (w.mask != nullptr) bits[j] = w.mask[i0 >> 5], more[j] = w.mask[min((i0 >> 5) + 1, (a.vocab - 1) >> 5)];
+        } else {
+          if (w.mask != nullptr) bits[j] = reinterpret_cast<const uint8_t*>(w.mask)[i0 >> 3];
+        }
       }
   };
   fetch(threadIdx.x);
@@ -255,10 +268,10 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
 
   // ---- the stream: tokens without marks
   int at = -1;                                     // first token of the vector that holds the best one
-  auto stream = [&](int i0, const uint4& raw, uint32_t byte) {
+  auto stream = [&](int i0, const uint4& raw, uint32_t allowed) {
     const T* v = reinterpret_cast<const T*>(&raw);
     constexpr uint32_t ones = (1u << N) - 1u;
-    const uint32_t skip = touched ? marks[(i0 - lo) >> 5] >> ((i0 - lo) & 31) & ones : 0u, allowed = byte >> (i0 & 7);
+    const uint32_t skip = !touched ? 0u : !kOdd ? marks[(i0 - lo) >> 5] >> ((i0 - lo) & 31) & ones : bits_at(marks, i0 - lo, (n - 1) >> 5) & ones;
     const uint32_t use = allowed & ~skip & ones;
     if constexpr (kSelect) {
       if (w.noisy) {
@@ -289,19 +302,23 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
   };
   for (int c = threadIdx.x; c < whole; c += kThreads * kBatch) {
     uint4 now[kBatch];
-    uint32_t byte[kBatch];
+    uint32_t allowed[kBatch];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) now[j] = ahead[j], byte[j] = bits[j];
+    for (int j = 0; j < kBatch; ++j) {
+      const int i0 = lov + (c + j * kThreads) * N;
+      now[j] = ahead[j];
+      allowed[j] = kOdd ? __funnelshift_r(bits[j], more[kOdd ? j : 0], i0 & 31) : bits[j] >> (i0 & 7);
+    }
     fetch(c + kThreads * kBatch);
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
-      if (c + j * kThreads < whole) stream(lo + (c + j * kThreads) * N, now[j], byte[j]);
+      if (c + j * kThreads < whole) stream(lov + (c + j * kThreads) * N, now[j], allowed[j]);
   }
   if constexpr (kSelect) {
     if (at >= 0 && !w.noisy) {
       const uint4 raw = *reinterpret_cast<const uint4*>(row + at);
       const T* v = reinterpret_cast<const T*>(&raw);
-      const uint32_t skip = touched ? marks[(at - lo) >> 5] >> ((at - lo) & 31) : 0u, allowed = w.mask != nullptr ? w.mask[at >> 5] >> (at & 31) : ~0u;
+      const uint32_t skip = touched ? bits_at(marks, at - lo, (n - 1) >> 5) : 0u, allowed = w.mask != nullptr ? bits_at(w.mask, at, (a.vocab - 1) >> 5) : ~0u;
       best.value = best.key;
 #pragma unroll
       for (int j = N - 1; j >= 0; --j) {
@@ -310,7 +327,8 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
       }
     }
   }
-  for (int i = lo + whole * N + threadIdx.x; i < hi; i += kThreads) {
+  for (int k = threadIdx.x; k < n - whole * N; k += kThreads) {      // before and behind them
+    const int i = k < head ? lo + k : lo + whole * N + k;
     const bool skip = touched && marks[(i - lo) >> 5] >> ((i - lo) & 31) & 1u;
     const bool allowed = w.mask == nullptr || w.mask[i >> 5] >> (i & 31) & 1u;
     const float f = as_float(row[i]), v = allowed || skip ? f : -CUDART_INF_F;
@@ -408,20 +426,27 @@ static int go(const XpLogitArgs& a, int wide, int ranks, int share, int smem, cu
   return e == cudaSuccess ? 0 : -100 - static_cast<int>(e);
 }
 
+template <bool kOdd, int kThreads>
+static int launch_as(const XpLogitArgs& a, int wide, int ranks, int share, int smem, cudaStream_t s) {
+  using bf16 = __nv_bfloat16;
+  if (a.out == nullptr) return a.f32 ? go<logit_controls_kernel<float, float, true, kOdd, kThreads>, kThreads>(a, wide, ranks, share, smem, s)
+                                     : go<logit_controls_kernel<bf16, float, true, kOdd, kThreads>, kThreads>(a, wide, ranks, share, smem, s);
+  if (a.out_f32) return a.f32 ? go<logit_controls_kernel<float, float, false, kOdd, kThreads>, kThreads>(a, wide, ranks, share, smem, s)
+                              : go<logit_controls_kernel<bf16, float, false, kOdd, kThreads>, kThreads>(a, wide, ranks, share, smem, s);
+  return a.f32 ? go<logit_controls_kernel<float, bf16, false, kOdd, kThreads>, kThreads>(a, wide, ranks, share, smem, s)
+               : go<logit_controls_kernel<bf16, bf16, false, kOdd, kThreads>, kThreads>(a, wide, ranks, share, smem, s);
+}
+
 template <int kThreads>
 static int launch(const XpLogitArgs& a, int ranks, cudaStream_t s) {
-  using bf16 = __nv_bfloat16;
   const int es = a.f32 ? 4 : 2, eo = a.out == nullptr ? 16 : a.out_f32 ? 4 : 2;
-  auto aligned = [](const void* p, int64_t ld, int e) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * e % 16 == 0; };
-  const int wide = aligned(a.logits, a.ld, es) && aligned(a.out, a.out == nullptr ? 0 : a.ld_out, eo);
+  auto based = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  const bool whole = a.ld * es % 16 == 0 && (a.out == nullptr || a.ld_out * eo % 16 == 0);
+  // 16 bytes a load where logits and result are aligned alike in every row
+  const int wide = based(a.logits) && based(a.out) && (whole || a.out == nullptr || a.ld == a.ld_out);
   const int share = ((a.vocab + ranks - 1) / ranks + kUnit - 1) / kUnit * kUnit;
   const int smem = 2 * kSlots * 4 + share / 8;
-  if (a.out == nullptr) return a.f32 ? go<logit_controls_kernel<float, float, true, kThreads>, kThreads>(a, wide, ranks, share, smem, s)
-                                     : go<logit_controls_kernel<bf16, float, true, kThreads>, kThreads>(a, wide, ranks, share, smem, s);
-  if (a.out_f32) return a.f32 ? go<logit_controls_kernel<float, float, false, kThreads>, kThreads>(a, wide, ranks, share, smem, s)
-                              : go<logit_controls_kernel<bf16, float, false, kThreads>, kThreads>(a, wide, ranks, share, smem, s);
-  return a.f32 ? go<logit_controls_kernel<float, bf16, false, kThreads>, kThreads>(a, wide, ranks, share, smem, s)
-               : go<logit_controls_kernel<bf16, bf16, false, kThreads>, kThreads>(a, wide, ranks, share, smem, s);
+  return wide && !whole ? launch_as<true, kThreads>(a, wide, ranks, share, smem, s) : launch_as<false, kThreads>(a, wide, ranks, share, smem, s);
 }
 
 }  // namespace controls

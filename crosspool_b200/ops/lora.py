@@ -39,6 +39,7 @@ class AdapterStack:
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
         self.ranks = torch.zeros(slots, dtype=torch.int32, device=device)
         self.device = self.a.device
+        self._fresh = [True] * slots       # never loaded: still zero
         end, ends = 0, []
         for n in self.parts:
             end += n
@@ -67,8 +68,10 @@ class AdapterStack:
             if x.dim() != 2 or y.dim() != 2 or not 1 <= r <= self.rank or tuple(x.shape) != (r, self.in_features) or tuple(y.shape) != (n, r):
                 raise ValueError(f"matrices {tuple(x.shape)} and {tuple(y.shape)} for {self.in_features} -> {n} features, rank up to {self.rank}")
             used = max(used, r)
-        self.a[slot].zero_()
-        self.b[slot].zero_()
+        if not self._fresh[slot]:
+            self.a[slot].zero_()
+            self.b[slot].zero_()
+        self._fresh[slot] = False
         r16, at = (used + 15) // 16 * 16, 0
         b16 = self.b[slot, :self.out_features * r16].view(self.out_features, r16)
         for i, (n, x, y) in enumerate(zip(self.parts, pa, pb)):

@@ -204,6 +204,22 @@ def test_histories_of_more_different_tokens_than_are_counted_at_once(select):
         assert torch.equal(L.adjust_logits(x, c).cpu(), want) and torch.equal(L.adjust_logits(y, c, out=y).cpu(), want)
 
 
+@pytest.mark.parametrize("dtype,to", [(torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float32, torch.float32), (torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("vocab", [3, 1021, 12291])
+def test_rows_that_begin_anywhere(vocab, dtype, to):
+    """A contiguous batch of an odd vocabulary, and results of the same pitch and of another one."""
+    from crosspool_b200.ops import logits as L
+
+    x, c, args = batch(17, vocab, dtype, seed=vocab + 1)
+    same = oracle(x, args, torch.float32).to(to)
+    assert torch.equal(L.adjust_logits(x, c, out=torch.empty(x.shape, dtype=to, device="cuda")).cpu(), same)
+    wide = torch.full((17, vocab + 5), 7.0, dtype=to, device="cuda")
+    assert torch.equal(L.adjust_logits(x, c, out=wide[:, :vocab]).cpu(), same) and (wide[:, vocab:] == 7.0).all()
+    full = L.adjust_logits(x, c, out=torch.empty(x.shape, device="cuda"))
+    want = torch.stack([(r == r.max()).nonzero()[0, 0] for r in full]).int()
+    assert torch.equal(L.select_tokens(x, c), want)
+
+
 def test_many_biases_of_few_tokens():
     from crosspool_b200.ops import logits as L
 
