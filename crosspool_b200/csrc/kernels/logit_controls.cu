@@ -406,7 +406,7 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
     for (int i = threadIdx.x; i < ranks * kWarps; i += 32) b.offer(keys_s[i], vals_s[i], toks_s[i]);
     b.warp();
     if (threadIdx.x == 0) {
-      a.tokens[r] = b.token;
+      a.tokens[r] = b.token == 0x7fffffff ? 0 : b.token;       // nothing but NaN
       if (a.values != nullptr) a.values[r] = b.value;
     }
   }

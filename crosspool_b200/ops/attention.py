@@ -239,8 +239,9 @@ class SharedPrefixPlan:
 def shared_prefix_plan(sizes: Sequence[int], prefixes: Sequence[int], *, rows: int, q_heads: int, kv_heads: int, head_dim: int, max_len: int,
                        device: str | torch.device = "cuda") -> SharedPrefixPlan:
     """The plan of a batch of ``rows`` rows whose first ``sizes[0]`` rows share their first ``prefixes[0]`` tokens (their block
-    tables name the same pages for them), the next ``sizes[1]`` rows ``prefixes[1]`` tokens and so on; rows behind the last group
-    share nothing. ``max_len``: bound of the sequence lengths while the plan is in use."""
+    tables name the same pages for them; a group's prefix is read through its first row's table, whatever that row's length), the
+    next ``sizes[1]`` rows ``prefixes[1]`` tokens and so on; rows behind the last group share nothing. ``max_len``: bound of the
+    sequence lengths while the plan is in use; rows are read no further."""
     if len(sizes) != len(prefixes) or any(n < 0 for n in sizes) or any(p < 0 for p in prefixes):
         raise ValueError("a size and a prefix, neither negative, for every group")
     if sum(sizes) > rows or (prefixes and max(prefixes) > max_len):
@@ -299,6 +300,8 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise ValueError(f"the workspace must hold {need} contiguous fp32 elements on the queries' device")
     if not batch:
         return out
+    if dev.type != "cuda":
+        raise ValueError("the kernel runs on a GPU")
     if batch > MAX_SHARED_ROWS:
         raise ValueError(f"{batch} rows: up to {MAX_SHARED_ROWS} are supported")
     if not k_cache.shape[0]:

@@ -110,6 +110,8 @@ def _args(logits: torch.Tensor, c: LogitControls) -> "native.LogitArgs":
 
 
 def _launch(s, dev) -> None:
+    if dev.type != "cuda":
+        raise ValueError("the kernel runs on a GPU")
     with native.on_device(dev):
         native.check(native.kernels().xp_logit_controls(C.byref(s), native.stream_of(dev)), "xp_logit_controls")
 
@@ -135,7 +137,7 @@ def select_tokens(logits: torch.Tensor, controls: LogitControls, temps: torch.Te
     """One token per row from the logits after ``controls``: the largest one (ties go to the lower id), or where ``temps[r] > 0`` a
     draw from ``softmax(adjusted / temperature)`` with ``seeds`` int32 ``[rows, 2]`` as in
     :func:`crosspool_b200.ops.attention.sample`. ``values`` (fp32 ``[rows]``) receives the adjusted logit of the token. A row without
-    an allowed token gives token 0 and the value ``-inf``."""
+    an allowed token gives token 0 and the value ``-inf``; NaN is never the largest."""
     s = _args(logits, controls)
     rows, dev = logits.shape[0], logits.device
     if logits.shape[1] == 0:

@@ -160,6 +160,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: Adapte
             raise ValueError("rows must be contiguous, 16-byte aligned, with pitches of whole 16 bytes")
     if plan.words.device != dev:
         raise ValueError("the plan lives on another device")
+    if rows and out.data_ptr() == x.data_ptr():
+        raise ValueError("out may be y, but not x")
+    if dev.type != "cuda":
+        raise ValueError("the kernel runs on a GPU")
     s = native.LoraArgs.from_buffer_copy(stack._fields)
     s.x, s.y, s.out = x.data_ptr(), y.data_ptr(), out.data_ptr()
     s.items, s.n_items, s.perm = plan._items, plan._n_items, plan._perm

@@ -141,6 +141,15 @@ def test_adapter_calls_that_are_refused():
             lora.lora_add(*args, **kw)
 
 
+def test_calls_on_the_cpu_are_refused():
+    s, p = lora.AdapterStack(1, 64, 64, 8, device="cpu"), lora.adapter_plan([0, -1], 1, device="cpu")
+    x, y = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(2, 64, dtype=torch.bfloat16)
+    for call in (lambda: lora.lora_add(y, x, s, p), lambda: lora.lora_add(y, x, s, p, out=x), lambda: A.paged_decode_shared(**attention_args()),
+                 lambda: L.adjust_logits(x, L.LogitControls()), lambda: L.select_tokens(x, L.LogitControls())):
+        with pytest.raises(ValueError, match="GPU|not x"):
+            call()
+
+
 def test_controls_that_are_refused():
     i, f = (lambda *s: torch.zeros(*s, dtype=torch.int32)), (lambda *s: torch.zeros(*s))
     for kw in (dict(history=i(2, 5)), dict(lens=i(2)), dict(history=f(2, 5), lens=i(2)), dict(history=i(2, 5), lens=i(3)), dict(history=i(5), lens=i(2)),

@@ -221,3 +221,51 @@ def run_quietly(sizes, prefixes, q, k, v, table, lens):
 
     plan = A.shared_prefix_plan(sizes, prefixes, rows=q.shape[0], q_heads=q.shape[1], kv_heads=k.shape[2], head_dim=q.shape[2], max_len=700)
     return A.paged_decode_shared(q, k, v, table, lens, plan)
+
+
+def test_a_cache_of_more_than_two_billion_elements():
+    """Pages at both ends of caches whose offsets do not fit 32 bits."""
+    q, k, v, table, lens = make([6], [640], 1, [1, 70, 300], 8, 8, 128, 64, poison=False)
+    pages = 2 ** 31 // (64 * 8 * 128) + 4096                         # 2.4 G elements each
+    used = torch.unique(torch.cat([table[r, :(int(n) + 63) // 64] for r, n in enumerate(lens)])).long()
+    to = torch.cat([torch.arange(len(used) // 2), pages - 1 - torch.arange(len(used) - len(used) // 2)]).cuda()[torch.randperm(len(used), generator=torch.Generator().manual_seed(2)).cuda()]
+    new = torch.zeros(k.shape[0], dtype=torch.int64, device="cuda")
+    new[used] = to
+    big = [torch.empty(pages, 64, 8, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for b, c in zip(big, (k, v)):
+        b[to] = c[used]
+    moved = new[table.long()].int()
+    got = run([6], [640], q, *big, moved, lens)
+    close(got, q, k, v, table, lens)
+    assert torch.equal(got, run([6], [640], q, k, v, table, lens))
+
+
+def test_most_rows():
+    """As many rows as a batch may have, in groups and alone."""
+    sizes, prefixes = [3000, 500], [96, 32]
+    data = make(sizes, prefixes, 596, [1, 3, 18], 2, 1, 64, 16)
+    close(run(sizes, prefixes, *data), *data)
+
+
+def test_workspaces_of_two_captured_graphs():
+    """Two graphs captured on one stream, each with memory of its own, replayed on two streams at once."""
+    from crosspool_b200.ops import attention as A
+
+    sets = [make([24], [512], 0, [5, 80], 8, 2, 128, 64, seed=i) for i in range(2)]
+    want = [run([24], [512], *s) for s in sets]
+    plans = [A.shared_prefix_plan([24], [512], rows=24, q_heads=8, kv_heads=2, head_dim=128, max_len=int(s[4].max())) for s in sets]
+    stream, graphs, outs = torch.cuda.Stream(), [], []
+    stream.wait_stream(torch.cuda.current_stream())
+    for s, p in zip(sets, plans):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            outs.append(A.paged_decode_shared(*s, p))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
