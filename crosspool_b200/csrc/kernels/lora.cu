@@ -35,6 +35,10 @@ constexpr int kPitch = 64 + 4;                       // fp32 row of a warp's par
 __device__ __forceinline__ void copy16(uint32_t dst, const bf16* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
+// (kept in the L1: other warps of the CTA read the same)
+__device__ __forceinline__ void copy16_kept(uint32_t dst, const bf16* src, bool ok) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ void copy8(uint32_t dst, const bf16* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // waits until at most `left` of the groups issued last are in flight
@@ -135,7 +139,12 @@ lora_kernel(XpLoraArgs a, int ranks) {
       continue;                                      // (the same for all CTAs of the cluster)
     }
     const bf16* bw = reinterpret_cast<const bf16*>(a.b) + static_cast<size_t>(slot) * a.n * a.rank;
-    if (b1 > b0 && warp == 0) {
+    // ---- h = x A^T, this CTA's share of k
+    const int kblocks = (a.k + 31) >> 5;
+    const int k0 = static_cast<int>(static_cast<long long>(kblocks) * rank / ranks), k1 = static_cast<int>(static_cast<long long>(kblocks) * (rank + 1) / ranks);
+    const bf16* x = reinterpret_cast<const bf16*>(a.x);
+    const bf16* aw = reinterpret_cast<const bf16*>(a.a) + static_cast<size_t>(slot) * a.parts * a.rank * a.k;
+    auto prefetch_second = [&]() {                   // B and y of the second product, to the L2
       int p, f, end, f1;
       locate(b1 - 1, p, f1, end);
       f1 = min(f1 + 32, end);
@@ -144,13 +153,7 @@ lora_kernel(XpLoraArgs a, int ranks) {
       for (uint32_t at = lane * 4096u; at < bytes; at += 32 * 4096u)
         prefetch_l2(reinterpret_cast<const uint8_t*>(bw + static_cast<size_t>(f) * rk) + at, min(4096u, bytes - at));
       if (lane < item.rows) prefetch_l2(y + static_cast<size_t>(a.perm[item.first + lane]) * a.ld_y + f, static_cast<uint32_t>(f1 - f) * 2);
-    }
-
-    // ---- h = x A^T, this CTA's share of k
-    const int kblocks = (a.k + 31) >> 5;
-    const int k0 = static_cast<int>(static_cast<long long>(kblocks) * rank / ranks), k1 = static_cast<int>(static_cast<long long>(kblocks) * (rank + 1) / ranks);
-    const bf16* x = reinterpret_cast<const bf16*>(a.x);
-    const bf16* aw = reinterpret_cast<const bf16*>(a.a) + static_cast<size_t>(slot) * a.parts * a.rank * a.k;
+    };
     // The warps share the columns of h in groups of kTiles tiles, and those of a group its blocks of k.
     const int all = a.parts * rk, n_tiles = all >> 3;   // columns of h, part after part
     const int groups = n_tiles <= kTiles ? 1 : n_tiles <= 2 * kTiles ? 2 : n_tiles <= 4 * kTiles ? 4 : 8, each = kWarps / groups;
@@ -173,8 +176,8 @@ lora_kernel(XpLoraArgs a, int ranks) {
         const bool in = kb < k1 && k < a.k;
         const int at = in ? k : 0;
         if (kb < k1) {
-          copy16(ring + s * stage, x0 + at, in && on0);
-          copy16(ring + s * stage + 512, x1 + at, in && on1);
+          copy16_kept(ring + s * stage, x0 + at, in && on0);
+          copy16_kept(ring + s * stage + 512, x1 + at, in && on1);
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
             if (t < tiles) copy16(ring + s * stage + 1024 + t * 512, wrow[t] + at, in);
@@ -183,6 +186,7 @@ lora_kernel(XpLoraArgs a, int ranks) {
       };
       const int kb0 = k0 + warp % each;
       for (int i = 0; i < depth; ++i) issue(kb0 + i * each, i);
+      if (warp == 0 && b1 > b0) prefetch_second();
       int s = 0;
       for (int kb = kb0; kb < k1; kb += each) {
         landed(depth - 1);

@@ -136,7 +136,7 @@ class AdapterRows:
     def fill(self, index: list[int], rows: int) -> int:
         """Writes the plan of a pass over ``rows`` rows to the pinned mirror (``index``: slots of the first rows); number of items."""
         n = lora.plan_words(rows)
-        return lora.fill_plan(index + [-1] * (rows - len(index)), self.host.numpy()[:n], rows, bare=False)
+        return lora.fill_plan(index + [-1] * (rows - len(index)), self.host.numpy()[:n], rows, bare=False, ranks=self.qkv[0].used)
 
     def copy(self, rows: int) -> None:
         n = lora.plan_words(rows)

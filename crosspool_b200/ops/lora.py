@@ -40,6 +40,7 @@ class AdapterStack:
         self.ranks = torch.zeros(slots, dtype=torch.int32, device=device)
         self.device = self.a.device
         self._fresh = [True] * slots       # never loaded: still zero
+        self.used = [0] * slots            # ranks in use, as in `ranks`
         end, ends = 0, []
         for n in self.parts:
             end += n
@@ -81,12 +82,14 @@ class AdapterStack:
             at += n
         self.scale[slot:slot + 1].fill_(float(scale))
         self.ranks[slot:slot + 1].fill_(r16)
+        self.used[slot] = r16
 
     def clear(self, slot: int) -> None:
         """Empties ``slot``: rows that name it keep ``y``."""
         if not 0 <= slot < self.slots:
             raise ValueError(f"slot {slot} of {self.slots}")
         self.ranks[slot:slot + 1].zero_()
+        self.used[slot] = 0
 
 
 def plan_words(rows: int) -> int:
@@ -94,9 +97,10 @@ def plan_words(rows: int) -> int:
     return 4 + 5 * rows
 
 
-def fill_plan(index: Sequence[int], words: np.ndarray, rows: int, bare: bool = True) -> int:
+def fill_plan(index: Sequence[int], words: np.ndarray, rows: int, bare: bool = True, ranks: Sequence[int] | None = None) -> int:
     """Writes the plan of ``index`` (adapter slot per row, negative: none) to ``words`` (``plan_words(rows)`` of them); returns its
-    number of items. ``bare``: rows without an adapter get items too (they are copied when the result goes elsewhere)."""
+    number of items. ``bare``: rows without an adapter get items too (they are copied when the result goes elsewhere). ``ranks``: of
+    the slots; items of high ranks come first, so that the last ones to start are short."""
     idx = np.maximum(np.asarray(index, dtype=np.int64).reshape(-1), -1)
     order = np.argsort(idx, kind="stable")
     srt = idx[order]
@@ -111,6 +115,10 @@ def fill_plan(index: Sequence[int], words: np.ndarray, rows: int, bare: bool = T
     if not bare:
         keep = slot >= 0
         first, n, slot = first[keep], n[keep], slot[keep]
+    if ranks is not None and len(slot):
+        cost = np.where(slot >= 0, np.asarray(ranks, dtype=np.int64)[np.maximum(slot, 0)], -1)
+        by = np.argsort(-cost, kind="stable")
+        first, n, slot = first[by], n[by], slot[by]
     items = words[4:4 + 4 * rows].reshape(rows, 4)
     items[:len(slot), 0], items[:len(slot), 1], items[:len(slot), 2] = slot, first, n
     words[4 + 4 * rows:4 + 4 * rows + len(order)] = order
@@ -138,7 +146,7 @@ def adapter_plan(index: Sequence[int], stack: "AdapterStack | int", device: str 
     if rows and max(index) >= slots:
         raise ValueError(f"adapter slot {max(index)} of {slots}")
     host = np.zeros(plan_words(rows), dtype=np.int32)
-    n = fill_plan(index, host, rows)
+    n = fill_plan(index, host, rows, ranks=stack.used if isinstance(stack, AdapterStack) else None)
     return AdapterPlan(torch.from_numpy(host).to(device), rows, n, slots)
 
 
