@@ -59,6 +59,7 @@ typedef struct XpLoraArgs {
   const void* b;              /* bf16, n * rank elements per slot, of which [n, ranks[slot]] are used, without gaps */
   const float* scale;         /* [slots] */
   const int* ranks;           /* [slots] rank in use, rounded up to 16; what lies behind it is zero */
+  const int* part_ranks;      /* [slots, XP_LORA_PARTS] the parts' own ranks (0: none) */
   const XpLoraItem* items;
   const int* n_items;         /* device word */
   const int* perm;            /* [rows] */

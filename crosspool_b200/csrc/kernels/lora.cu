@@ -260,11 +260,24 @@ lora_kernel(XpLoraArgs a, int ranks) {
         add4(u, *reinterpret_cast<const float4*>(from + s * 256));
         add4(v, *reinterpret_cast<const float4*>(from + s * 256 + 128));
       }
+      // Ranks behind a part's own are zero, whatever zeros times x gave; an infinity has no low part.
+      const int col = (kb * ranks + rank) * 16, over = a.part_ranks[slot * XP_LORA_PARTS + col / rk] - col % rk - (l & 3) * 4;
+      if (over < 4) {
+        if (over < 1) u.x = v.x = 0.f;
+        if (over < 2) u.y = v.y = 0.f;
+        if (over < 3) u.z = v.z = 0.f;
+        u.w = v.w = 0.f;
+      }
       uint4 hi, lo;
-      frag::split2(u.x, u.y, hi.x, lo.x);
-      frag::split2(v.x, v.y, hi.y, lo.y);
-      frag::split2(u.z, u.w, hi.z, lo.z);
-      frag::split2(v.z, v.w, hi.w, lo.w);
+      auto split2 = [](float e, float f, uint32_t& h, uint32_t& low) {
+        frag::split2(e, f, h, low);
+        if (isinf(e)) low &= 0xffff0000u;
+        if (isinf(f)) low &= 0x0000ffffu;
+      };
+      split2(u.x, u.y, hi.x, lo.x);
+      split2(v.x, v.y, hi.y, lo.y);
+      split2(u.z, u.w, hi.z, lo.z);
+      split2(v.z, v.w, hi.w, lo.w);
       const uint32_t to = frags_addr + static_cast<uint32_t>((kb * ranks + rank) * 32 + l) * 32u;
       for (int s = 0; s < ranks; ++s) {
         const uint32_t at = sm100::map_rank(to, s);

@@ -309,14 +309,16 @@ __device__ __forceinline__ void own_worker(const CUtensorMap* tmap_k, const CUte
       x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, o));
       x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, o));
     }
-    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);              // finite: every tile has a token
+    const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
     if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
-      const float c0 = exp2f(m0 - n0), c1 = exp2f(m1 - n1);
+      const float c0 = n0 > m0 ? exp2f(m0 - n0) : 1.f, c1 = n1 > m1 ? exp2f(m1 - n1) : 1.f;
       l0 *= c0, l1 *= c1, m0 = n0, m1 = n1;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) acc[j][0] *= c0, acc[j][1] *= c1, acc[j][2] *= c0, acc[j][3] *= c1;
     }
-    const float p0 = exp2f(v[0] - m0), p1 = exp2f(v[1] - m1), p2 = exp2f(v[2] - m0), p3 = exp2f(v[3] - m1);
+    // (keys that hold an infinity may leave no score above -inf so far: weights of 0 then)
+    const float z0 = m0 == -CUDART_INF_F ? 0.f : m0, z1 = m1 == -CUDART_INF_F ? 0.f : m1;
+    const float p0 = exp2f(v[0] - z0), p1 = exp2f(v[1] - z1), p2 = exp2f(v[2] - z0), p3 = exp2f(v[3] - z1);
     l0 += p0 + p2, l1 += p1 + p3;
     const uint32_t b0 = transpose8x8(pack2(p0, p1)), b1 = transpose8x8(pack2(p2, p3));
 #pragma unroll

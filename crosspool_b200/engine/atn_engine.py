@@ -655,6 +655,9 @@ class AttentionEngine:
             hv = self.dec_meta_host.numpy()
             hv[2 * self.ecfg.max_batch:3 * self.ecfg.max_batch] = -1  # no KV writes for padding rows
             self.dec_meta.copy_(self.dec_meta_host, non_blocking=True)
+            for options in (self.prefix_rows, self.adapter_rows):
+                if options is not None:
+                    options.words.zero_()        # the plan of another row bucket lies otherwise
             # First contact with the FFN ranks (kernel loading on both sides, first touch of peer mappings, Lane
             # threads reaching their first replay) gets a generous wait limit; every later wait keeps the normal one.
             relax = getattr(self.port, "set_wait_limit", None)
@@ -1036,7 +1039,11 @@ class AttentionEngine:
         with torch.cuda.stream(self.stream):
             self.dec_meta.copy_(self.dec_meta_host, non_blocking=True)
             self._stage_sampling(batch)
-            self._stage_options(batch, [True] * n, [self._adapter_slot(s) for s in batch] if self.adapter_rows is not None else None, B)
+            try:
+                self._stage_options(batch, [True] * n, [self._adapter_slot(s) for s in batch] if self.adapter_rows is not None else None, B)
+            except Exception:
+                self._b_key = None               # the step's rows are written anew when it is taken again
+                raise
             if self.prefix_rows is not None:
                 self.prefix_rows.copy()
             self._replay_decode(B)

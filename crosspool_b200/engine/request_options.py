@@ -220,6 +220,8 @@ class ControlRows:
     def stage(self, seqs: list, samples: list[bool]) -> None:
         """Fills and copies the rows of a pass (on the engine's stream): ``seqs[i]`` samples its next token in row i unless
         ``samples[i]`` is False (a portion of a prompt that is not its last)."""
+        # what may raise comes first: a step that failed here can be taken again
+        words = [self._mask(s) if wanted and s.controls is not None and s.controls.allowed is not None else None for s, wanted in zip(seqs, samples)]
         self._neutral()
         n, h = self.rows, self.meta_host.numpy()
         f, ids, vals = h[5 * n:8 * n].view(np.float32).reshape(3, n), self.bias_host[0].numpy(), self.bias_host[1].numpy().view(np.float32)
@@ -235,12 +237,8 @@ class ControlRows:
             for t, v in c.bias.items():
                 ids[biases], vals[biases] = t, v
                 biases += 1
-            words = c.allowed(list(s.generated)) if c.allowed is not None else None
-            if words is not None:
-                words = np.asarray(words)
-                if words.shape != (self.words,):
-                    raise ValueError(f"a mask of shape {words.shape} for {self.vocab} tokens ({self.words} words)")
-                self.masks_host[masks].numpy()[:] = words.astype(np.uint32).view(np.int32) if words.dtype != np.int32 else words
+            if words[i] is not None:
+                self.masks_host[masks].numpy()[:] = words[i]
                 h[4 * n + i] = masks
                 masks += 1
         h[8 * n + len(seqs):] = biases
@@ -249,6 +247,15 @@ class ControlRows:
             self.bias[:, :biases].copy_(self.bias_host[:, :biases], non_blocking=True)
         if masks:
             self.masks[:masks].copy_(self.masks_host[:masks], non_blocking=True)
+
+    def _mask(self, s) -> "np.ndarray | None":
+        words = s.controls.allowed(list(s.generated))
+        if words is None:
+            return None
+        words = np.asarray(words)
+        if words.shape != (self.words,):
+            raise ValueError(f"a mask of shape {words.shape} for {self.vocab} tokens ({self.words} words)")
+        return words.astype(np.uint32).view(np.int32) if words.dtype != np.int32 else words
 
     def _history(self, i: int, s, h: np.ndarray) -> None:
         """Row i's history: its slot gets the whole sequence once, then every call the token that the sequence grew by."""

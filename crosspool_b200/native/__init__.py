@@ -328,7 +328,7 @@ def _struct(name: str, doc: str, **fields):
 
 
 # request_api.h
-LoraArgs = _struct("LoraArgs", "XpLoraArgs", a_ptr="x y out a b scale ranks items n_items perm",
+LoraArgs = _struct("LoraArgs", "XpLoraArgs", a_ptr="x y out a b scale ranks part_ranks items n_items perm",
                    b_int="rows k n rank parts slots max_items ldx ld_y ld_out", c_int4="part_end")
 LogitArgs = _struct("LogitArgs", "XpLogitArgs (its controls first)",
                     a_ptr="history history_rows lens prompt_lens latest repetition frequency presence bias_ids bias_values bias_starts masks mask_index",

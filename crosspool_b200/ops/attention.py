@@ -212,8 +212,7 @@ class SharedPrefixPlan:
     a captured graph may be replayed with other words that keep to them. ``max_len`` bounds the sequences' lengths."""
 
     def __init__(self, words: torch.Tensor, rows: int, max_pieces: int, max_parts: int, max_len: int, q_heads: int, kv_heads: int, head_dim: int):
-        if rows > MAX_SHARED_ROWS or rows * -(-max_len // 16) * kv_heads * 2 >= 2 ** 31:
-            raise ValueError(f"{rows} rows of up to {max_len} tokens: up to {MAX_SHARED_ROWS} rows and 2^31 tiles of 16 tokens are supported")
+        _check_size(rows, max_len, kv_heads)
         self.words, self.rows, self.max_pieces, self.max_parts = words, rows, max_pieces, max_parts
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
         self.slices = decode_plan(max(rows, 1), kv_heads, max(max_len, 1)) if max_pieces == 0 else (1, 0)   # without prefixes: paged_decode's
@@ -257,6 +256,11 @@ def shared_prefix_plan(sizes: Sequence[int], prefixes: Sequence[int], *, rows: i
     return SharedPrefixPlan(torch.from_numpy(words).to(device), rows, count, parts, max_len, q_heads, kv_heads, head_dim)
 
 
+def _check_size(rows: int, max_len: int, kv_heads: int) -> None:
+    if rows > MAX_SHARED_ROWS or rows * -(-max_len // 16) * kv_heads * 2 >= 2 ** 31:
+        raise ValueError(f"{rows} rows of up to {max_len} tokens: up to {MAX_SHARED_ROWS} rows and 2^31 tiles of 16 tokens are supported")
+
+
 def _check_heads(q_heads: int, kv_heads: int, head_dim: int) -> None:
     if kv_heads < 1 or q_heads % kv_heads or not 1 <= q_heads // kv_heads <= 16 or head_dim not in (64, 128):
         raise ValueError(f"{q_heads} query and {kv_heads} KV heads of {head_dim}: up to 16 query heads per KV head of 64 or 128 are supported")
@@ -292,6 +296,12 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise ValueError("out must be like q")
     if out.data_ptr() % 16 or (ws is not None and ws.data_ptr() % 16):
         raise ValueError("out and the workspace must be 16-byte aligned")
+    if scale is None:
+        scale = d ** -0.5
+    elif not 0 < scale < math.inf:
+        raise ValueError(f"scale {scale}: the kernel takes positive numbers")
+    if batch > plan.rows:
+        _check_size(batch, plan.max_len, kv_heads)
     need = plan.workspace_floats(batch)
     if ws is None:
         if need:
@@ -302,8 +312,6 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         return out
     if dev.type != "cuda":
         raise ValueError("the kernel runs on a GPU")
-    if batch > MAX_SHARED_ROWS:
-        raise ValueError(f"{batch} rows: up to {MAX_SHARED_ROWS} are supported")
     if not k_cache.shape[0]:
         raise ValueError("a cache of no pages")
     s = native.DecodeSharedArgs.from_buffer_copy(plan._fields)
@@ -312,7 +320,7 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     a.ws = ws.data_ptr() if ws is not None else None
     a.block_table, a.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
     a.batch, a.page_size, a.max_blocks, a.num_pages = batch, page, block_table.stride(0), k_cache.shape[0]
-    a.scale = scale if scale is not None else d ** -0.5
+    a.scale = scale
     from .gemm import status_words
 
     a.status = status_words(dev).data_ptr()

@@ -23,7 +23,7 @@ class LogitControls:
     """What is done to the rows of a batch of logits; every tensor is optional and lives on the logits' device. Steps, in fp32 and
     in this order: ``v / repetition`` where ``v > 0`` and ``v * repetition`` elsewhere, for tokens of the history; minus ``frequency``
     times the occurrences behind the prompt; minus ``presence`` where there are any; plus the biases of the token; ``-inf`` where the
-    mask does not allow it.
+    mask does not allow it. Rows may name the same history, but then not bring a ``latest`` token for it.
 
     The tensors are read when a call runs: their contents may change between calls (and between replays of a captured graph)."""
 
@@ -76,6 +76,9 @@ class LogitControls:
             s.bias_total = self.bias_ids.shape[0]
         if len(rows) > 1 or len(devices) > 1:
             raise ValueError(f"controls of {sorted(rows)} rows on {len(devices)} devices")
+        for t in (self.history, self.masks):
+            if t is not None and t.shape[0] > 1 and not t.shape[1] <= t.stride(0) < 2 ** 31:
+                raise ValueError(f"rows of {t.shape[1]} words {t.stride(0)} apart")
         if self.history is not None:
             s.history_slots, s.history_cap, s.ld_history = *self.history.shape, self.history.stride(0)
             if self.history_rows is None and rows and self.history.shape[0] < max(rows):
@@ -96,6 +99,9 @@ def _args(logits: torch.Tensor, c: LogitControls) -> "native.LogitArgs":
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
         raise ValueError("logits must be bf16 or fp32 [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
+    ld = logits.stride(0) if rows > 1 else vocab
+    if not vocab <= ld < 2 ** 31:
+        raise ValueError(f"rows of {vocab} logits {ld} elements apart")
     if vocab > MAX_VOCAB:
         raise ValueError(f"{vocab} tokens: up to {MAX_VOCAB} are supported")
     if c._rows is not None and c._rows < rows:
@@ -105,7 +111,7 @@ def _args(logits: torch.Tensor, c: LogitControls) -> "native.LogitArgs":
     if c.masks is not None and c.masks.shape[0] and c.masks.shape[1] * 32 < vocab:
         raise ValueError(f"masks of {c.masks.shape[1]} words for {vocab} tokens")
     s = native.LogitArgs.from_buffer_copy(c._fields)
-    s.logits, s.rows, s.vocab, s.ld, s.f32 = logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, int(logits.dtype == _FLOAT)
+    s.logits, s.rows, s.vocab, s.ld, s.f32 = logits.data_ptr(), rows, vocab, ld, int(logits.dtype == _FLOAT)
     return s
 
 
@@ -124,9 +130,12 @@ def adjust_logits(logits: torch.Tensor, controls: LogitControls, *, out: torch.T
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     if out.shape != logits.shape or out.dtype not in (torch.bfloat16, _FLOAT) or out.stride(1) != 1 or out.device != logits.device:
         raise ValueError("out must be bf16 or fp32 of the logits' shape, with contiguous rows, on their device")
-    if out.data_ptr() == logits.data_ptr() and out.numel() and (out.dtype != logits.dtype or out.stride(0) != logits.stride(0)):
+    ld_out = out.stride(0) if out.shape[0] > 1 else out.shape[1]
+    if not out.shape[1] <= ld_out < 2 ** 31:
+        raise ValueError(f"rows of {out.shape[1]} results {ld_out} elements apart")
+    if out.data_ptr() == logits.data_ptr() and out.numel() and (out.dtype != logits.dtype or ld_out != s.ld):
         raise ValueError("adjusting in place keeps type and pitch")
-    s.out, s.ld_out, s.out_f32 = out.data_ptr(), out.stride(0) if out.shape[0] > 1 else out.shape[1], int(out.dtype == _FLOAT)
+    s.out, s.ld_out, s.out_f32 = out.data_ptr(), ld_out, int(out.dtype == _FLOAT)
     if out.numel():
         _launch(s, logits.device)
     return out

@@ -38,6 +38,7 @@ class AdapterStack:
         self.b = torch.zeros(slots, self.out_features * self.rank, dtype=torch.bfloat16, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
         self.ranks = torch.zeros(slots, dtype=torch.int32, device=device)
+        self.part_ranks = torch.zeros(slots, MAX_PARTS, dtype=torch.int32, device=device)
         self.device = self.a.device
         self._fresh = [True] * slots       # never loaded: still zero
         self.used = [0] * slots            # ranks in use, as in `ranks`
@@ -47,10 +48,12 @@ class AdapterStack:
             ends.append(end)
         s = native.LoraArgs()
         s.a, s.b, s.scale, s.ranks = self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), self.ranks.data_ptr()
+        s.part_ranks = self.part_ranks.data_ptr()
         s.k, s.n, s.rank, s.parts, s.slots = in_features, self.out_features, self.rank, len(self.parts), slots
         s.part_end = (C.c_int * 4)(*(ends + [end] * (4 - len(ends))))
         self._fields = bytes(s)
 
+    @torch.no_grad()
     def load(self, slot: int, a: torch.Tensor | Sequence[torch.Tensor], b: torch.Tensor | Sequence[torch.Tensor], scale: float = 1.0) -> None:
         """Puts an adapter into ``slot``: ``a`` ``[r, in]`` and ``b`` ``[out, r]``, or one pair per part (``None`` for a part
         without one); ranks may differ between parts. Ordered with the work of the current stream."""
@@ -82,6 +85,8 @@ class AdapterStack:
             at += n
         self.scale[slot:slot + 1].fill_(float(scale))
         self.ranks[slot:slot + 1].fill_(r16)
+        for i, x in enumerate(pa):
+            self.part_ranks[slot, i].fill_(0 if x is None else x.shape[0])
         self.used[slot] = r16
 
     def clear(self, slot: int) -> None:
@@ -164,8 +169,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: Adapte
     for t in (x, y, out):
         if t.dtype != torch.bfloat16 or t.device != dev:
             raise ValueError(f"{t.dtype} on {t.device}: bf16 on the stack's device ({dev}) is supported")
-        if t.stride(1) != 1 or (rows > 1 and t.stride(0) % 8) or t.data_ptr() % 16:
+        if t.stride(1) != 1 or (rows > 1 and (t.stride(0) % 8 or t.stride(0) >= 2 ** 31)) or t.data_ptr() % 16:
             raise ValueError("rows must be contiguous, 16-byte aligned, with pitches of whole 16 bytes")
+    if rows > 1 and (out.stride(0) < stack.out_features or (out.data_ptr() == y.data_ptr() and out.stride(0) != y.stride(0))):
+        raise ValueError("the rows of out must not overlap one another or other rows of y")
     if plan.words.device != dev:
         raise ValueError("the plan lives on another device")
     if rows and out.data_ptr() == x.data_ptr():

@@ -150,3 +150,20 @@ def test_graph_replays_with_other_plans():
         graph.replay()
         torch.cuda.synchronize()
         check(out, x, y, pairs, scales, index, 32)
+
+
+def test_infinities_go_through_the_ranks_that_there_are():
+    """Ranks that only fill up a tile, and parts without an adapter, add nothing to a row of infinities. Every A and B is positive:
+    the formula gives infinities, no NaN."""
+    from crosspool_b200.ops import lora
+
+    index = [0, 1, 0, 1]
+    x, y, stack, pairs, scales = make(4, 256, (64, 32, 64), [8, 21], 32, index, missing={(0, 1), (1, 0)})
+    pairs = [[(None if m is None else tuple(t.abs() + 0.125 for t in m), f) for m, f in p] for p in pairs]
+    for s, p in enumerate(pairs):
+        stack.load(s, [m[0] if m else None for m, _ in p], [m[1] if m else None for m, _ in p], scales[s])
+    x[0, 3], x[1, 200] = float("inf"), float("-inf")
+    got, inf = lora.lora_add(y, x, stack, lora.adapter_plan(index, stack)), float("inf")
+    assert (got[0, :64] == inf).all() and torch.equal(got[0, 64:96], y[0, 64:96]) and (got[0, 96:] == inf).all()
+    assert torch.equal(got[1, :64], y[1, :64]) and (got[1, 64:] == -inf).all()
+    check(got[2:], x[2:], y[2:], pairs, scales, index[2:], 32)

@@ -170,3 +170,44 @@ def test_controls_that_are_refused():
                  lambda: L.select_tokens(x, c, out=f(2))):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("inf"), float("nan")])
+def test_scales_that_are_refused(scale):
+    with pytest.raises(ValueError, match="scale"):
+        A.paged_decode_shared(**attention_args(), scale=scale)
+
+
+def test_batches_that_are_too_large_for_a_small_plan():
+    rows, max_len = 4096, 1 << 20
+    a = attention_args(q=torch.zeros(rows, 8, 128, dtype=torch.bfloat16), k_cache=torch.zeros(9, 16, 4, 128, dtype=torch.bfloat16),
+                       v_cache=torch.zeros(9, 16, 4, 128, dtype=torch.bfloat16), block_table=torch.zeros(1, max_len // 16, dtype=torch.int32).expand(rows, -1),
+                       seq_lens=torch.zeros(rows, dtype=torch.int32), plan=plan([4], [64], 4, 8, 4, max_len=max_len))
+    with pytest.raises(ValueError, match="tiles"):
+        A.paged_decode_shared(**a)
+
+
+def test_results_that_overlap_are_refused():
+    b = torch.bfloat16
+    s = lora.AdapterStack(2, 64, 48, 16, device="cpu")
+    p, x = lora.adapter_plan([0, 1, -1], s), torch.zeros(3, 64, dtype=b)
+    buf = torch.zeros(3 * 64, dtype=b)
+    y = buf.view(3, 64)[:, :48]
+    for out in (buf[:48].expand(3, 48), buf.as_strided((3, 48), (40, 1)), buf[:144].view(3, 48)):
+        with pytest.raises(ValueError, match="overlap"):
+            lora.lora_add(y, x, s, p, out=out)
+    z = torch.zeros(100)
+    with pytest.raises(ValueError, match="apart"):
+        L.adjust_logits(z.expand(3, 100), L.LogitControls())
+    with pytest.raises(ValueError, match="apart"):
+        L.adjust_logits(torch.zeros(3, 100), L.LogitControls(), out=z.expand(3, 100))
+    with pytest.raises(ValueError, match="apart"):
+        L.LogitControls(masks=torch.zeros(4, dtype=torch.int32).expand(2, 4), mask_index=torch.zeros(2, dtype=torch.int32))
+
+
+def test_adapters_that_are_trained_can_be_loaded():
+    s = lora.AdapterStack(1, 64, (32, 16), 20, device="cpu")
+    a, b = torch.ones(3, 64, requires_grad=True), torch.ones(16, 3, requires_grad=True)
+    s.load(0, [None, a], [None, b])
+    s.load(0, [None, a], [None, b], 2.0)
+    assert not s.a.requires_grad and not s.b.requires_grad and s.part_ranks.tolist() == [[0, 3, 0, 0]] and s.a.sum() == 3 * 64

@@ -284,3 +284,44 @@ def test_engines_that_are_refused():
     with pytest.raises(ValueError, match="rank"):
         eng.load_adapter("a", adapter(cfg, 1, rank=17))
     assert not eng.adapter_rows.names
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_step_whose_mask_failed_can_be_taken_again(graph):
+    from crosspool_b200.engine.request_options import TokenControls
+
+    results = []
+    for fail in (False, True):
+        cfg, eng, _ = build(controls=True, shared_prefix=True, prefix_cache=True, use_cuda_graph=graph, max_batch=8)
+        eng.warmup()
+        failed = []
+
+        def allowed(g):
+            if fail and len(g) in (0, 3, 4) and len(g) not in failed:
+                failed.append(len(g))
+                raise RuntimeError("no mask yet")
+            return only(cfg.vocab_size, range(len(g), 3000))
+
+        a, b = prompts(cfg, [30, 41], shared=20, seed=3)
+        seqs = [eng.add_request(a, 8, controls=TokenControls(repetition=1.3, frequency=0.5)), eng.add_request(b, 8, controls=TokenControls(allowed=allowed))]
+        while eng.has_work:
+            try:
+                eng.step()
+            except RuntimeError as e:
+                assert str(e) == "no mask yet"
+        assert failed == ([0, 3, 4] if fail else [])
+        results.append([s.generated for s in seqs])
+    assert results[0] == results[1]
+
+
+def test_an_engine_is_warmed_up_again():
+    """The plans' words of the last batch lie as its row bucket's; the other buckets' graphs find none."""
+    cfg, eng, ref = build(shared_prefix=True, prefix_cache=True, adapters=2, max_batch=16)
+    eng.load_adapter("a", adapter(cfg, 5))
+    reqs = [((p, 6), dict(adapter=n)) for p, n in zip(prompts(cfg, [50, 60, 70, 40, 33], shared=32, seed=4), ["a", None, "a", None, "a"])]
+    eng.warmup()
+    first, got = logits_of(eng, reqs)
+    eng.warmup()
+    assert not eng.prefix_rows.words.any() and not eng.adapter_rows.words.any()
+    second, again = logits_of(eng, reqs)
+    assert [s.generated for s in first] == [s.generated for s in second]

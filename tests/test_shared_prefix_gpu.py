@@ -269,3 +269,23 @@ def test_workspaces_of_two_captured_graphs():
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("prefix", [0, 512])
+def test_keys_of_minus_infinity_weigh_nothing(prefix, d):
+    """The first 40 own tokens of every row, and (but for one) the first 160 of the prefix, have scores of -inf. Without a prefix the
+    plan has one piece all the same, of rows that are empty."""
+    hk, page, rows = 2, 16, 5
+    q, k, v, table, lens = make([rows - 2, 2], [prefix, 64], 0, [90, 41, 300], 8, hk, d, page)
+    lens[rows - 2:] = 0
+    q = q.abs()
+    low = torch.tensor(float("-inf"), device="cuda").bfloat16()
+    for r in range(rows - 2):
+        for t in [*range(prefix, prefix + 40), *range(min(160, max(prefix - 1, 0)))]:
+            k[table[r, t // page].long(), t % page, :, 5] = low
+    k[table[rows - 2, :4].long()] = 0
+    v[table[rows - 2, :4].long()] = 0
+    got = run([rows - 2, 2], [prefix, 64], q, k, v, table, lens)
+    close(got, q, k, v, table, lens)
+    assert (got[rows - 2:] == 0).all()
