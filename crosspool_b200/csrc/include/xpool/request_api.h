@@ -55,8 +55,11 @@ typedef struct XpLoraArgs {
   const void* x;              /* bf16 [rows, ldx] */
   const void* y;              /* bf16 [rows, ld_y] */
   void* out;                  /* bf16 [rows, ld_out]; may be y */
-  const void* a;              /* bf16 [slots, parts, rank, k] */
-  const void* b;              /* bf16, n * rank elements per slot, of which [n, ranks[slot]] are used, without gaps */
+  /* bf16 [slots, parts, k / 32 rounded up, rank / 8, 8 ranks, 32 of k (zeros behind the last)] */
+  const void* a;
+  /* bf16, n * rank elements per slot, of which n * ranks[slot] are used, without gaps: blocks of up to 32 features of a part, in
+     each [ranks / 16][2][e: feature / 8][2][4 of 4 ranks][2][4 ranks], the twos being bit 2, bit 0 and bit 1 of the feature */
+  const void* b;
   const float* scale;         /* [slots] */
   const int* ranks;           /* [slots] rank in use, rounded up to 16; what lies behind it is zero */
   const int* part_ranks;      /* [slots, XP_LORA_PARTS] the parts' own ranks (0: none) */

@@ -6,10 +6,12 @@
 //   out = y + scale h B^T    the CTAs share the features, their warps blocks of 32
 //
 // Both products by mma.m16n8k16 with the rows as M. An adapter is read once for 16 rows or fewer: 32 flop a byte at most, far
-// below what the tensor pipe needs, so what counts is bytes in flight and the one exchange between the products. Fragments are
-// loaded from global memory straight to registers: the order of a sum's terms is free, so a lane's operand of two steps of k are 8
-// neighbouring elements (16 bytes) of a row of x or A, and the columns of four tiles of features are dealt so that a lane holds 8
-// neighbouring features of y and out. While the first product runs, B and y are brought to the L2.
+// below what the tensor pipe needs, so what counts is bytes in flight and the one exchange between the products. Every lane copies
+// its own fragments to shared memory and needs no barrier for them: the order of a sum's terms is free, so a lane's operand of two
+// steps of k are 8 neighbouring elements (16 bytes) of a row of x or A, and the columns of four tiles of features are dealt so that
+// a lane holds 8 neighbouring features of y and out. A and B lie in the order of the lanes, so that a copy of a warp is 512 bytes in
+// a row (eight rows of 64 bytes, or 32, before: 2000 rows of ranks 120 and 128 beside 4096 -> 4096 took 67 us, now 47). While the first
+// product runs, B and y are brought to the L2.
 //
 // h enters the second product as a bf16 pair (high and low part, 16 mantissa bits): its rounding to bf16 alone would be as large as
 // the result's. Sums are fp32.
@@ -31,7 +33,7 @@ constexpr int kItemRows = 16;
 constexpr int kMaxCluster = 8;
 constexpr int kPitch = 64 + 4;                       // fp32 row of a warp's partial sums
 
-// 16 or 8 bytes to shared memory; zeros when not ok
+// 16 bytes to shared memory; zeros when not ok
 __device__ __forceinline__ void copy16(uint32_t dst, const bf16* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
@@ -39,7 +41,6 @@ __device__ __forceinline__ void copy16(uint32_t dst, const bf16* src, bool ok) {
 __device__ __forceinline__ void copy16_kept(uint32_t dst, const bf16* src, bool ok) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copy8(uint32_t dst, const bf16* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
 __device__ __forceinline__ void issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // waits until at most `left` of the groups issued last are in flight
 __device__ __forceinline__ void landed(int left) {
@@ -51,11 +52,6 @@ __device__ __forceinline__ void landed(int left) {
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint2 lds8(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ void prefetch_l2(const void* p, uint32_t bytes) {      // whole 16 bytes
@@ -143,7 +139,7 @@ lora_kernel(XpLoraArgs a, int ranks) {
     const int kblocks = (a.k + 31) >> 5;
     const int k0 = static_cast<int>(static_cast<long long>(kblocks) * rank / ranks), k1 = static_cast<int>(static_cast<long long>(kblocks) * (rank + 1) / ranks);
     const bf16* x = reinterpret_cast<const bf16*>(a.x);
-    const bf16* aw = reinterpret_cast<const bf16*>(a.a) + static_cast<size_t>(slot) * a.parts * a.rank * a.k;
+    const bf16* aw = reinterpret_cast<const bf16*>(a.a) + static_cast<size_t>(slot) * a.parts * a.rank * kblocks * 32;
     auto prefetch_second = [&]() {                   // B and y of the second product, to the L2
       int p, f, end, f1;
       locate(b1 - 1, p, f1, end);
@@ -164,8 +160,8 @@ lora_kernel(XpLoraArgs a, int ranks) {
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
         acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
-        const int c = (t0 + min(t, tiles - 1)) * 8 + g;
-        wrow[t] = aw + (static_cast<size_t>(c / rk) * a.rank + c % rk) * a.k;
+        const int c = (t0 + min(t, tiles - 1)) * 8;
+        wrow[t] = aw + static_cast<size_t>(c / rk) * a.rank * kblocks * 32 + (c % rk >> 3) * 256 + lane * 8;
       }
       const uint32_t stage = (2 + tiles) * 512;
       const int depth = min(4, static_cast<int>(kRegion / stage));
@@ -180,7 +176,7 @@ lora_kernel(XpLoraArgs a, int ranks) {
           copy16_kept(ring + s * stage + 512, x1 + at, in && on1);
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
-            if (t < tiles) copy16(ring + s * stage + 1024 + t * 512, wrow[t] + at, in);
+            if (t < tiles) copy16(ring + s * stage + 1024 + t * 512, wrow[t] + static_cast<size_t>(kb) * a.rank * 32, true);
         }
         issued();
       };
@@ -228,9 +224,8 @@ lora_kernel(XpLoraArgs a, int ranks) {
     }
     sm100::cluster_sync();
     // ---- the first blocks of the second product are on their way
-    const uint32_t stage = 1024 + rk * 64;             // y, and 8 bytes per tile and block of ranks
+    const uint32_t stage = 1024 + rk * 64;             // y, and 16 bytes per two tiles and block of ranks
     const int depth = min(4, static_cast<int>(kRegion / stage));
-    const uint32_t ring8 = ring - lane * 8;
     auto issue = [&](int b, int s) {
       if (b < b1) {
         int p, f, end;
@@ -240,13 +235,11 @@ lora_kernel(XpLoraArgs a, int ranks) {
         copy16(ring + s * stage, y + static_cast<size_t>(r0) * a.ld_y + (in ? fl : f), in && on0);
         copy16(ring + s * stage + 512, y + static_cast<size_t>(r1) * a.ld_y + (in ? fl : f), in && on1);
         // column g of tile t is feature (g / 2) * 8 + 2 t + g % 2 of the block
-        const bool ing = f + (g >> 1) * 8 < end;
-        const bf16* brow = bw + static_cast<size_t>(ing ? f + (g >> 1) * 8 + (g & 1) : f) * rk + q * 4;
-#pragma unroll 2
-        for (int kb = 0; kb < rk >> 4; ++kb) {
-#pragma unroll
-          for (int t = 0; t < 4; ++t) copy8(ring8 + s * stage + 1024 + (kb * 4 + t) * 256, brow + t * 2 * rk + kb * 16);
-        }
+        const int eights = min(4, (end - f) >> 3);
+        const bool ing = g >> 1 < eights;
+        const bf16* brow = bw + static_cast<size_t>(f) * rk + (ing ? lane * 8 : 0);
+#pragma unroll 4
+        for (int i = 0; i < rk >> 3; ++i) copy16(ring + s * stage + 1024 + i * 512, brow + i * eights * 64, ing);
       }
       issued();
     };
@@ -296,7 +289,7 @@ lora_kernel(XpLoraArgs a, int ranks) {
       const int fl = f + q * 8;
       const bool in = fl < end;
       landed(depth - 1);
-      const uint32_t at = ring + s * stage, at8 = ring8 + s * stage + 1024;
+      const uint32_t at = ring + s * stage;
       const uint4 y0 = lds16(at), y1 = lds16(at + 512);
       float acc[4][4];
 #pragma unroll
@@ -307,10 +300,12 @@ lora_kernel(XpLoraArgs a, int ranks) {
         const uint4 hv = h[kb * 64], lv = h[kb * 64 + 1];
         const uint32_t hi[4] = {hv.x, hv.y, hv.z, hv.w}, lo[4] = {lv.x, lv.y, lv.z, lv.w};
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint2 w = lds8(at8 + (kb * 4 + t) * 256);
+        for (int t = 0; t < 4; t += 2) {
+          const uint4 w = lds16(at + 1024 + (kb * 2 + (t >> 1)) * 512);
           frag::mma(acc[t], hi, w.x, w.y);
           frag::mma(acc[t], lo, w.x, w.y);
+          frag::mma(acc[t + 1], hi, w.z, w.w);
+          frag::mma(acc[t + 1], lo, w.z, w.w);
         }
       }
       issue(b + depth * kWarps, s);

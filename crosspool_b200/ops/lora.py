@@ -21,10 +21,11 @@ ITEM_ROWS = 16        # rows of one adapter that a cluster of CTAs takes at once
 
 
 class AdapterStack:
-    """The adapters of one projection, slot by slot in bf16: ``a`` ``[slots, parts, rank, in]``, ``b`` with room for ``[out, rank]``
-    in each slot, a scale and a rank per slot. ``out_features``: a number, or one per part of a fused projection (q, k and v: each
-    part has an ``A`` of its own). A slot's rank is its adapter's, padded with zeros to a multiple of 16 (``rank`` at most); its
-    ``B`` lies without gaps, ``[out, slot's rank]``, so that low ranks cost no more bytes than they have."""
+    """The adapters of one projection, slot by slot in bf16, in the order in which the kernel's lanes read them
+    (``XpLoraArgs``): ``a`` with room for ``[rank, in]`` of every part (``in`` padded to a multiple of 32), ``b`` for ``[out, rank]``, a
+    scale and a rank per slot. ``out_features``: a number, or one per part of a fused projection (q, k and v: each part has an ``A``
+    of its own). A slot's rank is its adapter's, padded with zeros to a multiple of 16 (``rank`` at most); its ``B`` lies without
+    gaps, so that low ranks cost no more bytes than they have."""
 
     def __init__(self, slots: int, in_features: int, out_features: int | Sequence[int], max_rank: int, device: str | torch.device = "cuda"):
         self.parts = (int(out_features),) if isinstance(out_features, int) else tuple(int(n) for n in out_features)
@@ -34,7 +35,7 @@ class AdapterStack:
             raise ValueError(f"features {in_features} -> {self.parts}: multiples of 8 are supported")
         self.slots, self.in_features, self.out_features = slots, in_features, sum(self.parts)
         self.rank = (max_rank + 15) // 16 * 16
-        self.a = torch.zeros(slots, len(self.parts), self.rank, in_features, dtype=torch.bfloat16, device=device)
+        self.a = torch.zeros(slots, len(self.parts), self.rank, (in_features + 31) // 32 * 32, dtype=torch.bfloat16, device=device)
         self.b = torch.zeros(slots, self.out_features * self.rank, dtype=torch.bfloat16, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
         self.ranks = torch.zeros(slots, dtype=torch.int32, device=device)
@@ -77,11 +78,18 @@ class AdapterStack:
             self.b[slot].zero_()
         self._fresh[slot] = False
         r16, at = (used + 15) // 16 * 16, 0
-        b16 = self.b[slot, :self.out_features * r16].view(self.out_features, r16)
         for i, (n, x, y) in enumerate(zip(self.parts, pa, pb)):
             if x is not None:
-                self.a[slot, i, :x.shape[0]].copy_(x)
-                b16[at:at + n, :x.shape[0]].copy_(y)
+                wide = torch.zeros(self.rank, self.a.shape[3], dtype=torch.bfloat16, device=self.device)
+                wide[:x.shape[0], :self.in_features].copy_(x)
+                self.a[slot, i].view(-1, self.rank, 32).copy_(wide.view(self.rank, -1, 32).transpose(0, 1))
+                wide = torch.zeros(n, r16, dtype=torch.bfloat16, device=self.device)
+                wide[:, :x.shape[0]].copy_(y)
+                for f0, f1 in ((0, n // 32 * 32), (n // 32 * 32, n)):          # whole blocks, and a last one of fewer features
+                    if f0 < f1:
+                        e = min(f1 - f0, 32) // 8
+                        block = wide[f0:f1].view(-1, e, 2, 2, 2, r16 // 16, 4, 4).permute(0, 5, 2, 1, 4, 6, 3, 7)
+                        self.b[slot, (at + f0) * r16:(at + f1) * r16].view(block.shape).copy_(block)
             at += n
         self.scale[slot:slot + 1].fill_(float(scale))
         self.ranks[slot:slot + 1].fill_(r16)
