@@ -10,13 +10,14 @@
 // its own fragments to shared memory and needs no barrier for them: the order of a sum's terms is free, so a lane's operand of two
 // steps of k are 8 neighbouring elements (16 bytes) of a row of x or A, and the columns of four tiles of features are dealt so that
 // a lane holds 8 neighbouring features of y and out. A and B lie in the order of the lanes, so that a copy of a warp is 512 bytes in
-// a row (eight rows of 64 bytes, or 32, before: 2000 rows of ranks 120 and 128 beside 4096 -> 4096 took 67 us, now 47). While the first
+// a row (eight rows of 64 bytes, or 32, before: 2000 rows of ranks 120 and 128 beside 4096 -> 4096 took 67 us, then 47). While the first
 // product runs, B and y are brought to the L2.
 //
 // h enters the second product as a bf16 pair (high and low part, 16 mantissa bits): its rounding to bf16 alone would be as large as
 // the result's. Sums are fp32.
 #include <cooperative_groups.h>
 
+#include <type_traits>
 #include <utility>
 
 #include "xpool/mma_sync.cuh"
@@ -154,60 +155,77 @@ lora_kernel(XpLoraArgs a, int ranks) {
     const int all = a.parts * rk, n_tiles = all >> 3;   // columns of h, part after part
     const int groups = n_tiles <= kTiles ? 1 : n_tiles <= 2 * kTiles ? 2 : n_tiles <= 4 * kTiles ? 4 : 8, each = kWarps / groups;
     const int per = (n_tiles + groups - 1) / groups, t0 = warp / each * per, tiles = max(0, min(per, n_tiles - t0));
-    if (tiles > 0) {
-      float acc[kTiles][4];
-      const bf16* wrow[kTiles];
+    // (the steps are bound by their instructions: NT > 0 is a known number of tiles, which may lie side by side in one part)
+    auto first_product = [&](auto known, auto side_by_side) {
+      constexpr int NT = decltype(known)::value, kMost = NT > 0 ? NT : kTiles;
+      constexpr bool kBeside = decltype(side_by_side)::value;
+      float acc[kMost][4];
+      const bf16* wrow[kBeside ? 1 : kMost];
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+      for (int t = 0; t < kMost; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+#pragma unroll
+      for (int t = 0; t < (kBeside ? 1 : kMost); ++t) {
         const int c = (t0 + min(t, tiles - 1)) * 8;
         wrow[t] = aw + static_cast<size_t>(c / rk) * a.rank * kblocks * 32 + (c % rk >> 3) * 256 + lane * 8;
       }
-      const uint32_t stage = (2 + tiles) * 512;
+      const uint32_t stage = (2 + (NT > 0 ? NT : tiles)) * 512;
       const int depth = min(4, static_cast<int>(kRegion / stage));
-      const bf16* x0 = x + static_cast<size_t>(r0) * a.ldx;
-      const bf16* x1 = x + static_cast<size_t>(r1) * a.ldx;
-      auto issue = [&](int kb, int s) {
-        const int k = kb * 32 + q * 8;
-        const bool in = kb < k1 && k < a.k;
-        const int at = in ? k : 0;
+      const bf16* x0 = x + static_cast<size_t>(r0) * a.ldx + q * 8;
+      const bf16* x1 = x + static_cast<size_t>(r1) * a.ldx + q * 8;
+      const int k_left = a.k - q * 8;                // blocks that begin before it have elements of this lane
+      auto issue = [&](int kb, uint32_t to) {
         if (kb < k1) {
-          copy16_kept(ring + s * stage, x0 + at, in && on0);
-          copy16_kept(ring + s * stage + 512, x1 + at, in && on1);
+          const bool in = kb * 32 < k_left;
+          const int at = in ? kb * 32 : 0;
+          const size_t w_at = static_cast<size_t>(kb) * (a.rank * 32);
+          copy16_kept(to, x0 + (in ? at : -q * 8), in && on0);
+          copy16_kept(to + 512, x1 + (in ? at : -q * 8), in && on1);
+          if constexpr (kBeside) {
+            const bf16* from = wrow[0] + w_at;
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t)
-            if (t < tiles) copy16(ring + s * stage + 1024 + t * 512, wrow[t] + static_cast<size_t>(kb) * a.rank * 32, true);
+            for (int t = 0; t < NT; ++t) copy16(to + 1024 + t * 512, from + t * 256, true);
+          } else {
+#pragma unroll
+            for (int t = 0; t < kMost; ++t)
+              if (NT > 0 || t < tiles) copy16(to + 1024 + t * 512, wrow[t] + w_at, true);
+          }
         }
         issued();
       };
       const int kb0 = k0 + warp % each;
-      for (int i = 0; i < depth; ++i) issue(kb0 + i * each, i);
+      for (int i = 0; i < depth; ++i) issue(kb0 + i * each, ring + i * stage);
       if (warp == 0 && b1 > b0) prefetch_second();
-      int s = 0;
+      uint32_t at = ring;
       for (int kb = kb0; kb < k1; kb += each) {
         landed(depth - 1);
-        const uint32_t at = ring + s * stage;
         const uint4 u = lds16(at), v = lds16(at + 512);
         const uint32_t lo[4] = {u.x, v.x, u.y, v.y}, hi[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-          if (t < tiles) {
+        for (int t = 0; t < kMost; ++t)
+          if (NT > 0 || t < tiles) {
             const uint4 w = lds16(at + 1024 + t * 512);
             frag::mma(acc[t], lo, w.x, w.y);
             frag::mma(acc[t], hi, w.z, w.w);
           }
-        issue(kb + depth * each, s);
-        s = s + 1 == depth ? 0 : s + 1;
+        issue(kb + depth * each, at);
+        at = at + stage == ring + depth * stage ? ring : at + stage;
       }
       landed(0);
       __syncwarp();                                  // the partial sums lie over all lanes' copies
       float* mine = reinterpret_cast<float*>(smem + warp * kRegion) + g * kPitch + q * 2;
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-        if (t < tiles) {
+      for (int t = 0; t < kMost; ++t)
+        if (NT > 0 || t < tiles) {
           *reinterpret_cast<float2*>(mine + t * 8) = make_float2(acc[t][0], acc[t][1]);
           *reinterpret_cast<float2*>(mine + 8 * kPitch + t * 8) = make_float2(acc[t][2], acc[t][3]);
         }
+    };
+    if (tiles > 0) {
+      const bool beside = t0 * 8 / rk == (t0 + tiles - 1) * 8 / rk;
+      if (tiles == (kTiles == 4 ? 3 : 6)) first_product(std::integral_constant<int, kTiles == 4 ? 3 : 6>(), std::false_type());
+      else if (beside && tiles == 4) first_product(std::integral_constant<int, 4>(), std::true_type());
+      else if (beside && tiles == 2) first_product(std::integral_constant<int, 2>(), std::true_type());
+      else first_product(std::integral_constant<int, 0>(), std::false_type());
     }
     __syncthreads();
     if (!met) {
@@ -238,8 +256,12 @@ lora_kernel(XpLoraArgs a, int ranks) {
         const int eights = min(4, (end - f) >> 3);
         const bool ing = g >> 1 < eights;
         const bf16* brow = bw + static_cast<size_t>(f) * rk + (ing ? lane * 8 : 0);
+        if (eights == 4) {
 #pragma unroll 4
-        for (int i = 0; i < rk >> 3; ++i) copy16(ring + s * stage + 1024 + i * 512, brow + i * eights * 64, ing);
+          for (int i = 0; i < rk >> 3; ++i) copy16(ring + s * stage + 1024 + i * 512, brow + i * 256, true);
+        } else {
+          for (int i = 0; i < rk >> 3; ++i) copy16(ring + s * stage + 1024 + i * 512, brow + i * eights * 64, ing);
+        }
       }
       issued();
     };
@@ -357,10 +379,12 @@ extern "C" int xp_lora(const XpLoraArgs* a, void* stream) {
   if (a->part_end[a->parts - 1] != a->n) return -11;
   auto odd = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
   if (odd(a->x) || odd(a->y) || odd(a->out) || odd(a->a) || odd(a->b) || (a->rows > 1 && (a->ldx % 8 != 0 || a->ld_y % 8 != 0 || a->ld_out % 8 != 0))) return -12;
-  // Clusters as large as the SMs hold beside one another (two CTAs to an SM). us with 1 / 2 / 4 / 8 CTAs an item: 4 items of rank 16
-  // beside 1024 -> 4096 17 / 12 / 9 / 7; 39 items of ranks 8 to 64 beside 4096 -> 6144 77 / 44 / 36 / 31; 126 items of ranks 16 and 32
-  // beside 4096 -> 4096 27 / 23 / 26 / 33, of rank 128 73 / 67 / 61 / 71.
-  int ranks = a->max_items <= 48 ? 8 : a->max_items <= 80 ? 4 : a->max_items <= 296 ? 2 : 1;
+  // Clusters as large as the SMs hold beside one another: two CTAs to an SM, one where h has more than 256 columns. us with 1 / 2 / 4 /
+  // 8 CTAs an item: 4 items of rank 16 beside 1024 -> 4096 16 / 12 / 9 / 8; 39 items of ranks 8 to 64 beside 4096 -> 6144
+  // 58 / 35 / 26 / 22; 126 items beside 4096 -> 4096 of ranks 16 and 32 28 / 20 / 23 / 35, of rank 128 55 / 45 / 52 / 58, and in three
+  // parts of rank 128 97 / 107 / 105 / 148.
+  const int crowd = a->parts * a->rank <= 256 ? a->max_items : 2 * a->max_items;
+  int ranks = crowd <= 48 ? 8 : crowd <= 80 ? 4 : crowd <= 148 ? 2 : 1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return a->parts * a->rank <= 256 ? launch<4>(*a, ranks, s) : launch<8>(*a, ranks, s);
 }
