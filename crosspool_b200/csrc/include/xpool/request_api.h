@@ -55,6 +55,11 @@ typedef struct XpLoraArgs {
   const void* x;              /* bf16 [rows, ldx] */
   const void* y;              /* bf16 [rows, ld_y] */
   void* out;                  /* bf16 [rows, ld_out]; may be y */
+  int rows, ldx, ld_y, ld_out;
+  const XpLoraItem* items;
+  const int* n_items;         /* device word */
+  const int* perm;            /* [rows] */
+  int max_items, reserved;
   /* bf16 [slots, parts, k / 32 rounded up, rank / 8, 8 ranks, 32 of k (zeros behind the last)] */
   const void* a;
   /* bf16, n * rank elements per slot, of which n * ranks[slot] are used, without gaps: blocks of up to 32 features of a part, in
@@ -63,11 +68,7 @@ typedef struct XpLoraArgs {
   const float* scale;         /* [slots] */
   const int* ranks;           /* [slots] rank in use, rounded up to 16; what lies behind it is zero */
   const int* part_ranks;      /* [slots, XP_LORA_PARTS] the parts' own ranks (0: none) */
-  const XpLoraItem* items;
-  const int* n_items;         /* device word */
-  const int* perm;            /* [rows] */
-  int rows, k, n, rank, parts, slots, max_items;
-  int ldx, ld_y, ld_out;
+  int k, n, rank, parts, slots;
   int part_end[XP_LORA_PARTS]; /* features [0, part_end[0]) are part 0, and so on; multiples of 8 */
 } XpLoraArgs;
 int xp_lora(const XpLoraArgs* a, void* stream);

@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import math
+import struct
 from typing import Sequence
 
 import numpy as np
@@ -122,6 +123,7 @@ PREFIX_TOKENS = 16      # prefixes are shared in whole tiles of so many tokens; 
 PIECE_TOKENS = 128      # pieces of a prefix begin at multiples of this
 MAX_PARTS = 32          # pieces of one prefix
 MAX_SHARED_ROWS = 4096  # rows of a batch
+_SHARED_CALL = struct.Struct("7Q7if2iQ2i")   # XpDecodeAttnArgs, which begins XpDecodeSharedArgs
 
 
 def own_slots(rows: int, q_heads: int, kv_heads: int) -> int:
@@ -224,9 +226,7 @@ class SharedPrefixPlan:
         s.max_pieces, s.max_parts, s.plan_rows = max_pieces, max_parts, rows
         s.max_len = self.max_len = max_len
         s.own_slots = self.own = own_slots(rows, q_heads, kv_heads)
-        s.a.q_heads, s.a.kv_heads, s.a.head_dim = q_heads, kv_heads, head_dim
-        s.a.num_splits, s.a.chunk_tokens = self.slices
-        self._fields = bytes(s)
+        self._fields = bytes(s)[native.DecodeSharedArgs.pieces.offset:]
 
     def workspace_floats(self, batch: int) -> int:
         """Elements of the fp32 workspace of a call over ``batch`` rows."""
@@ -314,19 +314,12 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise ValueError("the kernel runs on a GPU")
     if not k_cache.shape[0]:
         raise ValueError("a cache of no pages")
-    s = native.DecodeSharedArgs.from_buffer_copy(plan._fields)
-    a = s.a
-    a.q, a.k_cache, a.v_cache, a.out = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr()
-    a.ws = ws.data_ptr() if ws is not None else None
-    a.block_table, a.seq_lens = block_table.data_ptr(), seq_lens.data_ptr()
-    a.batch, a.page_size, a.max_blocks, a.num_pages = batch, page, block_table.stride(0), k_cache.shape[0]
-    a.scale = scale
     from .gemm import status_words
 
-    a.status = status_words(dev).data_ptr()
-    with native.on_device(dev):
-        native.check(native.kernels().xp_decode_shared(C.byref(s), native.stream_of(dev)), "xp_decode_shared",
-                     1 + (plan.max_pieces > 0 or plan.slices[0] > 1))
+    call = _SHARED_CALL.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), ws.data_ptr() if ws is not None else 0,
+                             block_table.data_ptr(), seq_lens.data_ptr(), batch, q_heads, kv_heads, d, page, block_table.stride(0), plan.slices[0], scale,
+                             plan.slices[1], k_cache.shape[0], status_words(dev).data_ptr(), 0, 0)
+    native.run_packed("xp_decode_shared", call + plan._fields, dev, 1 + (plan.max_pieces > 0 or plan.slices[0] > 1))
     return out
 
 

@@ -7,7 +7,7 @@ or by temperature (the draw of :func:`crosspool_b200.ops.attention.sample`).
 
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -16,6 +16,7 @@ from .. import native
 
 _INT, _FLOAT = torch.int32, torch.float32
 MAX_VOCAB = 1 << 20
+_CALL = struct.Struct("6Q6i")      # what XpLogitArgs holds behind the controls
 
 
 @dataclass(frozen=True)
@@ -85,7 +86,7 @@ class LogitControls:
                 raise ValueError(f"{self.history.shape[0]} histories for {max(rows)} rows")
         if self.masks is not None:
             s.mask_count, s.ld_mask = self.masks.shape[0], self.masks.stride(0)
-        object.__setattr__(self, "_fields", bytes(s))
+        object.__setattr__(self, "_fields", bytes(s)[:native.LogitArgs.logits.offset])
         object.__setattr__(self, "_rows", rows.pop() if rows else None)
         object.__setattr__(self, "_device", devices.pop() if devices else None)
 
@@ -95,7 +96,8 @@ class LogitControls:
         return self._rows
 
 
-def _args(logits: torch.Tensor, c: LogitControls) -> "native.LogitArgs":
+def _check(logits: torch.Tensor, c: LogitControls) -> tuple[int, int, int, int]:
+    """Refuses what the kernel does not take; (rows, vocab, pitch, whether fp32)."""
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
         raise ValueError("logits must be bf16 or fp32 [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
@@ -110,34 +112,32 @@ def _args(logits: torch.Tensor, c: LogitControls) -> "native.LogitArgs":
         raise ValueError(f"controls on {c._device} for logits on {logits.device}")
     if c.masks is not None and c.masks.shape[0] and c.masks.shape[1] * 32 < vocab:
         raise ValueError(f"masks of {c.masks.shape[1]} words for {vocab} tokens")
-    s = native.LogitArgs.from_buffer_copy(c._fields)
-    s.logits, s.rows, s.vocab, s.ld, s.f32 = logits.data_ptr(), rows, vocab, ld, int(logits.dtype == _FLOAT)
-    return s
+    return rows, vocab, ld, logits.dtype is _FLOAT
 
 
-def _launch(s, dev) -> None:
+def _launch(controls: LogitControls, call: bytes, dev) -> None:
     if dev.type != "cuda":
         raise ValueError("the kernel runs on a GPU")
-    with native.on_device(dev):
-        native.check(native.kernels().xp_logit_controls(C.byref(s), native.stream_of(dev)), "xp_logit_controls")
+    native.run_packed("xp_logit_controls", controls._fields + call, dev)
 
 
 def adjust_logits(logits: torch.Tensor, controls: LogitControls, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """The logits after ``controls``, rounded once to ``out``'s type (bf16 or fp32; by default the logits' own). ``out`` may be
     ``logits`` itself."""
-    s = _args(logits, controls)
+    rows, vocab, ld, f32 = _check(logits, controls)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits)
     if out.shape != logits.shape or out.dtype not in (torch.bfloat16, _FLOAT) or out.stride(1) != 1 or out.device != logits.device:
         raise ValueError("out must be bf16 or fp32 of the logits' shape, with contiguous rows, on their device")
-    ld_out = out.stride(0) if out.shape[0] > 1 else out.shape[1]
-    if not out.shape[1] <= ld_out < 2 ** 31:
-        raise ValueError(f"rows of {out.shape[1]} results {ld_out} elements apart")
-    if out.data_ptr() == logits.data_ptr() and out.numel() and (out.dtype != logits.dtype or ld_out != s.ld):
+    ld_out = out.stride(0) if rows > 1 else vocab
+    if not vocab <= ld_out < 2 ** 31:
+        raise ValueError(f"rows of {vocab} results {ld_out} elements apart")
+    if not rows or not vocab:
+        return out
+    at, to = logits.data_ptr(), out.data_ptr()
+    if at == to and (out.dtype is not logits.dtype or ld_out != ld):
         raise ValueError("adjusting in place keeps type and pitch")
-    s.out, s.ld_out, s.out_f32 = out.data_ptr(), ld_out, int(out.dtype == _FLOAT)
-    if out.numel():
-        _launch(s, logits.device)
+    _launch(controls, _CALL.pack(at, to, 0, 0, 0, 0, rows, vocab, ld, ld_out, f32, out.dtype is _FLOAT), logits.device)
     return out
 
 
@@ -147,9 +147,9 @@ def select_tokens(logits: torch.Tensor, controls: LogitControls, temps: torch.Te
     draw from ``softmax(adjusted / temperature)`` with ``seeds`` int32 ``[rows, 2]`` as in
     :func:`crosspool_b200.ops.attention.sample`. ``values`` (fp32 ``[rows]``) receives the adjusted logit of the token. A row without
     an allowed token gives token 0 and the value ``-inf``; NaN is never the largest."""
-    s = _args(logits, controls)
-    rows, dev = logits.shape[0], logits.device
-    if logits.shape[1] == 0:
+    rows, vocab, ld, f32 = _check(logits, controls)
+    dev = logits.device
+    if vocab == 0:
         raise ValueError("logits of no tokens")
     if out is None:
         out = torch.empty(rows, dtype=_INT, device=dev)
@@ -159,11 +159,7 @@ def select_tokens(logits: torch.Tensor, controls: LogitControls, temps: torch.Te
             raise ValueError(f"{name} must be contiguous {dtype} {shape} on the logits' device")
     if (temps is None) != (seeds is None):
         raise ValueError("temps and seeds come together")
-    s.tokens = out.data_ptr()
-    if values is not None:
-        s.values = values.data_ptr()
-    if temps is not None:
-        s.temps, s.seeds = temps.data_ptr(), seeds.data_ptr()
     if rows:
-        _launch(s, dev)
+        at = [0 if t is None else t.data_ptr() for t in (temps, seeds, out, values)]
+        _launch(controls, _CALL.pack(logits.data_ptr(), 0, *at, rows, vocab, ld, 0, f32, 0), dev)
     return out

@@ -8,6 +8,7 @@ is an :class:`AdapterPlan`, made once per batch and used by all layers and proje
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Sequence
 
 import numpy as np
@@ -17,6 +18,7 @@ from .. import native
 
 MAX_RANK = 128
 MAX_PARTS = 4
+_CALL, _PLAN = struct.Struct("3Q4i"), struct.Struct("3Q2i")      # XpLoraArgs: of a call, then of its plan, then of its stack
 ITEM_ROWS = 16        # rows of one adapter that a cluster of CTAs takes at once; a plan's items hold at most so many
 
 
@@ -52,7 +54,7 @@ class AdapterStack:
         s.part_ranks = self.part_ranks.data_ptr()
         s.k, s.n, s.rank, s.parts, s.slots = in_features, self.out_features, self.rank, len(self.parts), slots
         s.part_end = (C.c_int * 4)(*(ends + [end] * (4 - len(ends))))
-        self._fields = bytes(s)
+        self._fields = bytes(s)[native.LoraArgs.a.offset:]
 
     @torch.no_grad()
     def load(self, slot: int, a: torch.Tensor | Sequence[torch.Tensor], b: torch.Tensor | Sequence[torch.Tensor], scale: float = 1.0) -> None:
@@ -146,7 +148,7 @@ class AdapterPlan:
     def __init__(self, words: torch.Tensor, rows: int, max_items: int, slots: int):
         self.words, self.rows, self.max_items, self.slots = words, rows, max_items, slots
         base = words.data_ptr()
-        self._items, self._n_items, self._perm = base + 16, base, base + 16 + 16 * rows
+        self._fields = _PLAN.pack(base + 16, base, base + 16 + 16 * rows, max_items, 0)
 
 
 def adapter_plan(index: Sequence[int], stack: "AdapterStack | int", device: str | torch.device | None = None) -> AdapterPlan:
@@ -168,30 +170,28 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: Adapte
     be ``y`` itself. bf16; rows may have a pitch (a multiple of 8 elements), so that a slice of a wider buffer can be read or written."""
     rows = x.shape[0]
     if out is None:
-        out = torch.empty(rows, stack.out_features, dtype=torch.bfloat16, device=x.device)
-    if x.dim() != 2 or x.shape[1] != stack.in_features or y.shape != (rows, stack.out_features) or out.shape != y.shape:
+        out = torch.empty_like(y)
+    if x.shape != (rows, stack.in_features) or y.shape != (rows, stack.out_features) or out.shape != y.shape:
         raise ValueError(f"x {tuple(x.shape)}, y {tuple(y.shape)}, out {tuple(out.shape)} beside a {stack.in_features} -> {stack.out_features} stack")
     if rows != plan.rows or plan.slots > stack.slots:
         raise ValueError(f"a plan of {plan.rows} rows and {plan.slots} slots for {rows} rows and {stack.slots} slots")
-    dev = stack.device
+    dev, bf16 = stack.device, torch.bfloat16
     for t in (x, y, out):
-        if t.dtype != torch.bfloat16 or t.device != dev:
+        if t.dtype is not bf16 or t.device != dev:
             raise ValueError(f"{t.dtype} on {t.device}: bf16 on the stack's device ({dev}) is supported")
-        if t.stride(1) != 1 or (rows > 1 and (t.stride(0) % 8 or t.stride(0) >= 2 ** 31)) or t.data_ptr() % 16:
-            raise ValueError("rows must be contiguous, 16-byte aligned, with pitches of whole 16 bytes")
-    if rows > 1 and (out.stride(0) < stack.out_features or (out.data_ptr() == y.data_ptr() and out.stride(0) != y.stride(0))):
+    at_x, at_y, at_out = x.data_ptr(), y.data_ptr(), out.data_ptr()
+    (ld_x, one_x), (ld_y, one_y), (ld_out, one_out) = x.stride(), y.stride(), out.stride()
+    if not one_x == one_y == one_out == 1 or (at_x | at_y | at_out) & 15 or (rows > 1 and ((ld_x | ld_y | ld_out) & 7 or max(ld_x, ld_y, ld_out) >> 31)):
+        raise ValueError("rows must be contiguous, 16-byte aligned, with pitches of whole 16 bytes")
+    if rows > 1 and (ld_out < stack.out_features or (at_out == at_y and ld_out != ld_y)):
         raise ValueError("the rows of out must not overlap one another or other rows of y")
     if plan.words.device != dev:
         raise ValueError("the plan lives on another device")
-    if rows and out.data_ptr() == x.data_ptr():
+    if rows and at_out == at_x:
         raise ValueError("out may be y, but not x")
     if dev.type != "cuda":
         raise ValueError("the kernel runs on a GPU")
-    s = native.LoraArgs.from_buffer_copy(stack._fields)
-    s.x, s.y, s.out = x.data_ptr(), y.data_ptr(), out.data_ptr()
-    s.items, s.n_items, s.perm = plan._items, plan._n_items, plan._perm
-    s.rows, s.max_items = rows, plan.max_items
-    s.ldx, s.ld_y, s.ld_out = x.stride(0), y.stride(0), out.stride(0)
-    with native.on_device(dev):
-        native.check(native.kernels().xp_lora(C.byref(s), native.stream_of(dev)), "xp_lora")
+    if rows <= 1:
+        ld_x = ld_y = ld_out = 0
+    native.run_packed("xp_lora", _CALL.pack(at_x, at_y, at_out, rows, ld_x, ld_y, ld_out) + plan._fields + stack._fields, dev)
     return out
