@@ -16,6 +16,7 @@ import numpy as np
 import torch
 
 from .. import native
+from .gemm import status_words
 
 
 def _stream(dev) -> int:
@@ -273,29 +274,30 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     of its group (``csrc/kernels/shared_prefix.cu``), then each row adds its own tokens. ``seq_lens`` count prefix and own tokens; a
     row of fewer tokens than its group's prefix reads all of them on its own. Rows without tokens give zeros."""
     batch, q_heads, d = q.shape
-    page, kv_heads = k_cache.shape[1], k_cache.shape[2]
-    if (q_heads, kv_heads, d) != (plan.q_heads, plan.kv_heads, plan.head_dim) or k_cache.shape != v_cache.shape or k_cache.shape[3] != d:
+    pages, page, kv_heads, kv_d = kv_shape = k_cache.shape
+    if (q_heads, kv_heads, d, d) != (plan.q_heads, plan.kv_heads, plan.head_dim, kv_d) or v_cache.shape != kv_shape:
         raise ValueError(f"q {tuple(q.shape)}, caches {tuple(k_cache.shape)} and {tuple(v_cache.shape)} for a plan of {plan.q_heads} query and "
                          f"{plan.kv_heads} KV heads of {plan.head_dim}")
     if page < 16 or page & (page - 1):
         raise ValueError(f"pages of {page} tokens: powers of two from 16 on are supported")
-    dev = q.device
-    for t in (q, k_cache, v_cache):
-        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.data_ptr() % 16 or t.device != dev:
-            raise ValueError("queries and caches must be contiguous, 16-byte aligned bf16 on one device")
-    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32 or block_table.device != dev or seq_lens.device != dev:
+    dev, bf16, i32 = q.device, torch.bfloat16, torch.int32
+    at_q, at_k, at_v = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    if (at_q | at_k | at_v) & 15 or not (q.dtype is k_cache.dtype is v_cache.dtype is bf16 and q.is_contiguous() and k_cache.is_contiguous()
+                                         and v_cache.is_contiguous() and k_cache.device == dev and v_cache.device == dev):
+        raise ValueError("queries and caches must be contiguous, 16-byte aligned bf16 on one device")
+    if not (block_table.dtype is seq_lens.dtype is i32 and block_table.device == dev and seq_lens.device == dev):
         raise ValueError("block_table and seq_lens must be int32 on the queries' device")
-    if block_table.dim() != 2 or block_table.shape[0] < batch or seq_lens.shape != (batch,) or not seq_lens.is_contiguous() \
-            or (block_table.shape[1] and block_table.stride(1) != 1):
+    if block_table.dim() != 2 or seq_lens.shape != (batch,) or not seq_lens.is_contiguous():
         raise ValueError(f"block_table {tuple(block_table.shape)} and seq_lens {tuple(seq_lens.shape)} for {batch} rows")
-    if plan.rows > batch or plan.words.device != dev or block_table.shape[1] * page < plan.max_len:
-        raise ValueError(f"a plan of {plan.rows} rows of up to {plan.max_len} tokens for {batch} rows of {block_table.shape[1]} pages")
+    (rows, width), (pitch, one) = block_table.shape, block_table.stride()
+    if rows < batch or (width and one != 1):
+        raise ValueError(f"block_table {tuple(block_table.shape)} and seq_lens {tuple(seq_lens.shape)} for {batch} rows")
+    if plan.rows > batch or plan.words.device != dev or width * page < plan.max_len:
+        raise ValueError(f"a plan of {plan.rows} rows of up to {plan.max_len} tokens for {batch} rows of {width} pages")
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
+    elif out.shape != q.shape or out.dtype is not bf16 or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be like q")
-    if out.data_ptr() % 16 or (ws is not None and ws.data_ptr() % 16):
-        raise ValueError("out and the workspace must be 16-byte aligned")
     if scale is None:
         scale = d ** -0.5
     elif not 0 < scale < math.inf:
@@ -308,17 +310,17 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
             ws = torch.empty(need, dtype=torch.float32, device=dev)
     elif ws.dtype != torch.float32 or ws.numel() < need or not ws.is_contiguous() or ws.device != dev:
         raise ValueError(f"the workspace must hold {need} contiguous fp32 elements on the queries' device")
+    at_out, at_ws = out.data_ptr(), ws.data_ptr() if ws is not None else 0
+    if (at_out | at_ws) & 15:
+        raise ValueError("out and the workspace must be 16-byte aligned")
     if not batch:
         return out
     if dev.type != "cuda":
         raise ValueError("the kernel runs on a GPU")
-    if not k_cache.shape[0]:
+    if not pages:
         raise ValueError("a cache of no pages")
-    from .gemm import status_words
-
-    call = _SHARED_CALL.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), ws.data_ptr() if ws is not None else 0,
-                             block_table.data_ptr(), seq_lens.data_ptr(), batch, q_heads, kv_heads, d, page, block_table.stride(0), plan.slices[0], scale,
-                             plan.slices[1], k_cache.shape[0], status_words(dev).data_ptr(), 0, 0)
+    call = _SHARED_CALL.pack(at_q, at_k, at_v, at_out, at_ws, block_table.data_ptr(), seq_lens.data_ptr(), batch, q_heads, kv_heads, d, page, pitch,
+                             plan.slices[0], scale, plan.slices[1], pages, status_words(dev).data_ptr(), 0, 0)
     native.run_packed("xp_decode_shared", call + plan._fields, dev, 1 + (plan.max_pieces > 0 or plan.slices[0] > 1))
     return out
 
