@@ -98,7 +98,8 @@ class LogitControls:
 
 def _check(logits: torch.Tensor, c: LogitControls) -> tuple[int, int, int, int]:
     """Refuses what the kernel does not take; (rows, vocab, pitch, whether fp32)."""
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.stride(1) != 1:
+    f32 = logits.dtype is _FLOAT
+    if logits.dim() != 2 or not (f32 or logits.dtype is torch.bfloat16) or logits.stride(1) != 1:
         raise ValueError("logits must be bf16 or fp32 [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
     ld = logits.stride(0) if rows > 1 else vocab
@@ -112,7 +113,12 @@ def _check(logits: torch.Tensor, c: LogitControls) -> tuple[int, int, int, int]:
         raise ValueError(f"controls on {c._device} for logits on {logits.device}")
     if c.masks is not None and c.masks.shape[0] and c.masks.shape[1] * 32 < vocab:
         raise ValueError(f"masks of {c.masks.shape[1]} words for {vocab} tokens")
-    return rows, vocab, ld, logits.dtype is _FLOAT
+    return rows, vocab, ld, f32
+
+
+def _check_rows(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple[int, ...], dev: torch.device) -> None:
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{name} must be contiguous {dtype} {shape} on the logits' device")
 
 
 def _launch(controls: LogitControls, call: bytes, dev) -> None:
@@ -153,12 +159,15 @@ def select_tokens(logits: torch.Tensor, controls: LogitControls, temps: torch.Te
         raise ValueError("logits of no tokens")
     if out is None:
         out = torch.empty(rows, dtype=_INT, device=dev)
-    for name, t, dtype, shape in (("out", out, _INT, (rows,)), ("values", values, _FLOAT, (rows,)), ("temps", temps, _FLOAT, (rows,)),
-                                  ("seeds", seeds, _INT, (rows, 2))):
-        if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != dev):
-            raise ValueError(f"{name} must be contiguous {dtype} {shape} on the logits' device")
+    else:
+        _check_rows("out", out, _INT, (rows,), dev)
+    if values is not None:
+        _check_rows("values", values, _FLOAT, (rows,), dev)
     if (temps is None) != (seeds is None):
         raise ValueError("temps and seeds come together")
+    if temps is not None:
+        _check_rows("temps", temps, _FLOAT, (rows,), dev)
+        _check_rows("seeds", seeds, _INT, (rows, 2), dev)
     if rows:
         at = [0 if t is None else t.data_ptr() for t in (temps, seeds, out, values)]
         _launch(controls, _CALL.pack(logits.data_ptr(), 0, *at, rows, vocab, ld, 0, f32, 0), dev)
