@@ -20,6 +20,9 @@ from ..ops import lora
 
 # ---------------------------------------------------------------------------------------------- shared prefixes
 
+DEEPEST = 64      # groups within groups that are looked at
+
+
 def shared_groups(tables: list[list[int]]) -> tuple[list[int], list[int], list[int]]:
     """Groups of sequences whose page tables begin alike: (order of the sequences, sizes of the groups, pages that each shares).
     Groups follow one another in the order; sequences that share nothing are groups of one with no pages. Where a group contains
@@ -32,18 +35,18 @@ def shared_groups(tables: list[list[int]]) -> tuple[list[int], list[int], list[i
             n += 1
         alike.append(n)
 
-    def split(lo: int, hi: int) -> tuple[int, list[tuple[int, int]]]:
+    def split(lo: int, hi: int, depth: int = 0) -> tuple[int, list[tuple[int, int]]]:
         """(pages saved, [(size, pages)]) for the sequences [lo, hi) of the order."""
         if hi - lo == 1:
             return 0, [(1, 0)]
         common = min(alike[lo:hi - 1])
         one = ((hi - lo - 1) * common, [(hi - lo, common)])
-        if common == alike[lo] and len(set(alike[lo:hi - 1])) == 1 and common > 0:
+        if common > 0 and (depth >= DEEPEST or len(set(alike[lo:hi - 1])) == 1):
             return one
         saved, parts, start = 0, [], lo
         for i in range(lo, hi):
             if i == hi - 1 or alike[i] == common:
-                s, p = split(start, i + 1)
+                s, p = split(start, i + 1, depth + 1)
                 saved, start = saved + s, i + 1
                 parts += p
         return one if one[0] >= saved and common > 0 else (saved, parts)

@@ -193,7 +193,7 @@ def fill_shared_plan(sizes: Sequence[int], prefixes: Sequence[int], words: np.nd
     while -(-longest // c) > max_parts or sum(-(-n // per) * -(-p // c) for _, n, p in groups) > max_pieces:
         if c >= longest:
             raise ValueError(f"{len(groups)} groups do not fit a plan of {max_pieces} pieces and {max_parts} parts")
-        c += PIECE_TOKENS
+        c += max(PIECE_TOKENS, c // 8 // PIECE_TOKENS * PIECE_TOKENS)
     count = most = tokens = 0
     for at, n, p in groups:
         k = -(-p // c)

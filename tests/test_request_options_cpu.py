@@ -107,3 +107,18 @@ def test_http_options():
     asyncio.run(go())
     loop.stop()
     assert seen == [{}, {"controls": TokenControls(repetition=1.3)}, {"adapter": "z"}]
+
+
+def test_groups_nested_deeper_than_is_looked_at():
+    """Every sequence shares one page more than the one before it: the groups cover all of them, and share no more than they have."""
+    from crosspool_b200.engine.request_options import shared_groups
+
+    n = 3000
+    tables = [list(range(i + 1)) + [10 ** 6 + i] for i in range(n)]
+    order, sizes, pages = shared_groups(tables)
+    assert sorted(order) == list(range(n)) and sum(sizes) == n
+    at = 0
+    for size, shared in zip(sizes, pages):
+        first = tables[order[at]][:shared]
+        assert len(first) == shared and all(tables[order[i]][:shared] == first for i in range(at, at + size))
+        at += size
