@@ -305,7 +305,7 @@ typedef struct XpDecodeAttnArgs {
   int num_pages;              /* pages in the cache (bound of the tensor maps); 0: SIMT kernel only */
   uint32_t* status;           /* optional: set non-zero when a bounded wait ran out */
   int force_simt;             /* testing: skip the tensor-core kernel */
-  int reserved;
+  int max_len;                /* rows are read no further than this (0: as far as seq_lens says; negative: not at all) */
 } XpDecodeAttnArgs;
 
 /* Tensor-core decode attention of single rows: padded query groups, keys and values of different widths, capped scores,

@@ -53,6 +53,12 @@ __device__ __forceinline__ void unpack(const RawVec<E>& r, float* out) {
   }
 }
 
+// Tokens of a row that are read.
+__device__ __forceinline__ int row_len(const XpDecodeAttnArgs& a, int b) {
+  const int len = a.seq_lens[b];
+  return a.max_len == 0 ? len : min(max(len, 0), max(a.max_len, 0));
+}
+
 // Partial result layout in the workspace: [batch, q_head, split, D + 2] floats:
 // D un-normalised accumulators, running max (log2 domain), running sum.
 template <int D, int GMAX>
@@ -64,7 +70,7 @@ decode_attn_kernel(XpDecodeAttnArgs a) {
 
   const int split = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int G = a.q_heads / a.kv_heads;
-  const int len = a.seq_lens[b];
+  const int len = row_len(a, b);
   const int nsplit = gridDim.x;
   // Fixed-size slices (chunk_tokens > 0) give every CTA the same amount of work whatever the
   // sequence length, so long and short sequences in one batch balance across the SMs; slices
@@ -341,7 +347,7 @@ __device__ __forceinline__ Span row_span(const A& args, int b) {
       s.len -= s.skip;
     }
   } else {
-    s.len = args.seq_lens[b];
+    s.len = row_len(args, b);
   }
   return s;
 }

@@ -853,7 +853,11 @@ static int launch(const XpDecodeSharedArgs& args, cudaStream_t s) {
 extern "C" int xp_decode_shared(const XpDecodeSharedArgs* r, void* stream) {
   const XpDecodeAttnArgs* a = &r->a;
   if (a->batch <= 0) return 0;
-  if (r->max_pieces <= 0) return xp_decode_attn(a, stream);      // no prefixes
+  if (r->max_pieces <= 0) {                                      // no prefixes
+    XpDecodeAttnArgs plain = *a;
+    plain.max_len = r->max_len > 0 ? r->max_len : -1;
+    return xp_decode_attn(&plain, stream);
+  }
   if (a->kv_heads <= 0 || a->q_heads % a->kv_heads != 0) return -10;
   if (a->ws == nullptr || (reinterpret_cast<uintptr_t>(a->ws) & 15) != 0 || (reinterpret_cast<uintptr_t>(a->out) & 7) != 0) return -11;
   if (a->q_heads / a->kv_heads > 16 || a->num_pages <= 0 || a->page_size < 16 || (a->page_size & (a->page_size - 1)) != 0 ||

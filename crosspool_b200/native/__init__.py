@@ -239,7 +239,7 @@ class DecodeAttnArgs(C.Structure):
         ("num_pages", C.c_int),
         ("status", C.c_void_p),
         ("force_simt", C.c_int),
-        ("reserved", C.c_int),
+        ("max_len", C.c_int),
     ]
 
 

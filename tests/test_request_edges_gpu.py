@@ -1,0 +1,47 @@
+"""Calls of the operators of requests at the edges of what their documentation allows."""
+import pytest
+import torch
+
+from request_oracle import paged_attention
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ shared prefixes
+
+def cache(rows, tokens, hq, hk, d, page, seed=0):
+    """Rows of ``tokens`` tokens each, in pages of their own."""
+    g = torch.Generator().manual_seed(seed)
+    wide = -(-tokens // page)
+    table = torch.randperm(rows * wide, generator=g).int().view(rows, wide)
+    k, v = (torch.randn(rows * wide, page, hk, d, generator=g).bfloat16() for _ in range(2))
+    q = (1.5 * torch.randn(rows, hq, d, generator=g)).bfloat16()
+    return [t.cuda() for t in (q, k, v, table)]
+
+
+def close(got, q, k, v, table, lens, scale=None):
+    """The weights are rounded to bf16 (half a step: 2^-8 of each), the result once more; what fp32 sums and 2 ** x add is below
+    2^-14 of the weighted values: scores below 64 carry d 2^-24 64 of error."""
+    want, mass = paged_attention(q, k, v, table, lens, scale)
+    off, tol = (got.double() - want).abs(), (2.0 ** -8 + 2.0 ** -14) * mass + 2.0 ** -8 * want.abs() + 1e-30
+    assert torch.isfinite(got).all() and (off <= tol).all(), (off / tol).max()
+
+
+@pytest.mark.parametrize("sizes,prefixes,max_len", [([], [], n) for n in (0, 1, 100, 640, 2000)] + [(s, p, n) for s, p in (([5], [7]), ([3], [64])) for n in (100, 640, 2000)])
+@pytest.mark.parametrize("rows,d", [(5, 128), (5, 64), (300, 64)])
+def test_rows_are_read_no_further_than_the_plans_bound(sizes, prefixes, max_len, rows, d):
+    """Whether the plan holds a prefix or not, and whether rows are read in one slice or in several. The tables hold all tokens
+    that the lengths name, so that reading on would stay in the cache."""
+    from crosspool_b200.ops import attention as A
+    from crosspool_b200.ops import gemm
+
+    q, k, v, table = cache(rows, max(max_len, 16) + 200, 8, 4, d, 16, seed=max_len)
+    for r in range(1, sum(sizes)):
+        table[r, :prefixes[0] // 16] = table[0, :prefixes[0] // 16]
+    lens = torch.full((rows,), max_len, dtype=torch.int32, device="cuda")
+    lens[0], lens[1], lens[2], lens[3] = max_len + 1, max_len + 200, max_len // 2, -3
+    plan = A.shared_prefix_plan(sizes, prefixes, rows=rows, q_heads=8, kv_heads=4, head_dim=d, max_len=max_len)
+    got = A.paged_decode_shared(q, k, v, table, lens, plan)
+    gemm.check_status(q.device)
+    close(got, q, k, v, table, lens.clamp(0, max_len))
+    assert not got[3].any()
