@@ -214,6 +214,7 @@ class AttentionEngine:
         self._last_was_prefill = False
         self.stats = {"prefill_steps": 0, "decode_steps": 0, "h2d_bytes": 0, "d2h_bytes": 0, "launches": 0}
         self.stream = torch.cuda.Stream(self.device)
+        self.stream.wait_stream(torch.cuda.current_stream(self.device))      # weights and buffers were filled there
         self._b_key = None
         self._b_pos = None
         self._b_last = None
@@ -338,12 +339,16 @@ class AttentionEngine:
     # ------------------------------------------------------------------ request API
     def load_adapter(self, name: str, layers: list[dict], scale: float = 1.0) -> None:
         """Loads a low-rank adapter of the attention projections (``layers[l]``: {``q``, ``k``, ``v``, ``o``: (A, B)}); requests name
-        it in ``add_request(adapter=name)``. Needs ``EngineConfig(adapters=...)``."""
+        it in ``add_request(adapter=name)``. Needs ``EngineConfig(adapters=...)``. The tensors are read behind the work of the
+        caller's current stream; they may be freed when the call returns."""
         if self.adapter_rows is None:
             raise ValueError("adapters need EngineConfig(adapters=...)")
+        self.stream.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(self.stream):
-            self.adapter_rows.load(name, layers, scale)
-            self.stream.synchronize()        # the caller may free its tensors
+            try:
+                self.adapter_rows.load(name, layers, scale)
+            finally:
+                self.stream.synchronize()
 
     def unload_adapter(self, name: str) -> None:
         """Frees the adapter's slot; refused while requests use it."""

@@ -55,6 +55,8 @@ class AdapterStack:
         s.k, s.n, s.rank, s.parts, s.slots = in_features, self.out_features, self.rank, len(self.parts), slots
         s.part_end = (C.c_int * 4)(*(ends + [end] * (4 - len(ends))))
         self._fields = bytes(s)[native.LoraArgs.a.offset:]
+        if self.device.type == "cuda":          # a slot may be loaded on any stream from here on
+            torch.cuda.current_stream(self.device).synchronize()
 
     @torch.no_grad()
     def load(self, slot: int, a: torch.Tensor | Sequence[torch.Tensor], b: torch.Tensor | Sequence[torch.Tensor], scale: float = 1.0) -> None:

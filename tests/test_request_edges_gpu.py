@@ -45,3 +45,50 @@ def test_rows_are_read_no_further_than_the_plans_bound(sizes, prefixes, max_len,
     gemm.check_status(q.device)
     close(got, q, k, v, table, lens.clamp(0, max_len))
     assert not got[3].any()
+
+
+# ------------------------------------------------------------------------------------------------ adapters
+
+def behind(stream, ms=60):
+    """Keeps ``stream`` busy for about so long."""
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(int(ms * 1.9e6))
+
+
+def test_adapters_computed_on_the_callers_stream_are_loaded_when_they_are_there():
+    from test_request_options_gpu import build
+
+    from crosspool_b200.ops import lora
+
+    cfg, eng, _ = build(adapters=1, adapter_rank=16)
+    g = torch.Generator().manual_seed(3)
+    a, b = (torch.randn(*s, generator=g).bfloat16().cuda() for s in ((8, cfg.hidden_size), (cfg.kv_size, 8)))
+    want = lora.AdapterStack(1, cfg.hidden_size, (cfg.q_size, cfg.kv_size, cfg.kv_size), 16)
+    want.load(0, [None, 2 * a, None], [None, 4 * b, None])
+    torch.cuda.synchronize()
+    late, side = [(torch.zeros_like(a), torch.zeros_like(b)) for _ in range(cfg.num_layers)], torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    behind(side)
+    with torch.cuda.stream(side):
+        for x, y in late:
+            x.copy_(a).mul_(2)
+            y.copy_(b).mul_(4)
+        eng.load_adapter("x", [{"k": pair} for pair in late])
+    for stack in eng.adapter_rows.qkv:
+        assert torch.equal(stack.a, want.a) and torch.equal(stack.b, want.b)
+
+
+def test_slots_of_a_stack_made_behind_other_work_are_loaded_on_any_stream():
+    from crosspool_b200.ops import lora
+
+    a, b = torch.ones(8, 256, device="cuda").bfloat16(), torch.ones(128, 8, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    maker, loader = torch.cuda.Stream(), torch.cuda.Stream()
+    behind(maker)
+    with torch.cuda.stream(maker):
+        stack = lora.AdapterStack(2, 256, 128, 8)
+    with torch.cuda.stream(loader):
+        stack.load(1, a, b, 0.5)
+    torch.cuda.synchronize()
+    assert stack.ranks.tolist() == [0, 16] and stack.scale.tolist() == [0.0, 0.5] and stack.part_ranks.tolist() == [[0] * 4, [8, 0, 0, 0]]
+    assert stack.a[1].float().sum() == 8 * 256 and stack.b[1].float().sum() == 128 * 8
