@@ -22,6 +22,7 @@ import torch
 
 from .engine.atn_engine import AttentionEngine, EngineConfig, Sequence
 from .engine.ffn_local import LocalFfnPort
+from .engine.request_options import RequestFailed
 from .models import config as model_config
 from .models.config import ModelConfig
 from .models.weights import load_attention_from_safetensors, random_attention_weights, random_ffn_weights
@@ -38,6 +39,8 @@ class InstanceHandle:
 @dataclass
 class StepResult:
     tokens: dict[str, list[tuple[Sequence, int]]] = field(default_factory=dict)
+    # requests that left their Instance because something of their own failed (a mask callback): (model, sequence, error)
+    failed: list[tuple[str, Sequence, Exception]] = field(default_factory=list)
 
     @property
     def num_tokens(self) -> int:
@@ -58,20 +61,31 @@ class Deployment:
 
     def add_request(self, model_id: str, prompt: list[int], max_new_tokens: int, arrival: float | None = None,
                     **sampling) -> Sequence:
-        """``sampling``: ``temperature`` and ``seed`` (engines built with ``EngineConfig(sampling=True)``)."""
+        """``sampling``: ``temperature`` and ``seed`` (engines built with ``EngineConfig(sampling=True)``), ``controls``, ``adapter``."""
         return self._by_id[model_id].engine.add_request(prompt, max_new_tokens, arrival, **sampling)
 
     @property
     def has_work(self) -> bool:
         return any(i.engine.has_work for i in self.instances)
 
+    @staticmethod
+    def _launch(i: InstanceHandle, res: StepResult) -> None:
+        """Starts an Instance's next step. Requests that fail on their own leave it, and the step is started without them."""
+        while i.engine.has_work:
+            try:
+                i.engine.launch_step()
+                return
+            except RequestFailed as e:
+                i.engine.drop_request(e.sequence, e.__cause__)
+                res.failed.append((i.model_id, e.sequence, e.__cause__))
+
     def step(self) -> StepResult:
         """One iteration of every Instance that has work."""
         active = [i for i in self.instances if i.engine.has_work]
         self.idle_tick()
-        for i in active:
-            i.engine.launch_step()
         res = StepResult()
+        for i in active:
+            self._launch(i, res)
         for i in active:
             res.tokens[i.model_id] = i.engine.collect_step()
         return res
@@ -95,7 +109,7 @@ class Deployment:
                 progressed = progressed or getattr(e, "step_is_device_work", True)
                 res.tokens[i.model_id] = e.collect_step()
             if e.has_work:
-                e.launch_step()
+                self._launch(i, res)
                 progressed = progressed or getattr(e, "step_is_device_work", True)
         if not progressed and not waiting:
             time.sleep(poll_s)          # every Instance with work is waiting for something on the host (KV capacity)
@@ -103,8 +117,7 @@ class Deployment:
             if len(waiting) == 1:       # nothing else to overlap with: wait for it (releases the interpreter lock)
                 i = waiting[0]
                 res.tokens[i.model_id] = i.engine.collect_step()
-                if i.engine.has_work:
-                    i.engine.launch_step()
+                self._launch(i, res)
             else:
                 time.sleep(poll_s)
         return res

@@ -83,6 +83,7 @@ class Sequence:
     refill_len: int = 0              # > 0 after a retraction: prompt + generated tokens to recompute before decoding on
     controls: TokenControls | None = None
     adapter: str | None = None       # name of a loaded adapter
+    error: Exception | None = None   # why the request was dropped before its end
 
     @property
     def fill_len(self) -> int:
@@ -413,6 +414,21 @@ class AttentionEngine:
         n = self.adapter_rows.fill(index, rows)
         self.adapter_rows.copy(rows)
         return n
+
+    def drop_request(self, s: "Sequence", error: Exception | None = None) -> None:
+        """Takes a request out of the engine before its end, with its pages and slots. Refused while a step is in flight. (After a step
+        that ended in a ``RequestFailed`` error, the next one goes on without that request.)"""
+        if self.step_in_flight:
+            raise RuntimeError("a step is in flight")
+        queue = next((q for q in (self.waiting, self.prefilling, self.running) if s in q), None)
+        if queue is None:
+            raise ValueError(f"sequence {s.seq_id} is not in the engine")
+        queue.remove(s)
+        if queue is self.waiting:
+            self._publish_demand(0, None)    # what the head of the queue asked for; the next step asks anew
+        self._b_key = None
+        self._release_pages(s)
+        s.error = error
 
     def _adapter_slot(self, s: "Sequence") -> int:
         return self.adapter_rows.names[s.adapter] if s.adapter is not None else -1

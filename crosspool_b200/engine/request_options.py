@@ -18,6 +18,15 @@ from ..ops import logits as L
 from ..ops import lora
 
 
+class RequestFailed(RuntimeError):
+    """What one request brought along failed in the step of all (``__cause__``: its error). Nothing was launched: the step can be taken
+    again, or without the request (``AttentionEngine.drop_request(sequence)``)."""
+
+    def __init__(self, sequence, error: Exception):
+        super().__init__(str(error))
+        self.sequence, self.__cause__ = sequence, error
+
+
 # ---------------------------------------------------------------------------------------------- shared prefixes
 
 DEEPEST = 64      # groups within groups that are looked at
@@ -155,7 +164,8 @@ class AdapterRows:
 class TokenControls:
     """Controls on the tokens of one request. ``repetition`` (1: none), ``frequency``, ``presence`` and ``bias`` as in
     :class:`~crosspool_b200.ops.logits.LogitControls`. ``allowed``: called with the generated tokens before every token; gives the
-    mask of the next one as ``ceil(vocab / 32)`` 32-bit words (bit i % 32 of word i / 32: token i), or None for no mask."""
+    mask of the next one as ``ceil(vocab / 32)`` 32-bit words (bit i % 32 of word i / 32: token i), or None for no mask. Where it
+    raises, or its mask has another shape or allows no token, the request fails (:class:`RequestFailed`), and no other does."""
 
     repetition: float = 1.0
     frequency: float = 0.0
@@ -224,7 +234,7 @@ class ControlRows:
         """Fills and copies the rows of a pass (on the engine's stream): ``seqs[i]`` samples its next token in row i unless
         ``samples[i]`` is False (a portion of a prompt that is not its last)."""
         # what may raise comes first: a step that failed here can be taken again
-        words = [self._mask(s) if wanted and s.controls is not None and s.controls.allowed is not None else None for s, wanted in zip(seqs, samples)]
+        words = [self.mask(s) if wanted and s.controls is not None and s.controls.allowed is not None else None for s, wanted in zip(seqs, samples)]
         self._neutral()
         n, h = self.rows, self.meta_host.numpy()
         f, ids, vals = h[5 * n:8 * n].view(np.float32).reshape(3, n), self.bias_host[0].numpy(), self.bias_host[1].numpy().view(np.float32)
@@ -251,14 +261,21 @@ class ControlRows:
         if masks:
             self.masks[:masks].copy_(self.masks_host[:masks], non_blocking=True)
 
-    def _mask(self, s) -> "np.ndarray | None":
-        words = s.controls.allowed(list(s.generated))
-        if words is None:
-            return None
-        words = np.asarray(words)
-        if words.shape != (self.words,):
-            raise ValueError(f"a mask of shape {words.shape} for {self.vocab} tokens ({self.words} words)")
-        return words.astype(np.uint32).view(np.int32) if words.dtype != np.int32 else words
+    def mask(self, s) -> "np.ndarray | None":
+        """The mask of a sequence's next token; :class:`RequestFailed` where the request gives none that a token fits."""
+        try:
+            words = s.controls.allowed(list(s.generated))
+            if words is None:
+                return None
+            words = np.asarray(words)
+            if words.shape != (self.words,):
+                raise ValueError(f"a mask of shape {words.shape} for {self.vocab} tokens ({self.words} words)")
+            words = words.astype(np.uint32).view(np.int32) if words.dtype != np.int32 else words
+            if not words[:-1].any() and not int(words[-1]) & ((1 << (self.vocab - 1) % 32 + 1) - 1):
+                raise ValueError("the mask allows no token")
+            return words
+        except Exception as e:
+            raise RequestFailed(s, e)
 
     def _history(self, i: int, s, h: np.ndarray) -> None:
         """Row i's history: its slot gets the whole sequence once, then every call the token that the sequence grew by."""

@@ -134,6 +134,13 @@ class EngineLoop:
             tick()          # idle Instances still answer elastic-KV capacity commands
         time.sleep(self.idle_sleep)
 
+    def _deliver_failed(self, res) -> None:
+        """Requests whose own mask or the like failed are answered with their error; serving goes on."""
+        for model_id, seq, error in getattr(res, "failed", ()):
+            p = self._by_seq.pop((model_id, seq.seq_id), None)
+            if p is not None:
+                p.deliver(error)
+
     def _run(self) -> None:
         try:
             while not self._stop.is_set():
@@ -163,6 +170,7 @@ class EngineLoop:
                 if self.sink is not None:
                     self.sink(batch, time.perf_counter())
                 deliver_batch(batch)
+                self._deliver_failed(res)      # behind their last tokens
         except Exception as e:  # device failure: fail every waiting request, stop (fail-stop)
             self.error = e
             for p in self._by_seq.values():

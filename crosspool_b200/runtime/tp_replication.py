@@ -89,6 +89,7 @@ class TpEngineLoop(EngineLoop):
                         self.tokens += 1
                         if done:
                             del self._by_seq[(model_id, seq.seq_id)]
+                self._deliver_failed(res)
         except Exception as e:
             self.error = e
             for p in self._by_seq.values():

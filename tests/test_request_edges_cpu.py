@@ -1,6 +1,7 @@
 """Operators of requests, their engine and their serving loop at the edges of what their documentation allows; no GPU is needed."""
 import contextlib
 
+import numpy as np
 import pytest
 import torch
 
@@ -39,3 +40,154 @@ def test_adapters_are_read_behind_the_callers_stream_and_before_the_call_returns
     with pytest.raises(ValueError, match="rank") if fails else contextlib.nullcontext():
         eng.load_adapter("x", [1], 2.0)
     assert done == [("wait", "caller"), (eng.stream, "x", [1], 2.0), "synchronize"]
+
+
+# ------------------------------------------------------------------------------------------------ masks
+
+def control_rows(vocab):
+    from crosspool_b200.engine.request_options import ControlRows
+
+    rows = ControlRows.__new__(ControlRows)
+    rows.vocab, rows.words = vocab, (vocab + 31) // 32
+    return rows
+
+
+def with_mask(allowed, generated=()):
+    from crosspool_b200.engine.atn_engine import Sequence
+    from crosspool_b200.engine.request_options import TokenControls
+
+    return Sequence(3, [1], 4, generated=list(generated), controls=TokenControls(allowed=allowed))
+
+
+@pytest.mark.parametrize("vocab,words", [(40, [0, 1]), (40, [0, 0x80]), (64, [0, 0x80000000]), (32, [1]), (1, [1]), (40, [0x80000000, 0])])
+@pytest.mark.parametrize("dtype", ["uint32", "int32", "int64"])
+def test_masks_that_a_token_fits(vocab, words, dtype):
+    want = np.array(words, dtype=np.uint32).view(np.int32)
+    given = want if dtype == "int32" else np.array(words, dtype=dtype)
+    assert control_rows(vocab).mask(with_mask(lambda g: given)).tolist() == want.tolist()
+    assert control_rows(vocab).mask(with_mask(lambda g: None)) is None
+
+
+@pytest.mark.parametrize("vocab,mask,match", [(40, [0, 0], "no token"), (40, [0, 0xffffff00], "no token"), (1, [0xfffffffe], "no token"), (64, [0, 0], "no token"),
+                                              (40, [1], "shape"), (40, [[1, 1]], "shape"), (40, "x", "shape")])
+def test_masks_that_fail_their_request(vocab, mask, match):
+    from crosspool_b200.engine.request_options import RequestFailed
+
+    s = with_mask(lambda g: mask if isinstance(mask, str) else np.array(mask, dtype=np.uint32))
+    with pytest.raises(RequestFailed, match=match) as e:
+        control_rows(vocab).mask(s)
+    assert e.value.sequence is s and isinstance(e.value.__cause__, ValueError)
+
+
+def test_a_request_is_dropped_with_its_pages():
+    eng = bare_engine()
+    eng._pending = eng._pre_inflight = eng._inflight = eng.capacity = None
+    a, b, c, d = (eng.add_request([i + 1], 4) for i in range(4))
+    eng.waiting.remove(b)
+    eng.waiting.remove(c)
+    eng.prefilling.append(b)
+    eng.running.append(c)
+    eng._b_key = (c.seq_id,)
+    why = ValueError("why")
+    for s in (a, b, c):
+        eng.drop_request(s, why)
+    assert list(eng.waiting) == [d] and not eng.prefilling and not eng.running and eng._b_key is None
+    assert eng.kv.released == [a.seq_id, b.seq_id, c.seq_id] and a.error is why and d.error is None
+    with pytest.raises(ValueError, match="not in"):
+        eng.drop_request(a)
+    eng._inflight = ([d], 1)
+    with pytest.raises(RuntimeError, match="in flight"):
+        eng.drop_request(d)
+
+
+class MaskedEngine:
+    """Stands for an engine: every request gets a token a step, the next one's number; one with a mask asks it first."""
+
+    def __init__(self):
+        self.live, self._out, self._next = [], None, 0
+
+    def add_request(self, prompt, max_new_tokens, arrival=None, controls=None):
+        from crosspool_b200.engine.atn_engine import Sequence
+
+        s = Sequence(self._next, list(prompt), max_new_tokens, controls=controls)
+        self._next += 1
+        self.live.append(s)
+        return s
+
+    has_work = property(lambda self: bool(self.live))
+    step_in_flight = property(lambda self: self._out is not None)
+
+    def step_ready(self):
+        return True
+
+    def drop_request(self, s, error=None):
+        assert self._out is None
+        self.live.remove(s)
+        s.error = error
+
+    def launch_step(self):
+        assert self._out is None, "launched twice"
+        for s in self.live:
+            if s.controls is not None:
+                control_rows(40).mask(s)
+        self._out = list(self.live)
+
+    def collect_step(self):
+        seqs, self._out = self._out or [], None
+        for s in seqs:
+            s.generated.append(len(s.generated))
+            if s.finished:
+                self.live.remove(s)
+        return [(s, s.generated[-1]) for s in seqs]
+
+
+def drain(p, timeout=20):
+    got = []
+    while True:
+        item = p.out.get(timeout=timeout)
+        if isinstance(item, Exception):
+            return got, item
+        got.append(item[0])
+        if item[1]:
+            return got, None
+
+
+@pytest.mark.parametrize("stepping", ["step", "step_async"])
+def test_a_mask_that_fails_ends_its_request_alone(stepping):
+    from crosspool_b200.deployment import Deployment, InstanceHandle
+    from crosspool_b200.engine.request_options import TokenControls
+    from crosspool_b200.runtime.serving import EngineLoop
+
+    dep = Deployment([InstanceHandle(m, None, MaskedEngine()) for m in ("a", "b")])
+    if stepping == "step":
+        dep.step_async = dep.step
+    loop = EngineLoop(dep)
+
+    def raises(g):
+        if len(g) == 2:
+            raise KeyError("grammar")
+        return None
+
+    masks = [raises, lambda g: np.zeros(2, dtype=np.uint32) if len(g) == 3 else None, lambda g: np.zeros(9, dtype=np.uint32)]
+    plain = [loop.submit(m, [1], 9) for m in ("a", "b")]
+    bad = [loop.submit("b", [1], 9, options={"controls": TokenControls(allowed=f)}) for f in masks]
+    alone = loop.submit("a", [1], 9, options={"controls": TokenControls(allowed=raises)})
+    loop.start()
+    try:
+        assert all(drain(p) == (list(range(9)), None) for p in plain)
+        got = [drain(p) for p in (*bad, alone)]
+        assert [(g, type(e)) for g, e in got] == [([0, 1], KeyError), ([0, 1, 2], ValueError), ([], ValueError), ([0, 1], KeyError)]
+        later = loop.submit("b", [1], 3)                        # the loop goes on, also after an Instance that was left without work
+        assert drain(later) == ([0, 1, 2], None) and loop.error is None and not loop._by_seq
+    finally:
+        loop.stop()
+
+
+def test_the_only_request_of_a_deployment_may_fail():
+    from crosspool_b200.deployment import Deployment, InstanceHandle
+    from crosspool_b200.engine.request_options import TokenControls
+
+    dep = Deployment([InstanceHandle("a", None, MaskedEngine())])
+    s = dep.add_request("a", [1], 4, controls=TokenControls(allowed=lambda g: np.zeros(2, dtype=np.int32)))
+    res = dep.step()
+    assert [(m, x) for m, x, _ in res.failed] == [("a", s)] and res.num_tokens == 0 and not dep.has_work and isinstance(s.error, ValueError)

@@ -92,3 +92,58 @@ def test_slots_of_a_stack_made_behind_other_work_are_loaded_on_any_stream():
     torch.cuda.synchronize()
     assert stack.ranks.tolist() == [0, 16] and stack.scale.tolist() == [0.0, 0.5] and stack.part_ranks.tolist() == [[0] * 4, [8, 0, 0, 0]]
     assert stack.a[1].float().sum() == 8 * 256 and stack.b[1].float().sum() == 128 * 8
+
+
+# ------------------------------------------------------------------------------------------------ masks
+
+@pytest.mark.parametrize("mixed", [False, True])
+def test_requests_whose_mask_fails_leave_the_engine_with_all_they_held(mixed):
+    import queue
+
+    import numpy as np
+    from test_request_options_gpu import adapter, build, prompts
+
+    from crosspool_b200.deployment import Deployment, InstanceHandle
+    from crosspool_b200.engine.request_options import TokenControls
+    from crosspool_b200.runtime.serving import EngineLoop
+
+    cfg, eng, _ = build(controls=True, shared_prefix=True, prefix_cache=True, adapters=1, max_batch=8, mixed_batches=mixed)
+    eng.load_adapter("a", adapter(cfg, 5))
+    eng.warmup()
+    full = eng.kv.allocator.free_pages
+    words = (cfg.vocab_size + 31) // 32
+
+    def until(n):
+        def allowed(g):
+            if len(g) == n:
+                raise KeyError(n)
+            return None
+        return TokenControls(repetition=1.2, presence=0.5, allowed=allowed)
+
+    cs = [None, until(0), until(1), until(6), TokenControls(allowed=lambda g: np.zeros(words, dtype=np.uint32) if len(g) == 4 else None),
+          TokenControls(allowed=lambda g: [1]), TokenControls(repetition=1.3)]
+    loop = EngineLoop(Deployment([InstanceHandle("m", cfg, eng)]))
+    ps = [loop.submit("m", p, 12, options={**({} if c is None else {"controls": c}), **({"adapter": "a"} if i % 2 else {})})
+          for i, (p, c) in enumerate(zip(prompts(cfg, [30, 41, 5, 18, 60, 7, 22], shared=40, seed=3), cs))]
+    loop.start()
+    try:
+        got = []
+        for p in ps:
+            toks = []
+            while True:
+                item = p.out.get(timeout=60)
+                if isinstance(item, Exception):
+                    got.append((len(toks), type(item).__name__))
+                    break
+                toks.append(item[0])
+                if item[1]:
+                    got.append((len(toks), None))
+                    break
+        assert got == [(12, None), (0, "KeyError"), (1, "KeyError"), (6, "KeyError"), (4, "ValueError"), (0, "ValueError"), (12, None)]
+        with pytest.raises(queue.Empty):
+            ps[0].out.get_nowait()
+    finally:
+        loop.stop()
+    assert loop.error is None and not eng.has_work and not eng.control_rows.slots and len(eng.control_rows.free) == 8
+    eng.kv.allocator.free(eng.prefix.evict(10 ** 6))
+    assert eng.kv.allocator.free_pages == full and not eng.kv.tables
