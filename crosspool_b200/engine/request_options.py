@@ -270,7 +270,8 @@ class ControlRows:
             words = np.asarray(words)
             if words.shape != (self.words,):
                 raise ValueError(f"a mask of shape {words.shape} for {self.vocab} tokens ({self.words} words)")
-            words = words.astype(np.uint32).view(np.int32) if words.dtype != np.int32 else words
+            # (a copy: the callback may fill the same buffer for the next sequence)
+            words = words.copy() if words.dtype == np.int32 else words.astype(np.uint32).view(np.int32)
             if not words[:-1].any() and not int(words[-1]) & ((1 << (self.vocab - 1) % 32 + 1) - 1):
                 raise ValueError("the mask allows no token")
             return words

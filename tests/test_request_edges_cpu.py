@@ -191,3 +191,18 @@ def test_the_only_request_of_a_deployment_may_fail():
     s = dep.add_request("a", [1], 4, controls=TokenControls(allowed=lambda g: np.zeros(2, dtype=np.int32)))
     res = dep.step()
     assert [(m, x) for m, x, _ in res.failed] == [("a", s)] and res.num_tokens == 0 and not dep.has_work and isinstance(s.error, ValueError)
+
+
+def test_masks_of_one_buffer_are_read_when_they_are_given():
+    """A grammar library may fill the same words for every call."""
+    words = np.zeros(2, dtype=np.int32)
+
+    def allowed(token):
+        def f(g):
+            words[:] = [1 << token, 0]
+            return words
+        return f
+
+    rows = control_rows(40)
+    got = [rows.mask(with_mask(allowed(t))) for t in (3, 9)]
+    assert [m.tolist() for m in got] == [[8, 0], [512, 0]]
