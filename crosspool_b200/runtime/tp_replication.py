@@ -15,6 +15,7 @@ step the replicated Instances in the same iterations.
 
 from __future__ import annotations
 
+import pickle
 
 from .serving import EngineLoop, Pending
 
@@ -32,11 +33,26 @@ class TpEngineLoop(EngineLoop):
         dist.broadcast_object_list(box, src=dist.get_global_rank(self.group, 0) if self.group is not None else 0, group=self.group)
         return box[0]["requests"], box[0]["stop"]
 
+    def _record(self, p: Pending) -> dict | None:
+        """What the other ranks are told of a request; None, and the request refused, where they cannot be told. (A mask callback has
+        its state in one process: ranks that called copies of their own might not choose the same tokens.)"""
+        record = {"model": p.model_id, "prompt": p.prompt, "max_new_tokens": p.max_new_tokens, "temperature": p.temperature,
+                  "seed": p.seed, "options": p.options}
+        try:
+            if getattr(p.options.get("controls"), "allowed", None) is not None:
+                raise ValueError("masks of allowed tokens are not available where attention runs tensor-parallel")
+            pickle.dumps(record)
+        except Exception as e:
+            p.deliver(e if isinstance(e, ValueError) else ValueError(f"a request that cannot be sent to the other ranks: {e}"))
+            return None
+        return record
+
     def _run(self) -> None:
         hosted = {i.model_id for i in getattr(self.dep, "instances", ())} or None
         try:
             while True:
                 mine: list[Pending] = []
+                records: list[dict] = []
                 local: list[Pending] = []
                 if self.leader or self.replicated is not None:
                     while not self._inbox.empty():
@@ -44,12 +60,13 @@ class TpEngineLoop(EngineLoop):
                         if self.replicated is not None and p.model_id not in self.replicated:
                             local.append(p)
                         elif self.leader:
-                            mine.append(p)
+                            record = self._record(p)
+                            if record is not None:
+                                mine.append(p)
+                                records.append(record)
                         else:
                             p.deliver(RuntimeError(f"{p.model_id} is served by its tensor-parallel leader, not by this rank"))
-                reqs, stop = self._exchange(
-                    [{"model": p.model_id, "prompt": p.prompt, "max_new_tokens": p.max_new_tokens, "temperature": p.temperature,
-                      "seed": p.seed, "options": p.options} for p in mine] if self.leader else None, self._stop.is_set())
+                reqs, stop = self._exchange(records if self.leader else None, self._stop.is_set())
                 if stop:
                     for p in local:
                         p.deliver(RuntimeError("the engine loop is stopping"))

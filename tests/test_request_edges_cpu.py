@@ -206,3 +206,70 @@ def test_masks_of_one_buffer_are_read_when_they_are_given():
     rows = control_rows(40)
     got = [rows.mask(with_mask(allowed(t))) for t in (3, 9)]
     assert [m.tolist() for m in got] == [[8, 0], [512, 0]]
+
+
+# ------------------------------------------------------------------------------------------------ replicated requests
+
+def _tp_rank(rank, port, q):
+    import os
+    import threading
+    import time
+
+    import torch.distributed as dist
+    from test_tp_replication import FakeDeployment
+
+    from crosspool_b200.engine.request_options import TokenControls
+    from crosspool_b200.runtime.tp_replication import TpEngineLoop
+
+    class Deployment(FakeDeployment):
+        def add_request(self, model, prompt, max_new_tokens, **kw):
+            s = super().add_request(model, prompt, max_new_tokens, **kw)
+            self.log[-1] += (kw,)
+            return s
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    dep = Deployment()
+    loop = TpEngineLoop(dep, None, leader=rank == 0, idle_sleep=0.001)
+    loop.start()
+    out = None
+    if rank == 0:
+        options = [{"controls": TokenControls(1.2, allowed=lambda g: None)}, {"controls": TokenControls(allowed=print)}, {"adapter": threading.Lock()},
+                   {"controls": TokenControls(1.5)}, {}]
+        asked = [loop.submit("m", [i + 1], 2, options=o) for i, o in enumerate(options)]
+        try:
+            out = [(g, type(e).__name__) for g, e in (drain(p) for p in asked)]
+        except Exception as e:
+            out = repr(e)
+        later = loop.submit("m", [9], 1)
+        time.sleep(0.05)
+        out = (out, drain(later)[0])
+        loop.stop()
+    else:
+        loop._thread.join(30)
+    q.put((rank, out, [e[2:] for e in dep.log if e[0] == "add"], repr(loop.error)))
+    dist.destroy_process_group()
+
+
+def test_options_that_cannot_be_replicated_fail_their_request_alone():
+    import multiprocessing as mp
+    import os
+
+    from crosspool_b200.engine.request_options import TokenControls
+
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    ps = [ctx.Process(target=_tp_rank, args=(r, 29900 + os.getpid() % 90, q), daemon=True) for r in (0, 1)]
+    for p in ps:
+        p.start()
+    try:
+        res = {r[0]: r[1:] for r in (q.get(timeout=60) for _ in ps)}
+    finally:
+        for p in ps:
+            p.join(10)
+            if p.is_alive():
+                p.terminate()
+    refused, done = res[0][0]
+    assert refused == [([], "ValueError")] * 3 + [([0, 1], "NoneType"), ([100, 101], "NoneType")] and done == [200]
+    added = [((4,), 2, {"controls": TokenControls(1.5)}), ((5,), 2, {}), ((9,), 1, {})]
+    assert res[0][1] == res[1][1] == added and res[0][2] == res[1][2] == "None"
