@@ -15,6 +15,7 @@ import numpy as np
 import torch
 
 from .. import native
+from .overlap import rows_meet
 
 MAX_RANK = 128
 MAX_PARTS = 4
@@ -169,7 +170,7 @@ def adapter_plan(index: Sequence[int], stack: "AdapterStack | int", device: str 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: AdapterPlan, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """``y[rows, out] + scale * (x[rows, in] @ A.T) @ B.T`` with every row's own adapter, rounded once; sums in fp32. ``out`` may
-    be ``y`` itself. bf16; rows may have a pitch (a multiple of 8 elements), so that a slice of a wider buffer can be read or written."""
+    be ``y`` itself, or rows that no row of ``x`` or ``y`` lies over. bf16; rows may have a pitch (a multiple of 8 elements), so that a slice of a wider buffer can be read or written."""
     rows = x.shape[0]
     if out is None:
         out = torch.empty_like(y)
@@ -189,8 +190,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: Adapte
         raise ValueError("the rows of out must not overlap one another or other rows of y")
     if plan.words.device != dev:
         raise ValueError("the plan lives on another device")
-    if rows and at_out == at_x:
-        raise ValueError("out may be y, but not x")
+    wide = 2 * stack.out_features
+    if rows and ((at_out != at_y and rows_meet(rows, at_out, 2 * ld_out, wide, at_y, 2 * ld_y, wide))
+                 or rows_meet(rows, at_out, 2 * ld_out, wide, at_x, 2 * ld_x, 2 * stack.in_features)):
+        raise ValueError("out may be y, but not x, and lie over neither")
     if dev.type != "cuda":
         raise ValueError("the kernel runs on a GPU")
     if rows <= 1:

@@ -1,5 +1,6 @@
 """Operators of requests, their engine and their serving loop at the edges of what their documentation allows; no GPU is needed."""
 import contextlib
+import random
 
 import numpy as np
 import pytest
@@ -273,3 +274,53 @@ def test_options_that_cannot_be_replicated_fail_their_request_alone():
     assert refused == [([], "ValueError")] * 3 + [([0, 1], "NoneType"), ([100, 101], "NoneType")] and done == [200]
     added = [((4,), 2, {"controls": TokenControls(1.5)}), ((5,), 2, {}), ((9,), 1, {})]
     assert res[0][1] == res[1][1] == added and res[0][2] == res[1][2] == "None"
+
+
+# ------------------------------------------------------------------------------------------------ results over inputs
+
+def test_rows_that_meet():
+    from crosspool_b200.ops.overlap import rows_meet
+
+    rng = random.Random(7)
+    for _ in range(3000):
+        rows = rng.randrange(0, 5)
+        pitch = rng.randrange(1, 12)
+        a, b = ((rng.randrange(0, 40), p, rng.randrange(1, 8)) for p in (pitch, pitch if rng.random() < 0.7 else rng.randrange(0, 12)))
+        sa, sb = ({at + r * p + i for r in range(rows) for i in range(w)} for at, p, w in (a, b))
+        got = rows_meet(rows, *a, *b)
+        assert got or not sa & sb                                   # never missed
+        wide = min(a[1], b[1]) >= max(a[2], b[2])
+        apart = not sa or not sb or max(sa) < min(sb) or max(sb) < min(sa)
+        assert not (got and apart)
+        if got and not sa & sb:                                     # what is refused all the same: pitches that differ, rows that wrap
+            assert a[1] != b[1] or not wide or (b[0] - a[0]) % a[1] + b[2] > a[1] or (b[0] - a[0]) % a[1] < a[2]
+
+
+def lora_case(rows=4):
+    from crosspool_b200.ops import lora
+
+    stack = lora.AdapterStack(2, 64, 48, 16, device="cpu")
+    return stack, lora.adapter_plan([0, 1, -1, 0][:rows], stack)
+
+
+def test_adapters_refuse_results_that_lie_over_other_rows():
+    from crosspool_b200.ops import lora
+
+    s, p = lora_case()
+    b = torch.bfloat16
+    buf, flat, x, y = torch.zeros(5, 128, dtype=b), torch.zeros(1024, dtype=b), torch.zeros(4, 64, dtype=b), torch.zeros(4, 48, dtype=b)
+    side = flat.as_strided((4, 64), (80, 1))                        # 64 of every 80 columns
+    for yy, xx, out in ((buf[:4, :48], x, buf[:4, 16:64]), (buf[:4, :48], x, buf[1:, :48]), (buf[1:, :48], x, buf[:4, :48]), (y, buf[:4, :64], buf[:4, 56:104]),
+                        (y, buf[:4, :64], buf[1:, :48]), (y, buf[:4, 64:], buf[:4, 64:112]), (y, side, flat.as_strided((4, 48), (64, 1), 64)),
+                        (y, side, flat.as_strided((4, 48), (80, 1), 72))):
+        with pytest.raises(ValueError, match="over"):
+            lora.lora_add(yy, xx, s, p, out=out)
+    for yy, xx, out in ((y, x, y), (buf[:4, :48], x, buf[:4, :48]), (buf[:4, :48], buf[:4, 64:], buf[:4, :48]), (y, buf[:4, :64], buf[:4, 64:112]),
+                        (buf[:4, :48], x, buf[:4, 48:96]), (y, side, flat.as_strided((4, 48), (64, 1), 512))):
+        with pytest.raises(ValueError, match="GPU"):
+            lora.lora_add(yy, xx, s, p, out=out)
+    one, plan = lora_case(1)
+    with pytest.raises(ValueError, match="over"):
+        lora.lora_add(buf[:1, :48], x[:1], one, plan, out=buf[:1, 40:88])
+    with pytest.raises(ValueError, match="GPU"):
+        lora.lora_add(buf[:1, :48], x[:1], one, plan, out=buf[:1, 48:96])
