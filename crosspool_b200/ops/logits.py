@@ -13,6 +13,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import native
+from .overlap import rows_meet
 
 _INT, _FLOAT = torch.int32, torch.float32
 MAX_VOCAB = 1 << 20
@@ -129,7 +130,7 @@ def _launch(controls: LogitControls, call: bytes, dev) -> None:
 
 def adjust_logits(logits: torch.Tensor, controls: LogitControls, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """The logits after ``controls``, rounded once to ``out``'s type (bf16 or fp32; by default the logits' own). ``out`` may be
-    ``logits`` itself."""
+    ``logits`` itself, or rows that none of theirs lies over."""
     rows, vocab, ld, f32 = _check(logits, controls)
     if out is None:
         out = torch.empty_like(logits)
@@ -143,6 +144,9 @@ def adjust_logits(logits: torch.Tensor, controls: LogitControls, *, out: torch.T
     at, to = logits.data_ptr(), out.data_ptr()
     if at == to and (out.dtype is not logits.dtype or ld_out != ld):
         raise ValueError("adjusting in place keeps type and pitch")
+    size, size_out = logits.element_size(), out.element_size()
+    if at != to and rows_meet(rows, at, size * ld, size * vocab, to, size_out * ld_out, size_out * vocab):
+        raise ValueError("out may be the logits themselves, but must not lie over other rows of them")
     _launch(controls, _CALL.pack(at, to, 0, 0, 0, 0, rows, vocab, ld, ld_out, f32, out.dtype is _FLOAT), logits.device)
     return out
 

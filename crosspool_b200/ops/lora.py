@@ -170,7 +170,8 @@ def adapter_plan(index: Sequence[int], stack: "AdapterStack | int", device: str 
 
 def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: AdapterPlan, *, out: torch.Tensor | None = None) -> torch.Tensor:
     """``y[rows, out] + scale * (x[rows, in] @ A.T) @ B.T`` with every row's own adapter, rounded once; sums in fp32. ``out`` may
-    be ``y`` itself, or rows that no row of ``x`` or ``y`` lies over. bf16; rows may have a pitch (a multiple of 8 elements), so that a slice of a wider buffer can be read or written."""
+    be ``y`` itself, or rows that no row of ``x`` or ``y`` lies over. bf16; rows may have a pitch (a multiple of 8 elements), so that a
+    slice of a wider buffer can be read or written."""
     rows = x.shape[0]
     if out is None:
         out = torch.empty_like(y)

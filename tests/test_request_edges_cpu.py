@@ -324,3 +324,16 @@ def test_adapters_refuse_results_that_lie_over_other_rows():
         lora.lora_add(buf[:1, :48], x[:1], one, plan, out=buf[:1, 40:88])
     with pytest.raises(ValueError, match="GPU"):
         lora.lora_add(buf[:1, :48], x[:1], one, plan, out=buf[:1, 48:96])
+
+
+def test_adjusted_logits_refuse_results_that_lie_over_other_rows():
+    from crosspool_b200.ops import logits as L
+
+    none, z, b = L.LogitControls(), torch.zeros(5, 100), torch.zeros(5, 200, dtype=torch.bfloat16)
+    for x, out in ((z[:4], z[1:]), (z[1:], z[:4]), (z[:, :60], z[:, 40:]), (b[:4, :100], b.view(torch.float32)[1:]), (z[:1, :60], z[:1, 40:]),
+                   (z.view(torch.bfloat16)[:, 100:], z)):
+        with pytest.raises(ValueError, match="over|in place"):
+            L.adjust_logits(x, none, out=out)
+    for x, out in ((z, z), (z[:2], z[2:4]), (z[:, :50], z[:, 50:]), (b[:4, :100], torch.zeros(4, 100)), (b[:, :100], b[:, 100:]), (z[:, 1:50], z[:, 51:])):
+        with pytest.raises(ValueError, match="GPU"):
+            L.adjust_logits(x, none, out=out)
