@@ -272,7 +272,7 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                         scale: float | None = None) -> torch.Tensor:
     """:func:`paged_decode` for a batch whose rows share prefixes: every prefix of ``plan`` is read and multiplied once for all rows
     of its group (``csrc/kernels/shared_prefix.cu``), then each row adds its own tokens. ``seq_lens`` count prefix and own tokens; a
-    row of fewer tokens than its group's prefix reads all of them on its own. Rows without tokens give zeros."""
+    row of fewer tokens than its group's prefix reads all of them on its own. Rows without tokens give zeros. ``out`` may be ``q``."""
     batch, q_heads, d = q.shape
     pages, page, kv_heads, kv_d = kv_shape = k_cache.shape
     if (q_heads, kv_heads, d, d) != (plan.q_heads, plan.kv_heads, plan.head_dim, kv_d) or v_cache.shape != kv_shape:
@@ -315,6 +315,8 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise ValueError("out and the workspace must be 16-byte aligned")
     if not batch:
         return out
+    if at_out != at_q and abs(at_out - at_q) < 2 * batch * q_heads * d:
+        raise ValueError("out may be q, but must not lie over other rows of it")
     if dev.type != "cuda":
         raise ValueError("the kernel runs on a GPU")
     if not pages:

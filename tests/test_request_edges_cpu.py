@@ -337,3 +337,22 @@ def test_adjusted_logits_refuse_results_that_lie_over_other_rows():
     for x, out in ((z, z), (z[:2], z[2:4]), (z[:, :50], z[:, 50:]), (b[:4, :100], torch.zeros(4, 100)), (b[:, :100], b[:, 100:]), (z[:, 1:50], z[:, 51:])):
         with pytest.raises(ValueError, match="GPU"):
             L.adjust_logits(x, none, out=out)
+
+
+@pytest.mark.parametrize("prefixes", [[64], []])
+def test_shared_prefix_attention_refuses_results_that_lie_over_other_queries(prefixes):
+    from crosspool_b200.ops import attention as A
+
+    bf, i32 = torch.bfloat16, torch.int32
+    buf = torch.zeros(5 * 8 * 128, dtype=bf)
+    rest = dict(k_cache=torch.zeros(9, 16, 2, 128, dtype=bf), v_cache=torch.zeros(9, 16, 2, 128, dtype=bf), block_table=torch.zeros(4, 8, dtype=i32),
+                seq_lens=torch.zeros(4, dtype=i32))
+    rest["plan"] = A.shared_prefix_plan([4] if prefixes else [], prefixes, rows=4, q_heads=8, kv_heads=2, head_dim=128, max_len=128, device="cpu")
+    q = buf[:4096].view(4, 8, 128)
+    for out in (buf[1024:].view(4, 8, 128), buf[8:4104].view(4, 8, 128)):
+        for a, b in ((q, out), (out, q)):
+            with pytest.raises(ValueError, match="over"):
+                A.paged_decode_shared(a, out=b, **rest)
+    for out in (q, torch.zeros_like(q)):
+        with pytest.raises(ValueError, match="GPU"):
+            A.paged_decode_shared(q, out=out, **rest)
