@@ -178,11 +178,16 @@ class TokenControls:
         return self.repetition != 1.0 or self.frequency != 0.0 or self.presence != 0.0
 
     def check(self, vocab: int, most_biases: int) -> None:
-        if not self.repetition > 0:
-            raise ValueError(f"repetition penalty {self.repetition} is not positive")
-        for v in (self.repetition, self.frequency, self.presence, *self.bias.values()):
-            if not np.isfinite(v):
-                raise ValueError(f"control {v} is not finite")
+        # as the kernel gets them, in 32 bits
+        try:
+            with np.errstate(over="ignore", under="ignore"):
+                values = np.array([self.repetition, self.frequency, self.presence, *self.bias.values()], dtype=np.float64).astype(np.float32)
+        except (TypeError, ValueError, OverflowError) as e:
+            raise ValueError(f"controls must be numbers: {e}") from None
+        if not values[0] > 0:
+            raise ValueError(f"repetition penalty {self.repetition} is not positive in 32 bits")
+        if not np.isfinite(values).all():
+            raise ValueError(f"a control of {values[~np.isfinite(values)][0]} in 32 bits")
         if len(self.bias) > most_biases:
             raise ValueError(f"{len(self.bias)} biases: up to {most_biases} are supported")
         if any(not 0 <= t < vocab for t in self.bias):

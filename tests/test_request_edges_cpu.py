@@ -356,3 +356,26 @@ def test_shared_prefix_attention_refuses_results_that_lie_over_other_queries(pre
     for out in (q, torch.zeros_like(q)):
         with pytest.raises(ValueError, match="GPU"):
             A.paged_decode_shared(q, out=out, **rest)
+
+
+# ------------------------------------------------------------------------------------------------ controls of a request
+
+@pytest.mark.parametrize("kw", [dict(repetition=1e-60), dict(repetition=1e39), dict(frequency=1e39), dict(presence=-1e39), dict(bias={1: 1e300}),
+                                dict(repetition=10 ** 400), dict(bias={1: -10 ** 400}), dict(repetition="x"), dict(frequency=None)])
+@pytest.mark.filterwarnings("error")
+def test_controls_that_32_bits_do_not_hold_are_refused(kw):
+    from crosspool_b200.engine.atn_engine import EngineConfig
+    from crosspool_b200.engine.request_options import TokenControls
+
+    eng = bare_engine()
+    eng.ecfg = EngineConfig(controls=True)
+    with pytest.raises(ValueError):
+        eng.add_request([1, 2], 4, controls=TokenControls(**kw))
+    assert not eng.waiting
+
+
+def test_controls_that_32_bits_hold_are_taken():
+    from crosspool_b200.engine.request_options import TokenControls
+
+    TokenControls(1e-30, 3e38, -3e38, {5: 3.4e38, 6: 1e-45}).check(40, 300)
+    TokenControls(np.float64(1.5), np.float32(0.1), 1, {5: np.float16(2)}).check(40, 300)
