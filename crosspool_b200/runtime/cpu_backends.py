@@ -247,7 +247,9 @@ class CpuOracleEngine:
         self.capacity.publish_demand(missing_pages, deadline)
 
     def add_request(self, prompt: list[int], max_new_tokens: int, arrival: float | None = None, deadline: float = 0.0,
-                    temperature: float = 0.0, seed: int = 0) -> Sequence:
+                    temperature: float = 0.0, seed: int = 0, controls=None, adapter: str | None = None) -> Sequence:
+        if controls is not None or adapter is not None:
+            raise ValueError("the CPU engine has no controls and no adapters")
         if len(prompt) == 0:
             raise ValueError("empty prompt")
         if max_new_tokens < 1:

@@ -379,3 +379,46 @@ def test_controls_that_32_bits_hold_are_taken():
 
     TokenControls(1e-30, 3e38, -3e38, {5: 3.4e38, 6: 1e-45}).check(40, 300)
     TokenControls(np.float64(1.5), np.float32(0.1), 1, {5: np.float16(2)}).check(40, 300)
+
+
+# ------------------------------------------------------------------------------------------------ HTTP
+
+def ask(loop, models, bodies):
+    """Status codes and answers of ``POST /generate`` with ``bodies``."""
+    import asyncio
+
+    import httpx
+
+    from crosspool_b200.runtime.serving import create_serving_app
+
+    app = create_serving_app(loop, models)
+
+    async def go():
+        async with httpx.AsyncClient(transport=httpx.ASGITransport(app=app), base_url="http://t") as c:
+            return [await c.post("/generate", json={"input_ids": [1, 2], "max_new_tokens": 2, **b}) for b in bodies]
+
+    return [(r.status_code, r.json()) for r in asyncio.run(go())]
+
+
+def served(loop, bodies):
+    loop.start()
+    try:
+        return ask(loop, ["m"], bodies)
+    finally:
+        loop.stop()
+
+
+def test_the_cpu_engine_answers_requests_with_options():
+    """Options that it does not have are the request's fault, not the server's."""
+    from crosspool_b200.models import config as mc
+    from crosspool_b200.models.weights import random_attention_weights, random_ffn_weights
+    from crosspool_b200.models import reference
+    from crosspool_b200.runtime.cpu_backends import CpuDeployment, CpuOracleEngine
+    from crosspool_b200.runtime.serving import EngineLoop
+
+    cfg = mc.preset("Qwen/Qwen3-0.6B").with_layers(1)
+    aw, fw = random_attention_weights(cfg, 1, "cpu", torch.float32), random_ffn_weights(cfg, 1, "cpu", torch.float32)
+    loop = EngineLoop(CpuDeployment({"m": CpuOracleEngine(cfg, aw, None, model=reference.ReferenceModel(cfg, aw, fw))}))
+    got = served(loop, [{"repetition_penalty": 1.3}, {"frequency_penalty": 0.2}, {"logit_bias": {"5": 1.0}}, {"adapter": "x"}])
+    assert [c for c, _ in got] == [422] * 4 and all("CPU engine" in b["detail"] for _, b in got)
+    assert loop.error is None
