@@ -194,20 +194,21 @@ class GenerateRequest(BaseModel):
     stream: bool = False
     temperature: float = 0.0
     seed: int = 0
-    # of engines with controls (EngineConfig.controls) and adapters
-    repetition_penalty: float = 1.0
-    frequency_penalty: float = 0.0
-    presence_penalty: float = 0.0
-    logit_bias: dict[int, float] = {}
+    # of engines with controls (EngineConfig.controls) and adapters; null is the neutral value
+    repetition_penalty: Optional[float] = 1.0
+    frequency_penalty: Optional[float] = 0.0
+    presence_penalty: Optional[float] = 0.0
+    logit_bias: Optional[dict[int, float]] = {}
     adapter: Optional[str] = None
 
     def options(self) -> dict:
         """Arguments of the engine's ``add_request`` beside the prompt, none for a plain request."""
         out: dict = {}
-        if self.repetition_penalty != 1.0 or self.frequency_penalty or self.presence_penalty or self.logit_bias:
+        repetition = 1.0 if self.repetition_penalty is None else self.repetition_penalty
+        if repetition != 1.0 or self.frequency_penalty or self.presence_penalty or self.logit_bias:
             from ..engine.request_options import TokenControls
 
-            out["controls"] = TokenControls(self.repetition_penalty, self.frequency_penalty, self.presence_penalty, dict(self.logit_bias))
+            out["controls"] = TokenControls(repetition, self.frequency_penalty or 0.0, self.presence_penalty or 0.0, dict(self.logit_bias or {}))
         if self.adapter is not None:
             out["adapter"] = self.adapter
         return out

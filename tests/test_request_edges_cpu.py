@@ -422,3 +422,16 @@ def test_the_cpu_engine_answers_requests_with_options():
     got = served(loop, [{"repetition_penalty": 1.3}, {"frequency_penalty": 0.2}, {"logit_bias": {"5": 1.0}}, {"adapter": "x"}])
     assert [c for c, _ in got] == [422] * 4 and all("CPU engine" in b["detail"] for _, b in got)
     assert loop.error is None
+
+
+def test_http_fields_that_are_null_are_neutral():
+    """Clients of other servers send null for fields that they leave alone."""
+    from crosspool_b200.runtime.serving import EngineLoop, GenerateRequest
+    from test_serving import FakeDeployment
+
+    nulls = {f: None for f in ("repetition_penalty", "frequency_penalty", "presence_penalty", "logit_bias", "adapter")}
+    assert GenerateRequest.model_validate({"input_ids": [1], **nulls}).options() == {}
+    r = GenerateRequest.model_validate({"input_ids": [1], **nulls, "presence_penalty": 0.5})
+    assert r.options()["controls"].presence == 0.5 and r.options()["controls"].repetition == 1.0
+    got = served(EngineLoop(FakeDeployment()), [nulls, {"logit_bias": None}])
+    assert [(c, b["output_ids"]) for c, b in got] == [(200, [3, 4])] * 2
