@@ -215,6 +215,7 @@ class SharedPrefixPlan:
     a captured graph may be replayed with other words that keep to them. ``max_len`` bounds the sequences' lengths."""
 
     def __init__(self, words: torch.Tensor, rows: int, max_pieces: int, max_parts: int, max_len: int, q_heads: int, kv_heads: int, head_dim: int):
+        _check_heads(q_heads, kv_heads, head_dim)
         _check_size(rows, max_len, kv_heads)
         self.words, self.rows, self.max_pieces, self.max_parts = words, rows, max_pieces, max_parts
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim

@@ -435,3 +435,13 @@ def test_http_fields_that_are_null_are_neutral():
     assert r.options()["controls"].presence == 0.5 and r.options()["controls"].repetition == 1.0
     got = served(EngineLoop(FakeDeployment()), [nulls, {"logit_bias": None}])
     assert [(c, b["output_ids"]) for c, b in got] == [(200, [3, 4])] * 2
+
+
+# ------------------------------------------------------------------------------------------------ plans
+
+@pytest.mark.parametrize("hq,hk,d", [(34, 2, 128), (8, 2, 96), (7, 2, 64), (8, 0, 64)])
+def test_plans_of_heads_that_no_kernel_takes_are_refused_when_they_are_made(hq, hk, d):
+    from crosspool_b200.ops import attention as A
+
+    with pytest.raises(ValueError, match="heads"):
+        A.SharedPrefixPlan(torch.zeros(A.shared_plan_words(4, 8), dtype=torch.int32), 4, 8, 4, 100, hq, hk, d)
