@@ -503,7 +503,8 @@ decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
   if constexpr (kRows) {
     if (args.softcap > 0.f) cap2 = args.softcap * 1.4426950408889634f, capx = 2.f * sscale / args.softcap;
   }
-  float m0 = kSig ? 0.f : -CUDART_INF_F, m1 = m0, l0 = 0.f, l1 = 0.f;
+  // (the lowest finite number, not -inf: keys that hold an infinity may leave no score above -inf so far, and weigh nothing then)
+  float m0 = kSig ? 0.f : -CUDART_MAX_NORMAL_F, m1 = m0, l0 = 0.f, l1 = 0.f;
   float b0 = 0.f, b1 = 0.f;                            // biases of rows g and g + 8, log2 domain
   if constexpr (kSig) {
     if (g < G) b0 = args.sigmoid_bias[hk * G + g] * 1.4426950408889634f;
@@ -595,7 +596,7 @@ decode_attn_tc_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_c
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
     mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-    const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);  // finite: every tile has a valid token
+    const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
     if (__any_sync(0xffffffffu, n0 > m0 || n1 > m1)) {
       const float c0 = exp2f(m0 - n0), c1 = exp2f(m1 - n1);
       l0 *= c0;

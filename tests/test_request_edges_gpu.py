@@ -147,3 +147,39 @@ def test_requests_whose_mask_fails_leave_the_engine_with_all_they_held(mixed):
     assert loop.error is None and not eng.has_work and not eng.control_rows.slots and len(eng.control_rows.free) == 8
     eng.kv.allocator.free(eng.prefix.evict(10 ** 6))
     assert eng.kv.allocator.free_pages == full and not eng.kv.tables
+
+
+# ------------------------------------------------------------------------------------------------ shared prefixes, infinities
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows,lens", [(3, [90, 41, 300]), (200, [90, 41, 300, 57]), (3, [700, 1500, 900])])
+def test_keys_of_minus_infinity_weigh_nothing_where_no_rows_share(rows, lens, d):
+    """The first 40 tokens of every row have scores of -inf; with long rows the first of several slices begins with them."""
+    from crosspool_b200.ops import attention as A
+    from crosspool_b200.ops import gemm
+
+    q, k, v, table = cache(rows, 1500, 8, 2, d, 16, seed=d)
+    n = torch.tensor([lens[r % len(lens)] for r in range(rows)], dtype=torch.int32, device="cuda")
+    q = q.abs()
+    for r in range(rows):
+        k[table[r, 0:2].long(), :, :, 5] = float("-inf")
+        k[table[r, 2].long(), :8, :, 5] = float("-inf")
+    plan = A.shared_prefix_plan([], [], rows=rows, q_heads=8, kv_heads=2, head_dim=d, max_len=int(n.max()))
+    for got in (A.paged_decode_shared(q, k, v, table, n, plan), A.paged_decode(q, k, v, table, n, max_len=1500)):
+        gemm.check_status(q.device)
+        close(got, q, k, v, table, n)
+
+
+@pytest.mark.parametrize("sizes,prefixes", [([], []), ([5], [320])])
+@pytest.mark.parametrize("tokens", [400, 2000])
+def test_results_may_lie_over_their_queries(sizes, prefixes, tokens):
+    from crosspool_b200.ops import attention as A
+    from crosspool_b200.ops import gemm
+
+    q, k, v, table = cache(9, tokens, 8, 2, 128, 16)
+    table[1:sum(sizes), :20] = table[:1, :20]
+    n = torch.tensor([tokens - 7 * r for r in range(9)], dtype=torch.int32, device="cuda")
+    plan = A.shared_prefix_plan(sizes, prefixes, rows=9, q_heads=8, kv_heads=2, head_dim=128, max_len=tokens)
+    want = A.paged_decode_shared(q, k, v, table, n, plan)
+    assert A.paged_decode_shared(q, k, v, table, n, plan, out=q) is q and torch.equal(q, want)
+    gemm.check_status(q.device)
