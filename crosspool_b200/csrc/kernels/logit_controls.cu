@@ -22,6 +22,7 @@
 #include <utility>
 
 #include "xpool/elem.cuh"
+#include "xpool/gumbel.cuh"
 #include "xpool/pdl.cuh"
 #include "xpool/request_api.h"
 
@@ -35,16 +36,6 @@ constexpr uint32_t kInPrompt = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3f
 constexpr int kMaxRanks = 8;
 constexpr int kBatch = 4;                          // loads of a thread in flight (kSlots is a multiple of 1024 * kBatch)
 constexpr int kUnit = 1024;                        // shares are multiples of so many tokens
-
-__device__ __forceinline__ uint32_t hash3(uint32_t a, uint32_t b, uint32_t c) {
-  uint64_t x = (static_cast<uint64_t>(a) << 32) ^ (static_cast<uint64_t>(b) * 0x9E3779B97F4A7C15ull) ^ c;
-  x ^= x >> 30;
-  x *= 0xBF58476D1CE4E5B9ull;
-  x ^= x >> 27;
-  x *= 0x94D049BB133111EBull;
-  x ^= x >> 31;
-  return static_cast<uint32_t>(x >> 16);
-}
 
 struct Row {
   const int* history;
@@ -185,10 +176,7 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
   Best best;
   auto key_of = [&](float v, int i) {
     float k = v * w.inv_t;
-    if (w.noisy) {
-      const float u = (static_cast<float>(hash3(w.seed, w.step, static_cast<uint32_t>(i)) >> 8) + 0.5f) * (1.f / 16777216.f);
-      k -= __logf(-__logf(u));
-    }
+    if (w.noisy) k -= gumbel::minus_noise(w.seed, w.step, static_cast<uint32_t>(i));
     return k;
   };
 

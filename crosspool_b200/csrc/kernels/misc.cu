@@ -6,6 +6,7 @@
 #include <utility>
 
 #include "xpool/api.h"
+#include "xpool/gumbel.cuh"
 #include "xpool/pdl.cuh"
 #include "xpool/sm100.cuh"
 
@@ -86,19 +87,7 @@ argmax_kernel(const T* logits, int* out, int vocab, int ld, int wide, int ranks)
   if (threadIdx.x == 0) out[at] = bi;
 }
 
-// Temperature sampling by the Gumbel-max trick: argmax_i (logit_i / T + g_i) with g_i = -log(-log u_i) draws
-// from softmax(logits / T) exactly, in one pass and without normalising. u_i comes from a counter-based hash
-// of (row seed, token index), so a (seed, step) pair always yields the same token. T <= 0 is greedy.
-__device__ __forceinline__ uint32_t hash3(uint32_t a, uint32_t b, uint32_t c) {
-  uint64_t x = (static_cast<uint64_t>(a) << 32) ^ (static_cast<uint64_t>(b) * 0x9E3779B97F4A7C15ull) ^ c;
-  x ^= x >> 30;
-  x *= 0xBF58476D1CE4E5B9ull;
-  x ^= x >> 27;
-  x *= 0x94D049BB133111EBull;
-  x ^= x >> 31;
-  return static_cast<uint32_t>(x >> 16);
-}
-
+// Temperature sampling by the Gumbel-max trick (gumbel.cuh). T <= 0 is greedy.
 template <typename T>
 __global__ void __launch_bounds__(1024)
 sample_kernel(const T* __restrict__ logits, const float* __restrict__ temps, const uint32_t* __restrict__ seeds,
@@ -113,10 +102,7 @@ sample_kernel(const T* __restrict__ logits, const float* __restrict__ temps, con
   int bi = 0x7fffffff;
   for (int i = threadIdx.x; i < vocab; i += 1024) {
     float v = to_f<T>(row[i]) * inv_t;
-    if (temp > 0.f) {
-      const float u = (static_cast<float>(hash3(seed, step, static_cast<uint32_t>(i)) >> 8) + 0.5f) * (1.f / 16777216.f);
-      v -= __logf(-__logf(u));
-    }
+    if (temp > 0.f) v -= xpool::gumbel::minus_noise(seed, step, static_cast<uint32_t>(i));
     if (v > best || (v == best && i < bi)) {
       best = v;
       bi = i;

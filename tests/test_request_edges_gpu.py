@@ -183,3 +183,43 @@ def test_results_may_lie_over_their_queries(sizes, prefixes, tokens):
     want = A.paged_decode_shared(q, k, v, table, n, plan)
     assert A.paged_decode_shared(q, k, v, table, n, plan, out=q) is q and torch.equal(q, want)
     gemm.check_status(q.device)
+
+
+# ------------------------------------------------------------------------------------------------ draws
+
+def highest_hashes(rows, vocab, steps):
+    """(row, step, token) of the draws whose noise comes from the last of 2^24 steps (``csrc/include/xpool/gumbel.cuh``)."""
+    import numpy as np
+
+    out = []
+    with np.errstate(over="ignore"):
+        for step in range(steps):
+            a, c = np.arange(rows, dtype=np.uint64)[:, None] << np.uint64(32), np.arange(vocab, dtype=np.uint64)[None]
+            x = a ^ (np.uint64(step) * np.uint64(0x9E3779B97F4A7C15)) ^ c
+            x ^= x >> np.uint64(30)
+            x *= np.uint64(0xBF58476D1CE4E5B9)
+            x ^= x >> np.uint64(27)
+            x *= np.uint64(0x94D049BB133111EB)
+            x ^= x >> np.uint64(31)
+            r, t = np.nonzero(((x >> np.uint64(16)) & np.uint64(0xFFFFFFFF)) >> np.uint64(8) == np.uint64(0xFFFFFF))
+            out += [(int(i), step, int(j)) for i, j in zip(r, t)]
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_no_noise_draws_a_token_that_has_no_weight(dtype):
+    """Every draw's highest noise is finite: a token 100 below another one at temperature 1 has a chance of e^-100."""
+    from crosspool_b200.ops import attention as A
+    from crosspool_b200.ops import logits as L
+
+    rows, vocab = 64, 4096
+    hits = highest_hashes(rows, vocab, 400)                          # 6 are expected of 10^8 draws
+    assert len(hits) >= 2
+    temps = torch.ones(rows, device="cuda")
+    for row, step, token in hits:
+        x = torch.full((rows, vocab), -50.0, device="cuda", dtype=dtype)
+        best = (token + 7) % vocab
+        x[:, best] = 50.0
+        seeds = torch.stack([torch.arange(rows), torch.full((rows,), step)], 1).int().cuda()
+        for got in (A.sample(x, temps, seeds), L.select_tokens(x, L.LogitControls(), temps, seeds)):
+            assert (got == best).all(), (row, step, token)
