@@ -19,6 +19,7 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <utility>
 
 #include "xpool/elem.cuh"
@@ -402,7 +403,7 @@ logit_controls_kernel(XpLogitArgs a, int wide, int ranks, int share) {
 
 template <auto kernel, int kThreads>
 static int go(const XpLogitArgs& a, int wide, int ranks, int share, int smem, cudaStream_t s) {
-  static uint64_t allowed = 0;                       // devices on which the kernel may have the shared memory
+  static std::atomic<uint64_t> allowed{0};           // devices on which the kernel may have the shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -21;
   if ((allowed >> (dev & 63) & 1) == 0) {

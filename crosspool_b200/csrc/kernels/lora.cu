@@ -17,6 +17,7 @@
 // the result's. Sums are fp32.
 #include <cooperative_groups.h>
 
+#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -354,7 +355,7 @@ lora_kernel(XpLoraArgs a, int ranks) {
 template <int kTiles>
 static int launch(const XpLoraArgs& a, int ranks, cudaStream_t s) {
   const int smem = smem_bytes(a.parts * a.rank, ranks, region_bytes<kTiles>());
-  static uint64_t allowed = 0;                       // devices on which the kernel may have the shared memory
+  static std::atomic<uint64_t> allowed{0};           // devices on which the kernel may have the shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -21;
   if ((allowed >> (dev & 63) & 1) == 0) {

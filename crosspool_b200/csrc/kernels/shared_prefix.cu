@@ -29,6 +29,8 @@
 // behind a common barrier.
 #include <math_constants.h>
 
+#include <atomic>
+
 #include "xpool/mma_sync.cuh"
 #include "xpool/pdl.cuh"
 #include "xpool/request_api.h"
@@ -815,7 +817,7 @@ shared_merge_kernel(XpDecodeSharedArgs args, int G) {
 
 // Shared memory above the default is asked for once per device and kernel.
 template <typename K>
-static int allow_smem(K kernel, int bytes, uint64_t& done) {
+static int allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -21;
   const uint64_t bit = 1ull << (dev & 63);
@@ -839,7 +841,7 @@ static int launch(const XpDecodeSharedArgs& args, cudaStream_t s) {
   constexpr int kTiles = 2 * (D / 64) * kRows * 128 + kStages * 2 * (D / 64) * kBN * 128, kRings = kWarps * ring_of<D>() * 16 * D * 4;
   constexpr int kSmem = (kTiles > kRings ? kTiles : kRings) + (2 * XP_PREFIX_ROWS + 1) * 4 + 1024;
   static_assert(kSmem + sizeof(Bars) <= 227 * 1024, "tiles exceed the shared memory of an SM");
-  static uint64_t allowed = 0;
+  static std::atomic<uint64_t> allowed{0};
   if (const int rc = allow_smem(shared_prefix_kernel<D>, kSmem, allowed); rc != 0) return rc;
   pdl::launch(shared_prefix_kernel<D>, 148, kThreads, kSmem, s, 1, mq, mk, mv, mk16, mv16, args, G, box_tokens);
   pdl::launch(shared_merge_kernel<D>, dim3(a.kv_heads, a.batch), kMergeThreads, 0, s, 1, args, G);

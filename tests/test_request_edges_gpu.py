@@ -223,3 +223,55 @@ def test_no_noise_draws_a_token_that_has_no_weight(dtype):
         seeds = torch.stack([torch.arange(rows), torch.full((rows,), step)], 1).int().cuda()
         for got in (A.sample(x, temps, seeds), L.select_tokens(x, L.LogitControls(), temps, seeds)):
             assert (got == best).all(), (row, step, token)
+
+
+# ------------------------------------------------------------------------------------------------ host threads
+
+FIRST_CALLS = """
+import sys, threading
+import torch
+from crosspool_b200.ops import attention as A, logits as L, lora
+
+torch.manual_seed(0)
+rows = 6
+q = torch.randn(rows, 8, 128, device="cuda").bfloat16()
+k, v = (torch.randn(rows * 8, 16, 2, 128, device="cuda").bfloat16() for _ in range(2))
+table = torch.arange(rows * 8, dtype=torch.int32, device="cuda").view(rows, 8)
+table[:, :4] = table[0, :4]
+lens = torch.full((rows,), 100, dtype=torch.int32, device="cuda")
+plan = A.shared_prefix_plan([rows], [64], rows=rows, q_heads=8, kv_heads=2, head_dim=128, max_len=128)
+stack = lora.AdapterStack(1, 256, 512, 16)
+stack.load(0, torch.randn(16, 256, device="cuda"), torch.randn(512, 16, device="cuda"))
+adapters = lora.adapter_plan([0] * rows, stack)
+x, y, z = torch.randn(rows, 256, device="cuda").bfloat16(), torch.randn(rows, 512, device="cuda").bfloat16(), torch.randn(rows, 9000, device="cuda")
+none = L.LogitControls()
+torch.cuda.synchronize()
+got, start = [None] * 4, threading.Barrier(4)
+
+
+def work(i):
+    out = []
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        for _ in range(50):
+            out = [A.paged_decode_shared(q, k, v, table, lens, plan), lora.lora_add(y, x, stack, adapters), L.select_tokens(z, none), L.adjust_logits(z, none)]
+        torch.cuda.current_stream().synchronize()
+    got[i] = out
+
+
+threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+want = [A.paged_decode_shared(q, k, v, table, lens, plan), lora.lora_add(y, x, stack, adapters), L.select_tokens(z, none), L.adjust_logits(z, none)]
+sys.exit(0 if all(g is not None and all(torch.equal(a, b) for a, b in zip(g, want)) for g in got) else 1)
+"""
+
+
+def test_first_calls_of_four_threads_at_once():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parent.parent
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stderr[-2000:]
