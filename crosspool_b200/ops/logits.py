@@ -132,7 +132,8 @@ def adjust_logits(logits: torch.Tensor, controls: LogitControls, *, out: torch.T
     """The logits after ``controls``, rounded once to ``out``'s type (bf16 or fp32; by default the logits' own). ``out`` may be
     ``logits`` itself, or rows that none of theirs lies over."""
     rows, vocab, ld, f32 = _check(logits, controls)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty_like(logits)
     if out.shape != logits.shape or out.dtype not in (torch.bfloat16, _FLOAT) or out.stride(1) != 1 or out.device != logits.device:
         raise ValueError("out must be bf16 or fp32 of the logits' shape, with contiguous rows, on their device")
@@ -145,7 +146,7 @@ def adjust_logits(logits: torch.Tensor, controls: LogitControls, *, out: torch.T
     if at == to and (out.dtype is not logits.dtype or ld_out != ld):
         raise ValueError("adjusting in place keeps type and pitch")
     size, size_out = logits.element_size(), out.element_size()
-    if at != to and rows_meet(rows, at, size * ld, size * vocab, to, size_out * ld_out, size_out * vocab):
+    if not fresh and at != to and rows_meet(rows, at, size * ld, size * vocab, to, size_out * ld_out, size_out * vocab):
         raise ValueError("out may be the logits themselves, but must not lie over other rows of them")
     _launch(controls, _CALL.pack(at, to, 0, 0, 0, 0, rows, vocab, ld, ld_out, f32, out.dtype is _FLOAT), logits.device)
     return out

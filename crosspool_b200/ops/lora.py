@@ -172,8 +172,8 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: Adapte
     """``y[rows, out] + scale * (x[rows, in] @ A.T) @ B.T`` with every row's own adapter, rounded once; sums in fp32. ``out`` may
     be ``y`` itself, or rows that no row of ``x`` or ``y`` lies over. bf16; rows may have a pitch (a multiple of 8 elements), so that a
     slice of a wider buffer can be read or written."""
-    rows = x.shape[0]
-    if out is None:
+    rows, fresh = x.shape[0], out is None
+    if fresh:
         out = torch.empty_like(y)
     if x.shape != (rows, stack.in_features) or y.shape != (rows, stack.out_features) or out.shape != y.shape:
         raise ValueError(f"x {tuple(x.shape)}, y {tuple(y.shape)}, out {tuple(out.shape)} beside a {stack.in_features} -> {stack.out_features} stack")
@@ -192,7 +192,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, stack: AdapterStack, plan: Adapte
     if plan.words.device != dev:
         raise ValueError("the plan lives on another device")
     wide = 2 * stack.out_features
-    if rows and ((at_out != at_y and rows_meet(rows, at_out, 2 * ld_out, wide, at_y, 2 * ld_y, wide))
+    if not fresh and ((at_out != at_y and rows_meet(rows, at_out, 2 * ld_out, wide, at_y, 2 * ld_y, wide))
                  or rows_meet(rows, at_out, 2 * ld_out, wide, at_x, 2 * ld_x, 2 * stack.in_features)):
         raise ValueError("out may be y, but not x, and lie over neither")
     if dev.type != "cuda":
