@@ -275,3 +275,58 @@ def test_first_calls_of_four_threads_at_once():
     root = Path(__file__).resolve().parent.parent
     done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=120)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+# ------------------------------------------------------------------------------------------------ calls that the documentation allows
+
+@pytest.mark.parametrize("hq,hk,d", [(14, 2, 64), (32, 8, 128)])
+@pytest.mark.parametrize("parts", [1, 8, 32])
+def test_long_prefixes_in_few_pieces(hq, hk, d, parts):
+    """Plans of few pieces, as an engine's captured steps bound them, and more rows in the call than in the plan."""
+    from crosspool_b200.ops import attention as A
+    from crosspool_b200.ops import gemm
+
+    rows, prefix, extra = 4, 20000, 2
+    q, k, v, table = cache(rows + extra, prefix + 96, hq, hk, d, 32, seed=parts)
+    table[1:rows, :prefix // 32] = table[0, :prefix // 32]
+    words = torch.zeros(A.shared_plan_words(rows, 40), dtype=torch.int32)
+    count, most = A.fill_shared_plan([rows], [prefix], words.numpy(), rows, 40, parts, q_heads=hq, kv_heads=hk, head_dim=d, own_tokens=200)
+    assert 1 <= most <= parts and count == most
+    plan = A.SharedPrefixPlan(words.cuda(), rows, 40, parts, prefix + 96, hq, hk, d)
+    lens = torch.tensor([prefix + 1, prefix + 96, prefix, prefix - 1, 33, 19000], dtype=torch.int32, device="cuda")
+    got = A.paged_decode_shared(q, k, v, table, lens, plan)
+    gemm.check_status(q.device)
+    close(got, q, k, v, table, lens)
+
+
+def test_rows_of_one_table():
+    """Every row reads the same sequence, through a table that is there once."""
+    from crosspool_b200.ops import attention as A
+    from crosspool_b200.ops import gemm
+
+    q, k, v, table = cache(70, 400, 8, 2, 128, 16)
+    one = table[:1].expand(70, -1)
+    lens = torch.full((70,), 400, dtype=torch.int32, device="cuda")
+    plan = A.shared_prefix_plan([70], [400], rows=70, q_heads=8, kv_heads=2, head_dim=128, max_len=400)
+    got = A.paged_decode_shared(q, k, v, one, lens, plan)
+    gemm.check_status(q.device)
+    close(got, q, k, v, one, lens)
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_selected_tokens_go_where_the_latest_ones_came_from(rows):
+    """A decode loop whose tokens of a step are the latest ones of the next."""
+    from crosspool_b200.ops import logits as L
+
+    vocab, steps = 9000, 5
+    tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    history = torch.full((rows, steps + 2), -1, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    c = L.LogitControls(history=history, lens=lens, latest=tokens, presence=torch.full((rows,), 100.0, device="cuda"))
+    x = torch.randn(rows, vocab, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    want = x.topk(steps, dim=1).indices.int()                         # the penalty keeps every token from coming twice
+    for step in range(steps):
+        L.select_tokens(x, c, out=tokens)
+        assert torch.equal(tokens, want[:, step])
+        lens += 1
+    assert torch.equal(history[:, :steps - 1], want[:, :steps - 1])
