@@ -299,6 +299,8 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype is not bf16 or not out.is_contiguous() or out.device != dev:
         raise ValueError("out must be like q")
+    elif 0 < abs(out.data_ptr() - at_q) < 2 * batch * q_heads * d:
+        raise ValueError("out may be q, but must not lie over other rows of it")
     if scale is None:
         scale = d ** -0.5
     elif not 0 < scale < math.inf:
@@ -316,8 +318,6 @@ def paged_decode_shared(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         raise ValueError("out and the workspace must be 16-byte aligned")
     if not batch:
         return out
-    if at_out != at_q and abs(at_out - at_q) < 2 * batch * q_heads * d:
-        raise ValueError("out may be q, but must not lie over other rows of it")
     if dev.type != "cuda":
         raise ValueError("the kernel runs on a GPU")
     if not pages:
