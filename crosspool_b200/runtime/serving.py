@@ -69,8 +69,9 @@ def _fan_out(items) -> None:
 
 class EngineLoop:
     """``sink``: an in-process consumer called on the loop thread once per engine step with that step's
-    ``[(Pending, (token, finished))]`` and a ``time.perf_counter()`` stamp taken after the step's tokens reached the
-    host; requests submitted with ``queued=False`` are delivered to it alone (no per-request queue)."""
+    ``[(Pending, (token, finished))]`` (an exception in the pair's place ends a request that failed) and a
+    ``time.perf_counter()`` stamp taken after the step's tokens reached the host; requests submitted with ``queued=False``
+    are delivered to it alone (no per-request queue)."""
 
     def __init__(self, deployment: SteppedDeployment, idle_sleep: float = 0.0005, sink=None):
         self.dep = deployment
@@ -134,12 +135,10 @@ class EngineLoop:
             tick()          # idle Instances still answer elastic-KV capacity commands
         time.sleep(self.idle_sleep)
 
-    def _deliver_failed(self, res) -> None:
-        """Requests whose own mask or the like failed are answered with their error; serving goes on."""
-        for model_id, seq, error in getattr(res, "failed", ()):
-            p = self._by_seq.pop((model_id, seq.seq_id), None)
-            if p is not None:
-                p.deliver(error)
+    def _failed(self, res) -> list[tuple[Pending, Exception]]:
+        """Requests that a step dropped because something of their own failed; they are answered with the error, serving goes on."""
+        found = [(self._by_seq.pop((model_id, seq.seq_id), None), error) for model_id, seq, error in getattr(res, "failed", ())]
+        return [(p, error) for p, error in found if p is not None]
 
     def _run(self) -> None:
         try:
@@ -151,7 +150,7 @@ class EngineLoop:
                     continue
                 res = self._step()
                 self.steps += 1
-                batch: list[tuple[Pending, tuple[int, bool]]] = []
+                batch: list[tuple[Pending, tuple[int, bool] | Exception]] = []
                 for model_id, pairs in res.tokens.items():
                     for seq, tok in pairs:
                         p = self._by_seq.get((model_id, seq.seq_id))
@@ -167,10 +166,10 @@ class EngineLoop:
                                     self.metrics.finished(model_id, seq)
                                 except Exception:      # a statistic must never stop the serving loop
                                     pass
+                batch += self._failed(res)         # behind their last tokens
                 if self.sink is not None:
                     self.sink(batch, time.perf_counter())
                 deliver_batch(batch)
-                self._deliver_failed(res)      # behind their last tokens
         except Exception as e:  # device failure: fail every waiting request, stop (fail-stop)
             self.error = e
             for p in self._by_seq.values():

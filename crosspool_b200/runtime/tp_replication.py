@@ -106,7 +106,8 @@ class TpEngineLoop(EngineLoop):
                         self.tokens += 1
                         if done:
                             del self._by_seq[(model_id, seq.seq_id)]
-                self._deliver_failed(res)
+                for p, error in self._failed(res):
+                    p.deliver(error)
         except Exception as e:
             self.error = e
             for p in self._by_seq.values():

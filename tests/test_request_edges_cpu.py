@@ -445,3 +445,32 @@ def test_plans_of_heads_that_no_kernel_takes_are_refused_when_they_are_made(hq, 
 
     with pytest.raises(ValueError, match="heads"):
         A.SharedPrefixPlan(torch.zeros(A.shared_plan_words(4, 8), dtype=torch.int32), 4, 8, 4, 100, hq, hk, d)
+
+
+def test_an_in_process_consumer_hears_of_requests_that_fail():
+    import threading
+
+    from crosspool_b200.deployment import Deployment, InstanceHandle
+    from crosspool_b200.engine.request_options import TokenControls
+    from crosspool_b200.runtime.serving import EngineLoop
+
+    heard, over = [], threading.Event()
+
+    def sink(batch, stamp):
+        heard.extend((p.tag, item) for p, item in batch)
+        if any(isinstance(item, Exception) for _, item in batch):
+            over.set()
+
+    def allowed(g):
+        if len(g) == 2:
+            raise KeyError("grammar")
+        return None
+
+    loop = EngineLoop(Deployment([InstanceHandle("a", None, MaskedEngine())]), sink=sink)
+    loop.submit("a", [1], 5, queued=False, tag="x", options={"controls": TokenControls(allowed=allowed)})
+    loop.start()
+    try:
+        assert over.wait(20)
+    finally:
+        loop.stop()
+    assert [t for t, _ in heard] == ["x"] * 3 and [i for _, i in heard[:2]] == [(0, False), (1, False)] and isinstance(heard[2][1], KeyError)
